@@ -555,6 +555,71 @@ int svb_spectral_norm_fwd(const float* w, float* u, float* v, float* w_sn, float
 int svb_spectral_norm_bwd(const float* dw_sn, const float* w, const float* u, const float* v, const float* sigma, float* dw, int R,
                           int C, float* workspace, void* stream);
 
+/* ==== pieces of a trainable attention block in the conv layout (fp32 or bf16 tensors) ====================================
+ * Tensors are fp32 (SVB_DT_F32) or bf16 (SVB_DT_BF16) as the call's dtype arguments say; every sum, statistic and softmax state is
+ * fp32.  fp32 tensors are multiplied on the matrix cores in three bf16 parts (six products, ~2^-23 per product).                  */
+#define SVB_DT_F32 0
+#define SVB_DT_BF16 1
+
+/* LayerNorm over the channels of x [B][C][T] with everything its gradient needs.  gamma, beta [C] (affine_dtype), either may be
+ * NULL.  mean, rstd [B][T] fp32, both or neither NULL.                                                                            */
+int svb_ln_nct_fwd(const void* x, const void* gamma, const void* beta, void* y, float* mean, float* rstd, int B, int C, int T,
+                   float eps, int dtype, int affine_dtype, void* stream);
+/* dx (dtype), dgamma, dbeta [C] (affine_dtype); any may be NULL.  Fixed order of summation.  ws: svb_ln_nct_bwd_workspace_floats
+ * floats (needed when dgamma or dbeta is wanted).  1 launch, 2 with affine gradients of more than one tile.                       */
+size_t svb_ln_nct_bwd_workspace_floats(int B, int C, int T, int dtype);
+int svb_ln_nct_bwd(const void* x, const void* gamma, const void* dy, const float* mean, const float* rstd, void* dx, void* dgamma,
+                   void* dbeta, float* ws, int B, int C, int T, int dtype, int affine_dtype, void* stream);
+
+/* ---- learned relative-position bias by buckets ----
+ * bucket(o), o = key - query: see csrc/rel_bucket.h.  edge[] ascending, near <= edge[0], near + n_edge + 1 buckets a side.        */
+#define SVB_REL_MAX_BUCKETS 64
+#define SVB_REL_MAX_EDGES 31
+#define SVB_REL_MAX_REACH 1024
+typedef struct SvbRelBuckets {
+    int n_buckets, both, near, n_edge;
+    int edge[SVB_REL_MAX_EDGES];
+} SvbRelBuckets;
+/* bias[h][i][j] = table[bucket(j - (q_start + i))][h];  table [n_buckets][H], bias [H][Tq][Tk], both of `dtype`.                   */
+int svb_bucket_bias_fwd(const void* table, void* bias, const SvbRelBuckets* buckets, int H, int Tq, int Tk, int q_start, int dtype,
+                        void* stream);
+/* dtable[k][h] = sum of dbias[h][i][j] over the pairs of bucket k, fixed order.  ws: svb_bucket_bias_bwd_workspace_floats.         */
+size_t svb_bucket_bias_bwd_workspace_floats(int H, int Tq, int Tk, int n_buckets);
+int svb_bucket_bias_bwd(const void* dbias, void* dtable, const SvbRelBuckets* buckets, float* ws, int H, int Tq, int Tk, int q_start,
+                        int dtype, void* stream);
+
+/* ---- attention with that bias inside ----
+ * out[b][h dk + d][i] = sum_j softmax_j(scale q_i . k_j + table[bucket(j - p_i)][h]) v_j[d],   p_i = start + i,
+ * start = q_start_b[b] where that is given, else q_start.  Keys j with keep[b][j] == 0, and with `causal` those with j > p_i, are
+ * hidden: what K and V hold there has no influence.  A query that sees no key gets zeros and passes no gradient.
+ * Shared heads: H query heads use Hkv key / value heads, query head h reads head h / (H / Hkv).
+ * q [B][H dk][Tq], k, v [B][Hkv dk][Tk]: unit time stride, any batch and channel stride (elements).  dk <= 128.
+ * out, dout, dq [B][H dk][Tq], dk, dv [B][Hkv dk][Tk] contiguous.  table, dtable [n_buckets][H] (table_dtype).
+ * Training: lse [B][H][Tq] and out_f32 (bf16 tensors only: out before its rounding, [B][H dk][Tq]) are written by the forward and
+ * read by the backward; both NULL for inference.                                                                                  */
+typedef struct SvbBucketAttn {
+    const void *q, *k, *v, *table;
+    const float* keep;          /* [B][Tk] or NULL */
+    const int* q_start_b;       /* [B] or NULL */
+    void* out;
+    float *lse, *out_f32;
+    long long q_sb, q_sc, k_sb, k_sc, v_sb, v_sc;
+    int B, H, Hkv, dk, Tq, Tk, q_start, causal, dtype, table_dtype;
+    float scale;
+    SvbRelBuckets buckets;
+} SvbBucketAttn;
+typedef struct SvbBucketAttnGrad {
+    const void* dout;           /* [B][H dk][Tq] contiguous */
+    void *d_q, *d_k, *d_v, *d_table; /* each may be NULL (d_k and d_v both or neither) */
+    float* ws;                  /* svb_bucket_attn_bwd_workspace_floats */
+} SvbBucketAttnGrad;
+/* ws may be NULL where svb_bucket_attn_fwd_workspace_floats says 0.  Few query rows and no lse: the keys are split over workgroups
+ * and joined (ws holds the parts); otherwise one launch of query tiles.                                                            */
+size_t svb_bucket_attn_fwd_workspace_floats(const SvbBucketAttn* a);
+int svb_bucket_attn_fwd(const SvbBucketAttn* a, float* ws, void* stream);
+size_t svb_bucket_attn_bwd_workspace_floats(const SvbBucketAttn* a);
+int svb_bucket_attn_bwd(const SvbBucketAttn* a, const SvbBucketAttnGrad* g, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -78,6 +78,25 @@ class SvbL1Pair(C.Structure):
                 ("scale", C.c_float), ("block0", C.c_int), ("mode", C.c_int), ("target", C.c_float)]
 
 
+SVB_REL_MAX_BUCKETS, SVB_REL_MAX_EDGES, SVB_REL_MAX_REACH = 64, 31, 1024
+SVB_DT_F32, SVB_DT_BF16 = 0, 1
+
+
+class SvbRelBuckets(C.Structure):
+    _fields_ = [(n, C.c_int) for n in ("n_buckets", "both", "near", "n_edge")] + [("edge", C.c_int * SVB_REL_MAX_EDGES)]
+
+
+class SvbBucketAttn(C.Structure):
+    _fields_ = ([(n, C.c_void_p) for n in ("q", "k", "v", "table", "keep", "q_start_b", "out", "lse", "out_f32")] +
+                [(n, C.c_longlong) for n in ("q_sb", "q_sc", "k_sb", "k_sc", "v_sb", "v_sc")] +
+                [(n, C.c_int) for n in ("B", "H", "Hkv", "dk", "Tq", "Tk", "q_start", "causal", "dtype", "table_dtype")] +
+                [("scale", C.c_float), ("buckets", SvbRelBuckets)])
+
+
+class SvbBucketAttnGrad(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("dout", "d_q", "d_k", "d_v", "d_table", "ws")]
+
+
 I, F, P, SZ, I64 = C.c_int, C.c_float, C.c_void_p, C.c_size_t, C.c_int64
 
 # name -> (restype, argtypes)   -- must mirror include/svb_hip.h exactly
@@ -127,6 +146,16 @@ SIGNATURES = {
     "svb_relpos_attn_pos_fwd": (I, [P, P, P, C.c_long, P, P, P, P, P, P, P, I, I, I, I, F, P]),
     "svb_glu_dwconv_bn_swish": (I, [P, P, P, P, P, P, P, F, P, I, I, I, I, P]),
     "svb_layernorm_nct_fwd": (I, [P, P, P, P, I, I, I, F, P]),
+    "svb_ln_nct_fwd": (I, [P, P, P, P, P, P, I, I, I, F, I, I, P]),
+    "svb_ln_nct_bwd_workspace_floats": (SZ, [I, I, I, I]),
+    "svb_ln_nct_bwd": (I, [P, P, P, P, P, P, P, P, P, I, I, I, I, I, P]),
+    "svb_bucket_bias_fwd": (I, [P, P, C.POINTER(SvbRelBuckets), I, I, I, I, I, P]),
+    "svb_bucket_bias_bwd_workspace_floats": (SZ, [I, I, I, I]),
+    "svb_bucket_bias_bwd": (I, [P, P, C.POINTER(SvbRelBuckets), P, I, I, I, I, I, P]),
+    "svb_bucket_attn_fwd_workspace_floats": (SZ, [C.POINTER(SvbBucketAttn)]),
+    "svb_bucket_attn_fwd": (I, [C.POINTER(SvbBucketAttn), P, P]),
+    "svb_bucket_attn_bwd_workspace_floats": (SZ, [C.POINTER(SvbBucketAttn)]),
+    "svb_bucket_attn_bwd": (I, [C.POINTER(SvbBucketAttn), C.POINTER(SvbBucketAttnGrad), P]),
     "svb_layernorm_bwd": (I, [P, P, P, P, P, P, P, P, I, I, I, P]),
     "svb_im2col": (I, [P, P] + [I] * 12 + [C.c_long] * 4 + [P]),
     "svb_col2im": (I, [P, P] + [I] * 12 + [C.c_long] * 2 + [P]),

@@ -1,0 +1,278 @@
+// attn_tiles.h -- tiles, fragments and products shared by bucket_attn_fwd.hip and bucket_attn_bwd.hip.
+//
+// Tensors are in the conv layout: a head's channels are rows, time is contiguous.  The matrix instruction (32x32x16, bf16, fp32
+// accumulate) takes from lane l = (l31 = l & 31, kb = l >> 5) eight consecutive k of row / column l31: k = 8 kb + 0..7.  A product over
+// the channels (scores) therefore needs a tile with the channels innermost, a product over time (values, gradients) one with time
+// innermost.  Tiles go global -> registers -> LDS in 4 x 4 blocks (4 channels x 4 positions, one 8- or 16-byte load per channel), and
+// each block is written in the orientation that its product reads:
+//   rows  [position][channel]   pitch 2 DKP + 16 bytes
+//   cols  [channel][position]   pitch 2 KT + 16 bytes, positions of each 16 reordered as 0-3, 8-11, 4-7, 12-15
+// Both pitches are odd multiples of 16 bytes: the 16-byte fragment reads of consecutive lanes fall on different banks.  The reordering
+// follows from the result layout: register r of lane (l31, kb) holds row 8 (r >> 2) + 4 kb + (r & 3) of column l31.  Registers 8 s .. 8 s + 7
+// are thus the eight k of the next product's B operand for the positions 16 s + {4 kb + 0..3, 8 + 4 kb + 0..3} -- nothing moves
+// between lanes from one product to the next.
+//
+// fp32 tensors: every operand is cut into three bf16 parts (24 bits of mantissa), six products, smallest first.  The parts of a tile
+// are separate planes in LDS, cut once per workgroup.
+#pragma once
+#include "rel_bucket.h"
+
+typedef __bf16 svbt_bf16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 svbt_bf16x2 __attribute__((ext_vector_type(2)));
+typedef float svbt_f2 __attribute__((ext_vector_type(2)));
+typedef float svbt_f4u __attribute__((ext_vector_type(4), aligned(4)));
+typedef unsigned svbt_u2u __attribute__((ext_vector_type(2), aligned(2)));
+
+#define SVBT_LOG2E 1.4426950408889634f
+#define SVBT_INF __builtin_inff()
+
+// T: float or unsigned short (bf16)
+template <typename T> struct SvbtParts;
+template <> struct SvbtParts<float> { static constexpr int NS = 3; };
+template <> struct SvbtParts<unsigned short> { static constexpr int NS = 1; };
+
+__device__ __forceinline__ unsigned svbt_pack2(float a, float b) {
+    const svbt_f2 v = {a, b};
+    const svbt_bf16x2 h = __builtin_convertvector(v, svbt_bf16x2);
+    unsigned u;
+    __builtin_memcpy(&u, &h, 4);
+    return u;
+}
+__device__ __forceinline__ float svbt_lo(unsigned u) { return __uint_as_float(u << 16); }
+__device__ __forceinline__ float svbt_hi(unsigned u) { return __uint_as_float(u & 0xffff0000u); }
+
+// two floats -> NS packed bf16 pairs that add up to them (to 2^-9, 2^-18, 2^-25 of each)
+template <int NS>
+__device__ __forceinline__ void svbt_parts2(float a, float b, unsigned (&p)[NS]) {
+    p[0] = svbt_pack2(a, b);
+    if constexpr (NS >= 2) {
+        const float ra = a - svbt_lo(p[0]), rb = b - svbt_hi(p[0]);
+        p[1] = svbt_pack2(ra, rb);
+        if constexpr (NS == 3) p[2] = svbt_pack2(ra - svbt_lo(p[1]), rb - svbt_hi(p[1]));
+    }
+}
+// eight floats -> NS operand fragments
+template <int NS>
+__device__ __forceinline__ void svbt_frag8(const float* v, svbt_bf16x8 (&f)[NS]) {
+    unsigned u[NS][4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        unsigned p[NS];
+        svbt_parts2<NS>(v[2 * e], v[2 * e + 1], p);
+#pragma unroll
+        for (int n = 0; n < NS; ++n) u[n][e] = p[n];
+    }
+#pragma unroll
+    for (int n = 0; n < NS; ++n) __builtin_memcpy(&f[n], u[n], 16);
+}
+// acc += A B.  `FLIP` issues the two mixed orders of three-part operands the other way round, so that A B and (B^T A^T)^T are equal
+// bit for bit: the backward recomputes the scores in both orientations and compares them with one log-sum.
+template <int NS, bool FLIP>
+__device__ __forceinline__ void svbt_mma(f32x16& acc, const svbt_bf16x8 (&a)[NS], const svbt_bf16x8 (&b)[NS]) {
+    if constexpr (NS == 3) {
+        constexpr int X = FLIP ? 0 : 1, Y = FLIP ? 1 : 0;
+        acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[2 * X], b[2 * Y], acc, 0, 0, 0);
+        acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[2 * Y], b[2 * X], acc, 0, 0, 0);
+        acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[1], b[1], acc, 0, 0, 0);
+        acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[X], b[Y], acc, 0, 0, 0);
+        acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[Y], b[X], acc, 0, 0, 0);
+    }
+    acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[0], b[0], acc, 0, 0, 0);
+}
+__device__ __forceinline__ void svbt_zero(f32x16& a) {
+#pragma unroll
+    for (int r = 0; r < 16; ++r) a[r] = 0.f;
+}
+// row of a 32 x 32 result that register r of this lane holds
+__device__ __forceinline__ int svbt_row(int r, int kb) { return 8 * (r >> 2) + 4 * kb + (r & 3); }
+
+__device__ __forceinline__ float svbt_load(const float* p) { return *p; }
+__device__ __forceinline__ float svbt_load(const unsigned short* p) { return svb_bf16_f32(*p); }
+__device__ __forceinline__ void svbt_store(float* p, float v) { *p = v; }
+__device__ __forceinline__ void svbt_store(unsigned short* p, float v) { *p = (unsigned short)svbt_pack2(v, v); }
+
+// Operand of this lane's own column t (position) for the channels 16 s + 8 kb + 0..7: read once per workgroup, 32 lanes along time.
+// `has` false or a channel beyond dk: zeros (whatever memory holds there).
+template <typename T, int NS>
+__device__ __forceinline__ void svbt_own_frag(const T* base, long long sc, int t, int s, int kb, int dk, bool has, svbt_bf16x8 (&f)[NS]) {
+    float v[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        const int d = 16 * s + 8 * kb + e;
+        v[e] = has && d < dk ? svbt_load(base + d * sc + t) : 0.f;
+    }
+    svbt_frag8<NS>(v, f);
+}
+
+// ---- staged tiles ----------------------------------------------------------------------------------------------------------
+// One 4 channel x 4 position block as loaded.
+template <typename T> struct SvbtBlock;
+template <> struct SvbtBlock<unsigned short> {
+    unsigned r[4][2];
+    __device__ __forceinline__ void load(const unsigned short* p, long long sc, int rows, int n) {      // rows, n: channels / positions that exist
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+            r[c][0] = r[c][1] = 0u;
+            if (c < rows) {
+                if (n >= 4) { const svbt_u2u t = *reinterpret_cast<const svbt_u2u*>(p + c * sc); r[c][0] = t.x; r[c][1] = t.y; }
+                else {
+                    if (n > 0) r[c][0] = p[c * sc];
+                    if (n > 1) r[c][0] |= (unsigned)p[c * sc + 1] << 16;
+                    if (n > 2) r[c][1] = p[c * sc + 2];
+                }
+            }
+        }
+    }
+    // positions whose bit is not set become zero
+    __device__ __forceinline__ void hide(unsigned seen) {
+        const unsigned m0 = (seen & 1 ? 0xffffu : 0u) | (seen & 2 ? 0xffff0000u : 0u), m1 = (seen & 4 ? 0xffffu : 0u) | (seen & 8 ? 0xffff0000u : 0u);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) { r[c][0] &= m0; r[c][1] &= m1; }
+    }
+    __device__ __forceinline__ void parts(unsigned (&o)[1][4][2]) const {
+#pragma unroll
+        for (int c = 0; c < 4; ++c) { o[0][c][0] = r[c][0]; o[0][c][1] = r[c][1]; }
+    }
+};
+template <> struct SvbtBlock<float> {
+    float r[4][4];
+    __device__ __forceinline__ void load(const float* p, long long sc, int rows, int n) {
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) r[c][e] = 0.f;
+            if (c < rows) {
+                if (n >= 4) {
+                    const svbt_f4u t = *reinterpret_cast<const svbt_f4u*>(p + c * sc);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) r[c][e] = t[e];
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 3; ++e) if (e < n) r[c][e] = p[c * sc + e];
+                }
+            }
+        }
+    }
+    __device__ __forceinline__ void hide(unsigned seen) {
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) r[c][e] = seen >> e & 1 ? r[c][e] : 0.f;
+    }
+    __device__ __forceinline__ void parts(unsigned (&o)[3][4][2]) const {
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                unsigned p[3];
+                svbt_parts2<3>(r[c][2 * h], r[c][2 * h + 1], p);
+#pragma unroll
+                for (int n = 0; n < 3; ++n) o[n][c][h] = p[n];
+            }
+    }
+};
+
+// KT positions x DKP channels of one tensor: NB blocks per thread of NT threads
+template <typename T, int DKP, int KT, int NT>
+struct SvbtTile {
+    static constexpr int NS = SvbtParts<T>::NS, JB = KT / 4, BLOCKS = JB * (DKP / 4), NB = (BLOCKS + NT - 1) / NT;
+    static constexpr int ROWP = 2 * DKP + 16, COLP = 2 * KT + 16;                       // pitches, bytes
+    static constexpr int ROWS_BYTES = KT * ROWP, COLS_BYTES = DKP * COLP;              // one part's plane
+    SvbtBlock<T> b[NB];
+
+    // positions j0 .. j0 + KT - 1 of [dk][.] rows at `base`; positions >= T_ and channels >= dk read as zero
+    __device__ __forceinline__ void load(const T* base, long long sc, int j0, int T_, int dk) {
+#pragma unroll
+        for (int i = 0; i < NB; ++i) {
+            const int id = threadIdx.x + i * NT, d = id / JB * 4, j = j0 + id % JB * 4;
+            if (BLOCKS % NT == 0 || id < BLOCKS) b[i].load(base + d * sc + j, sc, dk - d, T_ - j);
+        }
+    }
+    __device__ __forceinline__ void hide(unsigned long long seen) {
+#pragma unroll
+        for (int i = 0; i < NB; ++i) b[i].hide((unsigned)(seen >> ((threadIdx.x + i * NT) % JB * 4)) & 15u);
+    }
+    template <bool ROWS, bool COLS>
+    __device__ __forceinline__ void store(char* rows, char* cols) const {
+#pragma unroll
+        for (int i = 0; i < NB; ++i) {
+            const int id = threadIdx.x + i * NT, d = id / JB * 4, j = id % JB * 4;
+            if (BLOCKS % NT == 0 || id < BLOCKS) {
+                unsigned o[NS][4][2];
+                b[i].parts(o);
+#pragma unroll
+                for (int n = 0; n < NS; ++n) {
+                    if (COLS) {
+                        const int at = (j & ~15) + ((j & 4) << 1) + ((j & 8) >> 1);                    // 0, 4, 8, 12 -> 0, 8, 4, 12
+#pragma unroll
+                        for (int c = 0; c < 4; ++c)
+                            *reinterpret_cast<uint2*>(cols + n * COLS_BYTES + (d + c) * COLP + 2 * at) = make_uint2(o[n][c][0], o[n][c][1]);
+                    }
+                    if (ROWS) {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const unsigned a0 = o[n][0][e >> 1], a1 = o[n][1][e >> 1], a2 = o[n][2][e >> 1], a3 = o[n][3][e >> 1];
+                            const uint2 w = e & 1 ? make_uint2(a0 >> 16 | (a1 & 0xffff0000u), a2 >> 16 | (a3 & 0xffff0000u))
+                                                  : make_uint2((a0 & 0xffffu) | a1 << 16, (a2 & 0xffffu) | a3 << 16);
+                            *reinterpret_cast<uint2*>(rows + n * ROWS_BYTES + (j + e) * ROWP + 2 * d) = w;
+                        }
+                    }
+                }
+            }
+        }
+    }
+    // A operand, rows = positions 32 sub + l31, k = channels 16 s + 8 kb + 0..7
+    static __device__ __forceinline__ void row_frag(const char* rows, int sub, int s, int l31, int kb, svbt_bf16x8 (&f)[NS]) {
+#pragma unroll
+        for (int n = 0; n < NS; ++n) {
+            const uint4 t = *reinterpret_cast<const uint4*>(rows + n * ROWS_BYTES + (32 * sub + l31) * ROWP + 32 * s + 16 * kb);
+            __builtin_memcpy(&f[n], &t, 16);
+        }
+    }
+    // A operand, rows = channels 32 db + l31, k = the positions of registers 8 s .. 8 s + 7 of sub-tile sub
+    static __device__ __forceinline__ void col_frag(const char* cols, int db, int sub, int s, int l31, int kb, svbt_bf16x8 (&f)[NS]) {
+#pragma unroll
+        for (int n = 0; n < NS; ++n) {
+            const uint4 t = *reinterpret_cast<const uint4*>(cols + n * COLS_BYTES + (32 * db + l31) * COLP + 64 * sub + 32 * s + 16 * kb);
+            __builtin_memcpy(&f[n], &t, 16);
+        }
+    }
+};
+
+// ---- positions and masks -----------------------------------------------------------------------------------------------------
+// position of query 0 of batch entry b; far beyond any key it makes no difference how far
+__device__ __forceinline__ int svbt_start(const SvbBucketAttn& a, int b) {
+    const int s = a.q_start_b ? a.q_start_b[b] : a.q_start;
+    return max(-(1 << 29), min(1 << 29, s));
+}
+// bias of this head per offset o in [-R, R], times log2(e), into LDS (every thread of the workgroup; the caller synchronises)
+__device__ __forceinline__ void svbt_fill_bias(float* s_bias, const SvbBucketAttn& a, int h, int R, int nt) {
+    for (int o = threadIdx.x; o <= 2 * R; o += nt)
+        s_bias[o] = svb_ld_table(a.table, (size_t)svb_bucket_of(a.buckets, o - R) * a.H + h, a.table_dtype == SVB_DT_BF16) * SVBT_LOG2E;
+}
+// bits of the keys j0 .. j0 + 63 that exist (j < end) and are kept
+__device__ __forceinline__ unsigned long long svbt_keep_bits(float keep, int j0, int end, int lane) {
+    return __ballot(j0 + lane < end && keep != 0.f);
+}
+// last kept key + 1 of a batch entry (0: none), by one wave; 512 keys' loads in flight, from the end
+__device__ __forceinline__ int svbt_keep_end(const float* keep, int n, int lane) {
+    for (int j0 = (n - 1) / 512 * 512; j0 >= 0; j0 -= 512) {
+        float v[8];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) v[u] = keep[min(j0 + 64 * u + lane, n - 1)];
+        int last = 0;
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+            const unsigned long long m = __ballot(j0 + 64 * u + lane < n && v[u] != 0.f);
+            if (m) last = j0 + 64 * u + 64 - __builtin_clzll(m);
+        }
+        if (last) return last;
+    }
+    return 0;
+}
+// work item of a workgroup: consecutive items on one XCD (workgroups go round the 8 XCDs in turn), so that the workgroups of one
+// head share their keys and values in one L2
+__device__ __forceinline__ int svbt_item(int id, int total) {
+    const int x = id & 7, q = total >> 3, r = total & 7;
+    return x * q + min(x, r) + (id >> 3);
+}

@@ -1,0 +1,412 @@
+// bucket_attn_bwd.hip -- gradients of the attention with a learned relative-position bias by buckets.
+//
+//   t_ij = log2(e) (scale q_i . k_j + bias),  P_ij = 2^(t_ij - lse_i)  (recomputed),  dP_ij = dout_i . v_j,  delta_i = dout_i . out_i
+//   dS_ij = P_ij (dP_ij - delta_i):   dv_j = sum_i P_ij dout_i,  dk_j = scale sum_i dS_ij q_i,  dq_i = scale sum_j dS_ij k_j,
+//   dtable[k][h] = sum of dS_ij over the pairs of bucket k
+//
+// Two kernels, each of which owns what it sums, so that every sum has one order and nothing is added atomically between workgroups:
+// the first owns 32 queries per wave and walks the keys (dq, dtable, delta), the second owns 32 keys per wave and walks the queries of
+// all heads that share them (dk, dv).  That is seven products instead of five; the scores are computed in the orientation in which
+// their registers are the next product's operand (attn_tiles.h), so dS never moves between lanes.
+//
+// delta needs what rounding the output to bf16 destroys -- the sums over a bucket cancel, and the table's gradient is fp32 --, so the
+// forward keeps the output in fp32 for bf16 tensors.  P and dS are rounded to bf16 as operands for bf16 tensors (relative 2^-9 each,
+// averaged over the sum), and cut into three parts for fp32 tensors; dtable sums dS in fp32 before any rounding.
+// A row whose weight is all on one key (P == 1) has dS = 0: dP - delta is then rounding noise alone.
+//
+// dtable: dS of pairs further than the last bucket border is summed in registers; nearer pairs go to LDS, where each thread has its
+// own slot per bucket, and the slots are added in order at the end.
+#include "attn_tiles.h"
+
+int svb_bucket_attn_check(const SvbBucketAttn* a);
+int svb_bucket_table_reduce(const float* part, void* dtable, int rows, int nb, int H, int dtype, hipStream_t st);
+
+struct SvbBattnBwd {
+    const void* dout;
+    void *dq, *dk, *dv;
+    float *delta, *part;           // [B][H][Tq]; [H][B * query tiles][n_buckets] or NULL
+};
+
+__device__ __forceinline__ float svbt_ds(float p, float dp, float delta) {
+    const float ds = p * (dp - delta);
+    return p == 0.f || p == 1.f ? 0.f : ds;
+}
+
+// ---- dq, dtable, delta: 4 waves x 32 queries, keys staged ----------------------------------------------------------------------------
+template <typename T, int DKP, int KT, bool DOUBLE>
+__global__ __launch_bounds__(256, 1) void svb_bucket_attn_dq_kernel(SvbBucketAttn a, SvbBattnBwd g, int qtiles) {
+    typedef SvbtTile<T, DKP, KT, 256> Tile;
+    constexpr int NS = Tile::NS, NK = DKP / 16, NDB = DKP / 32, NSUB = KT / 32;
+    constexpr int BUF = NS * (2 * Tile::ROWS_BYTES + Tile::COLS_BYTES);
+    HIP_DYNAMIC_SHARED(char, smem)
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l31 = lane & 31, kb = lane >> 5;
+    const int item = svbt_item(blockIdx.x, gridDim.x);
+    const int bh = item / qtiles, b = bh / a.H, h = bh - b * a.H, hk = h / (a.H / a.Hkv);
+    const int qt = a.causal ? qtiles - 1 - (item - bh * qtiles) : item - bh * qtiles;
+    const int i0 = qt * 128, i = i0 + wave * 32 + l31;
+    const bool has = i < a.Tq;
+    const int start = svbt_start(a, b), R = svb_bucket_reach(a.buckets), nb = a.buckets.n_buckets;
+
+    // own operands, and delta on the way
+    const T* q = (const T*)a.q + b * a.q_sb + (long long)h * a.dk * a.q_sc;
+    const size_t head = ((size_t)b * a.H + h) * a.dk * a.Tq;
+    const T* dout = (const T*)g.dout + head;
+    const float* out = (NS == 3 ? (const float*)a.out : a.out_f32) + head;
+    const size_t row = ((size_t)b * a.H + h) * a.Tq + (has ? i : 0);
+    svbt_bf16x8 qf[NK][NS], of[NK][NS];
+    float delta = 0.f;
+#pragma unroll
+    for (int s = 0; s < NK; ++s) {
+        svbt_own_frag<T, NS>(q, a.q_sc, i, s, kb, a.dk, has, qf[s]);
+        float v[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const int d = 16 * s + 8 * kb + e;
+            const bool in = has && d < a.dk;
+            v[e] = in ? svbt_load(dout + (size_t)d * a.Tq + i) : 0.f;
+            delta = fmaf(v[e], in ? out[(size_t)d * a.Tq + i] : 0.f, delta);
+        }
+        svbt_frag8<NS>(v, of[s]);
+    }
+    delta += __shfl_xor(delta, 32, 64);
+    if (has && kb == 0) g.delta[row] = delta;
+    if (!g.dq && !g.part) return;                                       // (only delta is wanted; uniform)
+    const float lse = has ? a.lse[row] : SVBT_INF;
+
+    float* s_bias = (float*)(smem + (DOUBLE ? 2 : 1) * BUF);
+    float* s_sum = s_bias + ((2 * R + 1 + 3) & ~3);                      // [nb][256]
+    unsigned char* s_idx = (unsigned char*)(s_sum + (g.part ? nb * 256 : 0));
+    svbt_fill_bias(s_bias, a, h, R, 256);
+    if (g.part) {
+        for (int e = 0; e < nb; ++e) s_sum[e * 256 + threadIdx.x] = 0.f;
+        for (int o = threadIdx.x; o <= 2 * R; o += 256) s_idx[o] = (unsigned char)svb_bucket_of(a.buckets, o - R);
+    }
+
+    const T* k = (const T*)a.k + b * a.k_sb + (long long)hk * a.dk * a.k_sc;
+    const T* v = (const T*)a.v + b * a.v_sb + (long long)hk * a.dk * a.v_sc;
+    const float* keep = a.keep ? a.keep + (size_t)b * a.Tk : nullptr;
+    int end = keep ? svbt_keep_end(keep, a.Tk, lane) : a.Tk;
+    if (a.causal) end = max(0, min(end, start + min(i0 + 128, a.Tq)));
+    const int p0 = start + i0 + wave * 32, p1 = p0 + 31, p = start + i;
+    const int tiles = (end + KT - 1) / KT;
+    const float c = a.scale * SVBT_LOG2E;
+
+    f32x16 acc[NDB];
+#pragma unroll
+    for (int d = 0; d < NDB; ++d) svbt_zero(acc[d]);
+    float sum_past = 0.f, sum_ahead = 0.f;
+
+    Tile tk, tv;
+    unsigned long long seen = ~0ull;
+    constexpr unsigned long long ALL = KT == 64 ? ~0ull : 0xffffffffull;
+    auto fetch = [&](int t) {
+        tk.load(k, a.k_sc, t * KT, end, a.dk);
+        tv.load(v, a.v_sc, t * KT, end, a.dk);
+    };
+    auto bits = [&](int t) {
+        return ALL & (keep ? svbt_keep_bits(keep[min(t * KT + lane, a.Tk - 1)], t * KT, end, lane) : __ballot(t * KT + lane < end));
+    };
+    auto put = [&](int t) {
+        if (keep) { tk.hide(seen); tv.hide(seen); }
+        char* buf = smem + (DOUBLE ? (t & 1) * BUF : 0);
+        tk.template store<true, true>(buf, buf + 2 * NS * Tile::ROWS_BYTES);
+        tv.template store<true, false>(buf + NS * Tile::ROWS_BYTES, nullptr);
+    };
+    if (tiles > 0) {
+        fetch(0);
+        seen = bits(0);
+        put(0);
+    }
+    __syncthreads();
+    const float past = s_bias[0], ahead = s_bias[2 * R];
+    for (int t = 0; t < tiles; ++t) {
+        const unsigned long long now = seen;
+        const int j0 = t * KT;
+        if (t + 1 < tiles) fetch(t + 1);
+        const char* krows = smem + (DOUBLE ? (t & 1) * BUF : 0);
+        const char* vrows = krows + NS * Tile::ROWS_BYTES;
+        const char* kcols = vrows + NS * Tile::ROWS_BYTES;
+        if (now != 0ull && !(a.causal && j0 > p1)) {
+            const bool edge = now != ALL || (a.causal && j0 + KT - 1 > p0);
+            const bool behind = j0 + KT - 1 - p0 <= -R, before = j0 - p1 >= R;
+            const float flat = behind ? past : ahead;
+#pragma unroll
+            for (int u = 0; u < NSUB; ++u) {
+                f32x16 s, dp;
+                svbt_zero(s);
+                svbt_zero(dp);
+#pragma unroll
+                for (int x = 0; x < NK; ++x) {
+                    svbt_bf16x8 f[NS];
+                    Tile::row_frag(krows, u, x, l31, kb, f);
+                    svbt_mma<NS, false>(s, f, qf[x]);
+                    Tile::row_frag(vrows, u, x, l31, kb, f);
+                    svbt_mma<NS, false>(dp, f, of[x]);
+                }
+                const unsigned su = (unsigned)(now >> (32 * u));
+                const int qo = p - (j0 + 32 * u);
+                if (behind || before) {
+                    float sum = 0.f;
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) {
+                        const int rw = svbt_row(r, kb);
+                        float w = __builtin_amdgcn_exp2f(fmaf(s[r], c, flat) - lse);
+                        if (edge) w = (su >> rw & 1u) && !(a.causal && rw > qo) ? w : 0.f;
+                        s[r] = svbt_ds(w, dp[r], delta);
+                        sum += s[r];
+                    }
+                    if (behind) sum_past += sum;
+                    else sum_ahead += sum;
+                } else {
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) {
+                        const int rw = svbt_row(r, kb), o = max(-R, min(R, rw - qo)) + R;
+                        float w = __builtin_amdgcn_exp2f(fmaf(s[r], c, s_bias[o]) - lse);
+                        if (edge) w = (su >> rw & 1u) && !(a.causal && rw > qo) ? w : 0.f;
+                        s[r] = svbt_ds(w, dp[r], delta);
+                        if (g.part) atomicAdd(&s_sum[(int)s_idx[o] * 256 + threadIdx.x], s[r]);        // (this thread's own slot)
+                    }
+                }
+#pragma unroll
+                for (int x = 0; x < 2; ++x) {
+                    float w[8];
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) w[e] = s[8 * x + e];
+                    svbt_bf16x8 sf[NS];
+                    svbt_frag8<NS>(w, sf);
+#pragma unroll
+                    for (int d = 0; d < NDB; ++d) {
+                        svbt_bf16x8 f[NS];
+                        Tile::col_frag(kcols, d, u, x, l31, kb, f);
+                        svbt_mma<NS, false>(acc[d], f, sf);
+                    }
+                }
+            }
+        }
+        if (t + 1 < tiles) {
+            if (!DOUBLE) __syncthreads();
+            seen = bits(t + 1);
+            put(t + 1);
+        }
+        __syncthreads();
+    }
+    if (g.part) {
+        atomicAdd(&s_sum[(int)s_idx[0] * 256 + threadIdx.x], sum_past);
+        atomicAdd(&s_sum[(int)s_idx[2 * R] * 256 + threadIdx.x], sum_ahead);
+        __syncthreads();
+        float* part = g.part + (((size_t)h * a.B + b) * qtiles + qt) * nb;
+        for (int e = wave; e < nb; e += 4) {
+            const float* x = s_sum + e * 256 + lane;
+            const float w = svb_wave_sum((x[0] + x[64]) + (x[128] + x[192]));
+            if (lane == 0) part[e] = w;
+        }
+    }
+    if (!has || !g.dq) return;
+    T* dq = (T*)g.dq + head + i;
+#pragma unroll
+    for (int d = 0; d < NDB; ++d)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            const int ch = 32 * d + svbt_row(r, kb);
+            if (ch < a.dk) svbt_store(dq + (size_t)ch * a.Tq, acc[d][r] * a.scale);
+        }
+}
+
+// ---- dk, dv: 4 waves x 32 keys, queries of the heads that share them staged -----------------------------------------------------------
+template <typename T, int DKP, int KT, bool DOUBLE>
+__global__ __launch_bounds__(256, 1) void svb_bucket_attn_dkv_kernel(SvbBucketAttn a, SvbBattnBwd g, int ktiles) {
+    typedef SvbtTile<T, DKP, KT, 256> Tile;
+    constexpr int NS = Tile::NS, NK = DKP / 16, NDB = DKP / 32, NSUB = KT / 32;
+    constexpr int TILE = NS * 2 * (Tile::ROWS_BYTES + Tile::COLS_BYTES), BUF = TILE + 2 * KT * 4;
+    HIP_DYNAMIC_SHARED(char, smem)
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l31 = lane & 31, kb = lane >> 5;
+    const int item = svbt_item(blockIdx.x, gridDim.x);
+    const int bk = item / ktiles, b = bk / a.Hkv, hk = bk - b * a.Hkv, G = a.H / a.Hkv;
+    const int jt = (item - bk * ktiles) * 128, jw = jt + wave * 32, j = jw + l31;
+    const bool has = j < a.Tk, kept = has && (!a.keep || a.keep[(size_t)b * a.Tk + j] != 0.f);
+    const int start = svbt_start(a, b), R = svb_bucket_reach(a.buckets);
+    float* s_bias = (float*)(smem + (DOUBLE ? 2 : 1) * BUF);
+
+    const T* k = (const T*)a.k + b * a.k_sb + (long long)hk * a.dk * a.k_sc;
+    const T* v = (const T*)a.v + b * a.v_sb + (long long)hk * a.dk * a.v_sc;
+    svbt_bf16x8 kf[NK][NS], vf[NK][NS];
+#pragma unroll
+    for (int s = 0; s < NK; ++s) {
+        svbt_own_frag<T, NS>(k, a.k_sc, j, s, kb, a.dk, kept, kf[s]);
+        svbt_own_frag<T, NS>(v, a.v_sc, j, s, kb, a.dk, kept, vf[s]);
+    }
+    const bool all_kept = __ballot(!kept) == 0ull, none_kept = __ballot(kept) == 0ull;
+    f32x16 dk[NDB], dv[NDB];
+#pragma unroll
+    for (int d = 0; d < NDB; ++d) { svbt_zero(dk[d]); svbt_zero(dv[d]); }
+
+    // queries that see a key of this workgroup: i >= first
+    const int first = a.causal ? max(0, min(jt - start, a.Tq)) / KT : 0;
+    const int tiles = max(0, (a.Tq + KT - 1) / KT - first);
+    const float c = a.scale * SVBT_LOG2E;
+    Tile tq, td;
+    float stat = 0.f;                                                   // this thread's lse (threads < KT) or delta (KT .. 2 KT - 1)
+    const int steps = G * tiles;
+    const bool any_kept = none_kept ? false : true;
+    auto fetch = [&](int n) {
+        const int hh = hk * G + n / tiles, i0 = (first + n % tiles) * KT;
+        const size_t hd = (size_t)b * a.H + hh;
+        tq.load((const T*)a.q + b * a.q_sb + (long long)hh * a.dk * a.q_sc, a.q_sc, i0, a.Tq, a.dk);
+        td.load((const T*)g.dout + hd * a.dk * a.Tq, a.Tq, i0, a.Tq, a.dk);
+        if (threadIdx.x < 2 * KT) {
+            const int i = i0 + (threadIdx.x & (KT - 1));
+            const float none = threadIdx.x < KT ? SVBT_INF : 0.f;       // (a query that does not exist has P = 0)
+            stat = i < a.Tq ? (threadIdx.x < KT ? a.lse : g.delta)[hd * a.Tq + i] : none;
+        }
+    };
+    auto put = [&](int n) {
+        char* buf = smem + (DOUBLE ? (n & 1) * BUF : 0);
+        tq.template store<true, true>(buf, buf + 2 * NS * Tile::ROWS_BYTES);
+        td.template store<true, true>(buf + NS * Tile::ROWS_BYTES, buf + NS * (2 * Tile::ROWS_BYTES + Tile::COLS_BYTES));
+        if (threadIdx.x < 2 * KT) ((float*)(buf + TILE))[threadIdx.x] = stat;
+    };
+    float past = 0.f, ahead = 0.f;
+    if (steps > 0) { fetch(0); put(0); }
+    for (int n = 0; n < steps; ++n) {
+        if (n % tiles == 0) {                                           // a new head's bias (every thread is behind the last tile's barrier)
+            svbt_fill_bias(s_bias, a, hk * G + n / tiles, R, 256);
+            __syncthreads();
+            past = s_bias[0];
+            ahead = s_bias[2 * R];
+        }
+        if (n + 1 < steps) fetch(n + 1);
+        const char* qrows = smem + (DOUBLE ? (n & 1) * BUF : 0);
+        const char* drows = qrows + NS * Tile::ROWS_BYTES;
+        const char* qcols = drows + NS * Tile::ROWS_BYTES;
+        const char* dcols = qcols + NS * Tile::COLS_BYTES;
+        const float* stats = (const float*)(qrows + TILE);
+        const int pt = start + (first + n % tiles) * KT;                // position of the tile's first query
+        if (any_kept && !(a.causal && jw > pt + KT - 1)) {              // (wave-uniform)
+            const bool edge = !all_kept || (a.causal && jw + 31 > pt);
+            const bool behind = jw + 31 - pt <= -R, before = jw - (pt + KT - 1) >= R;
+            const float flat = behind ? past : ahead;
+#pragma unroll
+            for (int u = 0; u < NSUB; ++u) {
+                f32x16 s, dp;
+                svbt_zero(s);
+                svbt_zero(dp);
+#pragma unroll
+                for (int x = 0; x < NK; ++x) {
+                    svbt_bf16x8 f[NS];
+                    Tile::row_frag(qrows, u, x, l31, kb, f);
+                    svbt_mma<NS, true>(s, f, kf[x]);
+                    Tile::row_frag(drows, u, x, l31, kb, f);
+                    svbt_mma<NS, true>(dp, f, vf[x]);
+                }
+                const int jo = j - (pt + 32 * u);                       // offset against query row 0 of the sub-tile
+#pragma unroll
+                for (int r4 = 0; r4 < 4; ++r4) {
+                    const float4 ls = *reinterpret_cast<const float4*>(stats + 32 * u + 8 * r4 + 4 * kb);
+                    const float4 dl = *reinterpret_cast<const float4*>(stats + KT + 32 * u + 8 * r4 + 4 * kb);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const int r = 4 * r4 + e, o = jo - svbt_row(r, kb);
+                        float bias = flat;
+                        if (!(behind || before)) bias = s_bias[max(-R, min(R, o)) + R];
+                        float w = __builtin_amdgcn_exp2f(fmaf(s[r], c, bias) - ls[e]);
+                        if (edge) w = kept && !(a.causal && o > 0) ? w : 0.f;
+                        s[r] = w;
+                        dp[r] = svbt_ds(w, dp[r], dl[e]);
+                    }
+                }
+#pragma unroll
+                for (int x = 0; x < 2; ++x) {
+                    float w[8], z[8];
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) { w[e] = s[8 * x + e]; z[e] = dp[8 * x + e]; }
+                    svbt_bf16x8 pf[NS], sf[NS];
+                    svbt_frag8<NS>(w, pf);
+                    svbt_frag8<NS>(z, sf);
+#pragma unroll
+                    for (int d = 0; d < NDB; ++d) {
+                        svbt_bf16x8 f[NS];
+                        Tile::col_frag(dcols, d, u, x, l31, kb, f);
+                        svbt_mma<NS, false>(dv[d], f, pf);
+                        Tile::col_frag(qcols, d, u, x, l31, kb, f);
+                        svbt_mma<NS, false>(dk[d], f, sf);
+                    }
+                }
+            }
+        }
+        if (n + 1 < steps) {
+            if (!DOUBLE) __syncthreads();
+            put(n + 1);
+        }
+        __syncthreads();
+    }
+    if (!has) return;
+    const size_t head = ((size_t)b * a.Hkv + hk) * a.dk * a.Tk + j;
+#pragma unroll
+    for (int d = 0; d < NDB; ++d)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            const int ch = 32 * d + svbt_row(r, kb);
+            if (ch < a.dk) {
+                svbt_store((T*)g.dk + head + (size_t)ch * a.Tk, dk[d][r] * a.scale);
+                svbt_store((T*)g.dv + head + (size_t)ch * a.Tk, dv[d][r]);
+            }
+        }
+}
+
+// ---- host ------------------------------------------------------------------------------------------------------------------------
+template <typename K>
+static int bwd_lds(K* kern, int lds) {
+    return lds > 65536 && hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024) != hipSuccess;
+}
+
+template <typename T, int DKP, int KT, bool DOUBLE>
+static int bwd_launch(const SvbBucketAttn* a, const SvbBattnBwd& g, hipStream_t st) {
+    typedef SvbtTile<T, DKP, KT, 256> Tile;
+    const int nbuf = DOUBLE ? 2 : 1, span = 2 * svb_bucket_reach(a->buckets) + 1;
+    {
+        const int qtiles = (a->Tq + 127) / 128;
+        int lds = nbuf * Tile::NS * (2 * Tile::ROWS_BYTES + Tile::COLS_BYTES) + ((span + 3) & ~3) * 4;
+        if (g.part) lds += a->buckets.n_buckets * 1024 + span;
+        auto* kern = svb_bucket_attn_dq_kernel<T, DKP, KT, DOUBLE>;
+        if (bwd_lds(kern, lds)) return SVB_ERR_LAUNCH;
+        hipLaunchKernelGGL(kern, dim3((unsigned)(a->B * a->H * qtiles)), dim3(256), lds, st, *a, g, qtiles);
+        SVB_CHECK_LAUNCH();
+    }
+    if (g.dk) {
+        const int ktiles = (a->Tk + 127) / 128;
+        const int lds = nbuf * (2 * Tile::NS * (Tile::ROWS_BYTES + Tile::COLS_BYTES) + 2 * KT * 4) + span * 4;
+        auto* kern = svb_bucket_attn_dkv_kernel<T, DKP, KT, DOUBLE>;
+        if (bwd_lds(kern, lds)) return SVB_ERR_LAUNCH;
+        hipLaunchKernelGGL(kern, dim3((unsigned)(a->B * a->Hkv * ktiles)), dim3(256), lds, st, *a, g, ktiles);
+        SVB_CHECK_LAUNCH();
+    }
+    return SVB_OK;
+}
+
+static size_t delta_floats(const SvbBucketAttn* a) { return ((size_t)a->B * a->H * a->Tq + 3) & ~(size_t)3; }
+
+extern "C" size_t svb_bucket_attn_bwd_workspace_floats(const SvbBucketAttn* a) {
+    if (!a || a->B <= 0 || a->H <= 0 || a->Tq <= 0) return 0;
+    return delta_floats(a) + (size_t)a->H * a->B * ((a->Tq + 127) / 128) * a->buckets.n_buckets;
+}
+
+extern "C" int svb_bucket_attn_bwd(const SvbBucketAttn* a, const SvbBucketAttnGrad* g, void* stream) {
+    int rc = svb_bucket_attn_check(a);
+    if (rc != SVB_OK) return rc;
+    if (!g || !g->dout || !g->ws || !a->lse || (a->dtype == SVB_DT_BF16 && !a->out_f32) || (!g->d_k != !g->d_v)) return SVB_ERR_ARG;
+    hipStream_t st = (hipStream_t)stream;
+    SvbBattnBwd w = {g->dout, g->d_q, g->d_k, g->d_v, g->ws, g->d_table ? g->ws + delta_floats(a) : nullptr};
+    if (a->dtype == SVB_DT_BF16) {
+        if (a->dk <= 32) rc = bwd_launch<unsigned short, 32, 64, true>(a, w, st);
+        else if (a->dk <= 64) rc = bwd_launch<unsigned short, 64, 64, true>(a, w, st);
+        else if (a->dk <= 96) rc = bwd_launch<unsigned short, 96, 64, false>(a, w, st);
+        else rc = bwd_launch<unsigned short, 128, 64, false>(a, w, st);
+    } else {
+        if (a->dk <= 32) rc = bwd_launch<float, 32, 32, true>(a, w, st);
+        else if (a->dk <= 64) rc = bwd_launch<float, 64, 32, false>(a, w, st);
+        else if (a->dk <= 96) rc = bwd_launch<float, 96, 32, false>(a, w, st);
+        else rc = bwd_launch<float, 128, 32, false>(a, w, st);
+    }
+    if (rc != SVB_OK || !g->d_table) return rc;
+    return svb_bucket_table_reduce(w.part, g->d_table, a->B * ((a->Tq + 127) / 128), a->buckets.n_buckets, a->H, a->table_dtype, st);
+}

@@ -1,0 +1,42 @@
+// rel_bucket.h -- the bucket of a relative position, shared by bucket_bias.hip and bucket_attn_{fwd,bwd}.hip.
+//
+// A key at offset  o = key - query  falls into one of n_buckets: with `both`, half of the buckets serve o > 0 and half o <= 0 and
+// the distance is m = |o|; without it only the past counts, m = max(-o, 0).  Of a side's w buckets the first half hold one
+// distance each (m < near), the others grow geometrically up to max_distance:  bucket = near + #{t : edge[t] <= m}.
+// edge[t] is the least m with  near (max_distance / near)^((t+1) / (w - near)) <= m,  found by the caller in whole numbers, so
+// that a distance on a border has one answer; beyond the last edge nothing changes any more.
+#pragma once
+#include "svb_common.h"
+#include "../../include/svb_hip.h"
+
+// least distance from which a side's bucket stays the same
+static __host__ __device__ __forceinline__ int svb_bucket_reach(const SvbRelBuckets& b) {
+    return b.n_edge > 0 ? b.edge[b.n_edge - 1] : b.near;
+}
+
+__device__ __forceinline__ int svb_bucket_of(const SvbRelBuckets& b, int off) {
+    int base = 0, m = off < 0 ? -off : 0;
+    if (b.both && off > 0) { base = b.n_buckets / 2; m = off; }
+    if (m < b.near) return base + m;
+    int k = base + b.near;
+    for (int t = 0; t < b.n_edge; ++t) k += b.edge[t] <= m ? 1 : 0;
+    return k;
+}
+
+// host: is this a partition that the kernels can index with?
+static inline bool svb_bucket_valid(const SvbRelBuckets* b) {
+    if (!b || b->n_buckets < 2 || b->n_buckets > SVB_REL_MAX_BUCKETS || (b->both && (b->n_buckets & 1))) return false;
+    const int side = b->both ? b->n_buckets / 2 : b->n_buckets;
+    if (b->near < 1 || b->n_edge < 0 || b->n_edge > SVB_REL_MAX_EDGES || b->near + b->n_edge + 1 > side) return false;
+    int last = b->near;
+    for (int t = 0; t < b->n_edge; ++t) {
+        if (b->edge[t] < last || b->edge[t] > SVB_REL_MAX_REACH) return false;
+        last = b->edge[t];
+    }
+    return b->near <= SVB_REL_MAX_REACH;
+}
+
+__device__ __forceinline__ float svb_bf16_f32(unsigned short h) { return __uint_as_float((unsigned)h << 16); }
+__device__ __forceinline__ float svb_ld_table(const void* t, size_t i, int is_bf16) {
+    return is_bf16 ? svb_bf16_f32(((const unsigned short*)t)[i]) : ((const float*)t)[i];
+}

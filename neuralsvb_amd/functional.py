@@ -9,6 +9,7 @@ conv1d / conv_transpose1d carry the fusions the reference expresses as separate 
 wn_stack is the whole gated conv stack `WN.forward` (fs2_vae.py:61-91) as ONE autograd node with a hand-scheduled
 backward, so no intermediate is kept that the backward does not need.
 """
+import functools
 import weakref
 
 import torch
@@ -872,11 +873,138 @@ def layer_norm(x, gamma, beta, eps=1e-5):
     return _LayerNormFn.apply(x, gamma, beta, float(eps))
 
 
+class _LayerNormNCTFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, gamma, beta, eps):
+        x, gamma, beta = _c(x), _c(gamma), _c(beta)
+        y, mean, rstd = K.ln_nct_fwd(x, gamma, beta, eps, save_stats=True)
+        ctx.affine_dtype = gamma.dtype if gamma is not None else beta.dtype if beta is not None else torch.float32
+        ctx.save_for_backward(x, gamma, mean, rstd)
+        return y
+
+    @staticmethod
+    def backward(ctx, dy):
+        x, gamma, mean, rstd = ctx.saved_tensors
+        return K.ln_nct_bwd(x, gamma, _c(dy), mean, rstd, *ctx.needs_input_grad[:3], affine_dtype=ctx.affine_dtype) + (None,)
+
+
 def layer_norm_nct(x, gamma, beta, eps=1e-5):
-    """LayerNorm over the channel dim of [B, C, T]; forward only (used inside the frozen PPG encoder)."""
-    if torch.is_grad_enabled() and (x.requires_grad or gamma.requires_grad):
-        raise RuntimeError("layer_norm_nct is forward-only (frozen encoder); use layer_norm for trainable paths")
-    return K.layernorm_nct_fwd(x.contiguous(), gamma, beta, eps)
+    """LayerNorm over the channel dim of x [B, C, T] (float32 or bfloat16), differentiable.  gamma, beta [C] of float32 or of x's
+    dtype, each may be None.  Statistics and sums are float32; the affine gradients have a fixed order of summation."""
+    if x.dim() != 3:
+        raise ValueError(f"layer_norm_nct: x must be [B, C, T], got {tuple(x.shape)}")
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, gamma, beta)):
+        return _LayerNormNCTFn.apply(x, gamma, beta, float(eps))
+    if x.dtype == torch.float32 and x.numel():
+        return K.layernorm_nct_fwd(x.contiguous(), gamma, beta, eps)
+    return K.ln_nct_fwd(_c(x), _c(gamma), _c(beta), eps)
+
+
+@functools.lru_cache(maxsize=64)
+def _bucket_edges(side, far):
+    """Least distances of the geometric buckets after the first of a side's `side` buckets: near (far / near)^(t / w) <= m for
+    t = 1 .. w - 1, in whole numbers ((far / near)^t <= (m / near)^w), so that a distance on a border has one answer."""
+    near = side // 2
+    w, edges, m = side - near, [], near
+    for t in range(1, w):
+        while far ** t * near ** (w - t) > m ** w:
+            m += 1
+        edges.append(m)
+    return near, tuple(edges)
+
+
+class RelativeBuckets:
+    """How relative positions share the rows of a bias table [n_buckets, H].  The key at offset o = key - query: `bidirectional` gives
+    half of the rows to o > 0 and half to o <= 0, with distance |o|; otherwise all rows serve the past, distance max(-o, 0).  Of a
+    side's rows the first half stand for one distance each, the others for geometrically growing ranges up to max_distance, the last
+    for all that is further."""
+
+    def __init__(self, n_buckets=32, max_distance=128, bidirectional=True):
+        n_buckets, max_distance = int(n_buckets), int(max_distance)
+        side = n_buckets // 2 if bidirectional else n_buckets
+        if not 2 <= n_buckets <= L_.SVB_REL_MAX_BUCKETS or (bidirectional and n_buckets % 2) or side < 2:
+            raise ValueError(f"n_buckets: 2 (one side) or 4 (both, even) ... {L_.SVB_REL_MAX_BUCKETS}, got {n_buckets}")
+        if not side // 2 < max_distance <= L_.SVB_REL_MAX_REACH:
+            raise ValueError(f"max_distance: {side // 2 + 1} ... {L_.SVB_REL_MAX_REACH}, got {max_distance}")
+        self.n_buckets, self.max_distance, self.bidirectional = n_buckets, max_distance, bool(bidirectional)
+        near, edges = _bucket_edges(side, max_distance)
+        self.c = L_.SvbRelBuckets(n_buckets, int(self.bidirectional), near, len(edges), (L_.C.c_int * L_.SVB_REL_MAX_EDGES)(*edges))
+
+    def __repr__(self):
+        return f"RelativeBuckets({self.n_buckets}, {self.max_distance}, bidirectional={self.bidirectional})"
+
+
+class _BucketBiasFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, table, buckets, tq, tk, q_start):
+        ctx.cfg = (buckets, q_start)
+        return K.bucket_bias_fwd(_c(table), buckets, tq, tk, q_start)
+
+    @staticmethod
+    def backward(ctx, dbias):
+        buckets, q_start = ctx.cfg
+        return K.bucket_bias_bwd(_c(dbias), buckets, q_start), None, None, None, None
+
+
+def bucket_bias(table, buckets, tq, tk, q_start=None):
+    """The learned bias of `buckets` (RelativeBuckets) as a [H, tq, tk] tensor of table's dtype (float32 or bfloat16), differentiable:
+    bias[h, i, j] = table[bucket(j - (q_start + i)), h].  table [n_buckets, H]; q_start: position of query 0 (default: the queries are
+    the last tq of the keys' positions)."""
+    tq, tk = int(tq), int(tk)
+    q_start = tk - tq if q_start is None else int(q_start)
+    if tq < 0 or tk < 0:
+        raise ValueError(f"bucket_bias: lengths {tq}, {tk}")
+    return _BucketBiasFn.apply(table, buckets.c, tq, tk, q_start)
+
+
+class _BucketAttnFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, table, keep, q_start, cfg):
+        out, lse, o32 = K.bucket_attn_fwd(q, k, v, table, *cfg[:2], keep, q_start, *cfg[2:], train=True)
+        ctx.cfg = cfg
+        ctx.start = None if isinstance(q_start, torch.Tensor) else q_start
+        ctx.save_for_backward(q, k, v, table, keep, None if ctx.start is not None else q_start, out if o32 is None else None, lse, o32)
+        return out
+
+    @staticmethod
+    def backward(ctx, dout):
+        q, k, v, table, keep, starts, out, lse, o32 = ctx.saved_tensors
+        nq, nk, nv, nt = ctx.needs_input_grad[:4]
+        cfg = ctx.cfg
+        dq, dk, dv, dt = K.bucket_attn_bwd(_c(dout), q, k, v, table, *cfg[:2], keep, starts if ctx.start is None else ctx.start, *cfg[2:], out,
+                                           lse, o32, nq, nk or nv, nt)
+        return dq, dk if nk else None, dv if nv else None, dt, None, None, None
+
+
+def _time_rows(t):
+    return t if t.dim() != 3 or t.shape[2] <= 1 or t.stride(2) == 1 else t.contiguous()
+
+
+def bucket_attention(q, k, v, table, buckets, n_head, keep=None, causal=False, scale=None, q_start=None):
+    """Attention in the conv layout with the learned bias of `buckets` (RelativeBuckets) inside, differentiable in q, k, v and table.
+
+    q [B, H dk, Tq], k, v [B, Hkv dk, Tk] (float32 or bfloat16; any batch and channel strides, e.g. slices of one projection),
+    H = n_head a multiple of Hkv: query head h reads key / value head h // (H / Hkv).  dk <= 128.  table [n_buckets, H], float32 or
+    bfloat16.  keep [B, Tk] float32: 0 hides a key, and whatever k and v hold there has no influence.  causal: a query sees the keys
+    up to its own position.  scale: 1 / sqrt(dk).  q_start: position of query 0 among the keys, an int or an int32 tensor [B] (default
+    Tk - Tq); with causal=True and Tq = 1 a tensor of cached lengths - 1 serves one new token per request from caches of one capacity.
+    A query that sees no key gives zeros and no gradient.  -> [B, H dk, Tq].
+
+    float32 tensors are multiplied in three bf16 parts whatever `conv_precision` says (as the rel-pos attention of the fp32 mode)."""
+    n_head = int(n_head)
+    if n_head < 1:
+        raise ValueError(f"bucket_attention: n_head = {n_head}")
+    q, k, v, table, keep = _time_rows(q), _time_rows(k), _time_rows(v), _c(table), _c(keep)
+    if scale is None:
+        scale = (q.shape[1] // n_head) ** -0.5 if q.dim() == 3 and q.shape[1] >= n_head else 1.0
+    if q_start is None:
+        q_start = k.shape[-1] - q.shape[-1]
+    elif isinstance(q_start, torch.Tensor):
+        q_start = q_start.contiguous()
+    cfg = (buckets.c, n_head, bool(causal), float(scale))
+    if torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, v, table)):
+        return _BucketAttnFn.apply(q, k, v, table, keep, q_start, cfg)
+    return K.bucket_attn_fwd(q, k, v, table, *cfg[:2], keep, q_start, *cfg[2:])
 
 
 class _SsimMapFn(torch.autograd.Function):

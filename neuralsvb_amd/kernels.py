@@ -1034,6 +1034,175 @@ def layernorm_nct_fwd(x, gamma, beta, eps=1e-5):
     return y
 
 
+_DT = {torch.float32: L.SVB_DT_F32, torch.bfloat16: L.SVB_DT_BF16}
+
+
+def _dt(t, what):
+    code = _DT.get(t.dtype)
+    if code is None:
+        raise TypeError(f"{what}: expected float32 or bfloat16, got {t.dtype}")
+    return code
+
+
+def _issue(t, what, fn, *args):
+    """One C-ABI call that launches on t's device, whichever device is current."""
+    idx = t.get_device()
+    if idx < 0 or idx == torch._C._cuda_getDevice():
+        L.check(fn(*args), what)
+    else:
+        with torch.cuda.device(idx):
+            L.check(fn(*args), what)
+
+
+def ln_nct_fwd(x, gamma, beta, eps=1e-5, save_stats=False):
+    """LayerNorm over dim 1 of [B, C, T], fp32 or bf16 -> y, and with save_stats mean, rstd [B, T].  gamma, beta [C] or None, both of
+    x's dtype or both float32."""
+    for t in (gamma, beta):
+        if t is not None and (tuple(t.shape) != (x.shape[1],) or t.dtype not in (x.dtype, torch.float32)):
+            raise ValueError(f"gamma, beta: [{x.shape[1]}] of {x.dtype} or float32, got {tuple(t.shape)} of {t.dtype}")
+    if gamma is not None and beta is not None and gamma.dtype != beta.dtype:
+        raise TypeError("gamma and beta must have one dtype")
+    dt, adt = _dt(x, "ln_nct_fwd"), _dt(gamma if gamma is not None else beta if beta is not None else x, "ln_nct_fwd")
+    lib, st = _prep(x, gamma, beta)
+    B, c, t = x.shape
+    y = torch.empty_like(x)
+    mean = rstd = None
+    if save_stats:
+        mean, rstd = (torch.empty((B, t), device=x.device, dtype=torch.float32) for _ in range(2))
+    if x.numel():
+        _issue(x, "svb_ln_nct_fwd", lib.svb_ln_nct_fwd, _ptr(x), _ptr(gamma), _ptr(beta), _ptr(y), _ptr(mean), _ptr(rstd), B, c, t,
+               float(eps), dt, adt, st)
+    return (y, mean, rstd) if save_stats else y
+
+
+def ln_nct_bwd(x, gamma, dy, mean, rstd, want_dx=True, want_dgamma=True, want_dbeta=True, affine_dtype=torch.float32):
+    """-> dx, dgamma, dbeta (None where not wanted); affine gradients in affine_dtype."""
+    if dy.shape != x.shape or dy.dtype != x.dtype:
+        raise ValueError("dy must have the shape and dtype of x")
+    lib, st = _prep(x, gamma, dy, mean, rstd)
+    B, c, t = x.shape
+    dx = torch.empty_like(x) if want_dx else None
+    dg, db = (torch.empty((c,), device=x.device, dtype=affine_dtype) if w else None for w in (want_dgamma, want_dbeta))
+    if not x.numel():
+        return dx, dg.zero_() if want_dgamma else None, db.zero_() if want_dbeta else None
+    ws = None
+    if want_dgamma or want_dbeta:
+        ws = torch.empty((lib.svb_ln_nct_bwd_workspace_floats(B, c, t, _DT[x.dtype]),), device=x.device, dtype=torch.float32)
+    _issue(x, "svb_ln_nct_bwd", lib.svb_ln_nct_bwd, _ptr(x), _ptr(gamma), _ptr(dy), _ptr(mean), _ptr(rstd), _ptr(dx), _ptr(dg), _ptr(db),
+           _ptr(ws), B, c, t, _DT[x.dtype], _DT[affine_dtype], st)
+    return dx, dg, db
+
+
+def _table_shape(table, buckets, n_head, what):
+    if table.dim() != 2 or table.shape[0] != buckets.n_buckets or (n_head is not None and table.shape[1] != n_head):
+        raise ValueError(f"{what}: table must be [{buckets.n_buckets}, {'heads' if n_head is None else n_head}], got {tuple(table.shape)}")
+
+
+def bucket_bias_fwd(table, buckets, tq, tk, q_start):
+    """table [n_buckets, H] -> bias [H, tq, tk]: table[bucket(j - (q_start + i))].  buckets: an _lib.SvbRelBuckets."""
+    _table_shape(table, buckets, None, "bucket_bias")
+    dt = _dt(table, "bucket_bias")
+    lib, st = _prep(table)
+    out = torch.empty((table.shape[1], tq, tk), device=table.device, dtype=table.dtype)
+    if out.numel():
+        _issue(table, "svb_bucket_bias_fwd", lib.svb_bucket_bias_fwd, _ptr(table), _ptr(out), C.byref(buckets), table.shape[1], tq, tk, q_start,
+               dt, st)
+    return out
+
+
+def bucket_bias_bwd(dbias, buckets, q_start):
+    """dbias [H, tq, tk] -> dtable [n_buckets, H]."""
+    dt = _dt(dbias, "bucket_bias")
+    lib, st = _prep(dbias)
+    h, tq, tk = dbias.shape
+    dtable = torch.empty((buckets.n_buckets, h), device=dbias.device, dtype=dbias.dtype)
+    if not dbias.numel():
+        return dtable.zero_()
+    ws = torch.empty((lib.svb_bucket_bias_bwd_workspace_floats(h, tq, tk, buckets.n_buckets),), device=dbias.device, dtype=torch.float32)
+    _issue(dbias, "svb_bucket_bias_bwd", lib.svb_bucket_bias_bwd, _ptr(dbias), _ptr(dtable), C.byref(buckets), _ptr(ws), h, tq, tk, q_start, dt, st)
+    return dtable
+
+
+def _bucket_attn_desc(q, k, v, table, buckets, n_head, keep, q_start, causal, scale):
+    """The checked call description (lib, stream, SvbBucketAttn without outputs)."""
+    _table_shape(table, buckets, n_head, "bucket_attention")
+    if q.dim() != 3 or k.dim() != 3 or k.shape != v.shape or q.shape[0] != k.shape[0] or q.shape[1] % n_head:
+        raise ValueError(f"bucket_attention: q [B, H dk, Tq], k, v [B, Hkv dk, Tk] with {n_head} heads, got {tuple(q.shape)}, {tuple(k.shape)}, "
+                         f"{tuple(v.shape)}")
+    B, D, tq = q.shape
+    dk, tk = D // n_head, k.shape[2]
+    if not 1 <= dk <= 128 or k.shape[1] % dk or n_head % max(1, k.shape[1] // dk):
+        raise ValueError(f"bucket_attention: {k.shape[1]} key channels are no divisor of {n_head} heads of {dk} channels (at most 128)")
+    if not (q.dtype == k.dtype == v.dtype):
+        raise TypeError("bucket_attention: q, k and v must have one dtype")
+    for t in (q, k, v):
+        if (t.shape[2] > 1 and t.stride(2) != 1) or t.device != q.device:
+            raise ValueError("bucket_attention: q, k, v need unit time stride and one device")
+    d = L.SvbBucketAttn()
+    d.dtype, d.table_dtype = _dt(q, "bucket_attention"), _dt(table, "bucket_attention: table")
+    if keep is not None:
+        _f32(keep)
+        if tuple(keep.shape) != (B, tk):
+            raise ValueError(f"bucket_attention: keep must be [{B}, {tk}], got {tuple(keep.shape)}")
+    if isinstance(q_start, torch.Tensor):
+        if q_start.dtype != torch.int32 or tuple(q_start.shape) != (B,):
+            raise ValueError(f"bucket_attention: q_start must be an int or int32 [{B}]")
+        d.q_start_b, starts = _ptr(q_start), q_start
+    else:
+        d.q_start, starts = int(q_start), None
+    lib, st = _prep(table, keep, starts)
+    if table.get_device() != q.get_device():
+        raise ValueError(f"tensors on different devices: {table.device} vs {q.device}")
+    d.q, d.k, d.v, d.table, d.keep = _ptr(q), _ptr(k), _ptr(v), _ptr(table), _ptr(keep)
+    d.q_sb, d.q_sc, d.k_sb, d.k_sc, d.v_sb, d.v_sc = q.stride(0), q.stride(1), k.stride(0), k.stride(1), v.stride(0), v.stride(1)
+    d.B, d.H, d.Hkv, d.dk, d.Tq, d.Tk = B, n_head, k.shape[1] // dk, dk, tq, tk
+    d.causal, d.scale, d.buckets = int(bool(causal)), float(scale), buckets
+    return lib, st, d
+
+
+def bucket_attn_fwd(q, k, v, table, buckets, n_head, keep, q_start, causal, scale, train=False):
+    """-> out [B, H dk, Tq]; with train also lse [B, H, Tq] and, for bf16 tensors, out in float32 (None for float32)."""
+    lib, st, d = _bucket_attn_desc(q, k, v, table, buckets, n_head, keep, q_start, causal, scale)
+    B, D, tq = q.shape
+    out = torch.empty((B, D, tq), device=q.device, dtype=q.dtype)
+    lse = o32 = None
+    if train:
+        lse = torch.empty((B, n_head, tq), device=q.device, dtype=torch.float32)
+        if q.dtype != torch.float32:
+            o32 = torch.empty((B, D, tq), device=q.device, dtype=torch.float32)
+    if out.numel() and not k.shape[2]:
+        out.zero_()                                    # (no key at all)
+    elif out.numel():
+        d.out, d.lse, d.out_f32 = _ptr(out), _ptr(lse), _ptr(o32)
+        n = lib.svb_bucket_attn_fwd_workspace_floats(C.byref(d))
+        ws = torch.empty((n,), device=q.device, dtype=torch.float32) if n else None
+        _issue(q, "svb_bucket_attn_fwd", lib.svb_bucket_attn_fwd, C.byref(d), _ptr(ws), st)
+    return (out, lse, o32) if train else out
+
+
+def bucket_attn_bwd(dout, q, k, v, table, buckets, n_head, keep, q_start, causal, scale, out, lse, o32, want_q=True, want_kv=True,
+                    want_table=True):
+    """-> dq, (dk, dv), dtable, contiguous, None where not wanted.  out is read for float32 tensors, o32 for bfloat16 ones (the other may
+    be None)."""
+    lib, st, d = _bucket_attn_desc(q, k, v, table, buckets, n_head, keep, q_start, causal, scale)
+    _prep(dout, out, lse, o32)
+    dq = torch.empty(q.shape, device=q.device, dtype=q.dtype) if want_q else None
+    dk, dv = (torch.empty(k.shape, device=q.device, dtype=q.dtype) if want_kv else None for _ in range(2))
+    dt = torch.empty(table.shape, device=q.device, dtype=table.dtype) if want_table else None
+    if not q.numel() or not k.numel():
+        for t in (dq, dk, dv, dt):
+            if t is not None:
+                t.zero_()
+        return dq, dk, dv, dt
+    d.out, d.lse, d.out_f32 = _ptr(o32 if out is None else out), _ptr(lse), _ptr(o32)
+    g = L.SvbBucketAttnGrad()
+    g.dout, g.d_q, g.d_k, g.d_v, g.d_table = _ptr(dout), _ptr(dq), _ptr(dk), _ptr(dv), _ptr(dt)
+    ws = torch.empty((lib.svb_bucket_attn_bwd_workspace_floats(C.byref(d)),), device=q.device, dtype=torch.float32)
+    g.ws = _ptr(ws)
+    _issue(q, "svb_bucket_attn_bwd", lib.svb_bucket_attn_bwd, C.byref(d), C.byref(g), st)
+    return dq, dk, dv, dt
+
+
 def batchnorm_nct_fwd(x, gamma, beta, running_mean, running_var, num_batches, momentum, eps, groups=1, training=True, mask=None):
     """nn.BatchNorm1d on [B,C,T] (csrc/batchnorm.hip): train mode per batch group (running statistics and the batch counter
     updated in place, in group order) -> (y, save [2,groups,C]); eval mode (optionally `* mask[b,t]`) -> (y, None)."""

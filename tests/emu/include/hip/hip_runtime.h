@@ -255,6 +255,8 @@ static inline double __dsub_rn(double a, double b) { volatile double r = a - b; 
 static inline double __dmul_rn(double a, double b) { volatile double r = a * b; return r; }
 static inline double __ddiv_rn(double a, double b) { volatile double r = a / b; return r; }
 #define __expf(x) expf(x)            /* (glibc declares but does not export __expf) */
+#define __log2f(x) log2f(x)
+#define __builtin_amdgcn_exp2f(x) exp2f(x)
 static inline float rsqrtf(float x) { return 1.0f / sqrtf(x); }
 static inline float __frcp_rn(float x) { return 1.0f / x; }
 static inline void sincosf_emu(float x, float* s, float* c) { *s = sinf(x); *c = cosf(x); }
