@@ -5,8 +5,9 @@
 // Scores are computed transposed, S^T = K Q^T, one query per lane column: a query's maximum and sum are 16 registers and one exchange
 // with the other half of the wave, and S^T turns into the B operand of  O^T = V^T P^T  without moving (attn_tiles.h).
 // P is rounded to bf16 for bf16 tensors (relative 2^-9 per weight, averaged over the keys; l sums what was not rounded) and cut into
-// three parts for fp32 tensors.  A training forward of bf16 tensors takes P in two parts: the backward gets delta_i = dout_i . out_i from
-// this output, and the sums of dS over a bucket cancel down to delta's error (table gradient 5e-4 off with one part, below 1e-6 with two).
+// three parts for fp32 tensors.  A training forward of bf16 tensors takes P in three parts too: the backward gets delta_i = dout_i . out_i
+// from this output, and the sums of dS over a bucket cancel down to delta's error (B2 H16/4 dk128 T2048: the table's gradient is 5e-4
+// off with one part, 1e-6 with two, 2e-7 with three, as with 32-bit arithmetic throughout).
 //
 // The bias of a pair is that of its diagonal: a head's table is expanded to one value per offset in LDS.  A tile of keys that lies
 // further than the last bucket border from all queries of a wave has one bias for all its pairs and reads none.
@@ -175,8 +176,8 @@ __global__ __launch_bounds__(256, 1) void svb_bucket_attn_fwd_kernel(SvbBucketAt
                         Tile::col_frag(cols, d, u, x, l31, kb, f);
                         if constexpr (PP == NS) svbt_mma<NS, false>(st.o[d], f, pf);
                         else {
-                            st.o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(f[0], pf[1], st.o[d], 0, 0, 0);
-                            st.o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(f[0], pf[0], st.o[d], 0, 0, 0);
+#pragma unroll
+                            for (int n = PP - 1; n >= 0; --n) st.o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(f[0], pf[n], st.o[d], 0, 0, 0);
                         }
                     }
                 }
@@ -246,7 +247,7 @@ extern "C" int svb_bucket_attn_fwd(const SvbBucketAttn* a, float* ws, void* stre
     return a->dk <= 32 ? fwd_launch<T, 32, KT, true, PP>(a, st) : a->dk <= 64 ? fwd_launch<T, 64, KT, true, PP>(a, st) \
          : a->dk <= 96 ? fwd_launch<T, 96, KT, true, PP>(a, st) : fwd_launch<T, 128, KT, true, PP>(a, st)
     if (a->dtype == SVB_DT_F32) SVB_FWD_GO(float, 32, 3);
-    if (a->lse) SVB_FWD_GO(unsigned short, 64, 2);
+    if (a->lse) SVB_FWD_GO(unsigned short, 64, 3);
     SVB_FWD_GO(unsigned short, 64, 1);
 #undef SVB_FWD_GO
 }
