@@ -593,7 +593,7 @@ int svb_bucket_bias_bwd(const void* dbias, void* dtable, const SvbRelBuckets* bu
  * start = q_start_b[b] where that is given, else q_start.  Keys j with keep[b][j] == 0, and with `causal` those with j > p_i, are
  * hidden: what K and V hold there has no influence.  A query that sees no key gets zeros and passes no gradient.
  * Shared heads: H query heads use Hkv key / value heads, query head h reads head h / (H / Hkv).
- * q [B][H dk][Tq], k, v [B][Hkv dk][Tk]: unit time stride, any batch and channel stride (elements).  dk <= 128.
+ * q [B][H dk][Tq], k, v [B][Hkv dk][Tk]: unit time stride, any batch stride, channel stride 0 ... 2^25 (elements).  dk <= 128.
  * out, dout, dq [B][H dk][Tq], dk, dv [B][Hkv dk][Tk] contiguous.  table, dtable [n_buckets][H] (table_dtype).
  * Training: lse [B][H][Tq] and out_f32 (bf16 tensors only: out before its rounding, [B][H dk][Tq]) are written by the forward and
  * read by the backward; both NULL for inference.                                                                                  */

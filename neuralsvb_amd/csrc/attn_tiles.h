@@ -16,6 +16,7 @@
 // are separate planes in LDS, cut once per workgroup.
 #pragma once
 #include "rel_bucket.h"
+#include <svb_opaque.h>
 
 typedef __bf16 svbt_bf16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 svbt_bf16x2 __attribute__((ext_vector_type(2)));
@@ -83,8 +84,16 @@ __device__ __forceinline__ void svbt_zero(f32x16& a) {
 #pragma unroll
     for (int r = 0; r < 16; ++r) a[r] = 0.f;
 }
-// row of a 32 x 32 result that register r of this lane holds
-__device__ __forceinline__ int svbt_row(int r, int kb) { return 8 * (r >> 2) + 4 * kb + (r & 3); }
+// row of a 32 x 32 result that register r of this lane holds: svbt_reg(r) + 4 kb
+__device__ __forceinline__ constexpr int svbt_reg(int r) { return 8 * (r >> 2) + (r & 3); }
+__device__ __forceinline__ int svbt_row(int r, int kb) { return svbt_reg(r) + 4 * kb; }
+// a value of this tile that the compiler may not take apart: sums of it and 16 or 32 constants would otherwise be split into what changes
+// per tile and what does not, and the latter kept in as many registers through the whole loop
+__device__ __forceinline__ int svbt_fresh(int x) {
+    unsigned u = (unsigned)x;
+    svb_opaque(u);
+    return (int)u;
+}
 
 __device__ __forceinline__ float svbt_load(const float* p) { return *p; }
 __device__ __forceinline__ float svbt_load(const unsigned short* p) { return svb_bf16_f32(*p); }
@@ -185,7 +194,9 @@ struct SvbtTile {
 #pragma unroll
         for (int i = 0; i < NB; ++i) {
             const int id = threadIdx.x + i * NT, d = id / JB * 4, j = j0 + id % JB * 4;
-            if (BLOCKS % NT == 0 || id < BLOCKS) b[i].load(base + d * sc + j, sc, dk - d, T_ - j);
+            long long off = d * sc + j;
+            svb_opaque(off);                                            // (one offset per block through the loop, not one per row)
+            if (BLOCKS % NT == 0 || id < BLOCKS) b[i].load(base + off, sc, dk - d, T_ - j);
         }
     }
     __device__ __forceinline__ void hide(unsigned long long seen) {

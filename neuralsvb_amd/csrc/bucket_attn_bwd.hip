@@ -34,7 +34,7 @@ __device__ __forceinline__ float svbt_ds(float p, float dp, float delta) {
 
 // ---- dq, dtable, delta: 4 waves x 32 queries, keys staged ----------------------------------------------------------------------------
 template <typename T, int DKP, int KT, bool DOUBLE>
-__global__ __launch_bounds__(256, 1) void svb_bucket_attn_dq_kernel(SvbBucketAttn a, SvbBattnBwd g, int qtiles) {
+__global__ __launch_bounds__(256, DKP <= 64 ? 2 : 1) void svb_bucket_attn_dq_kernel(SvbBucketAttn a, SvbBattnBwd g, int qtiles) {
     typedef SvbtTile<T, DKP, KT, 256> Tile;
     constexpr int NS = Tile::NS, NK = DKP / 16, NDB = DKP / 32, NSUB = KT / 32;
     constexpr int BUF = NS * (2 * Tile::ROWS_BYTES + Tile::COLS_BYTES);
@@ -150,15 +150,14 @@ __global__ __launch_bounds__(256, 1) void svb_bucket_attn_dq_kernel(SvbBucketAtt
                 }
 #pragma unroll
                 for (int r = 0; r < 16; ++r) dp[r] -= dp_neg[r];
-                const unsigned su = (unsigned)(now >> (32 * u));
-                const int qo = p - (j0 + 32 * u);
+                const unsigned su = (unsigned)(now >> (32 * u)) >> (4 * kb);
+                const int o0 = svbt_fresh(j0 + 32 * u + 4 * kb - p);     // offset of register row 0
                 if (behind || before) {
                     float sum = 0.f;
 #pragma unroll
                     for (int r = 0; r < 16; ++r) {
-                        const int rw = svbt_row(r, kb);
                         float w = __builtin_amdgcn_exp2f(fmaf(s[r], c, flat) - lse);
-                        if (edge) w = (su >> rw & 1u) && !(a.causal && rw > qo) ? w : 0.f;
+                        if (edge) w = (su >> svbt_reg(r) & 1u) && !(a.causal && o0 + svbt_reg(r) > 0) ? w : 0.f;
                         s[r] = svbt_ds(w, dp[r], delta);
                         sum += s[r];
                     }
@@ -167,9 +166,9 @@ __global__ __launch_bounds__(256, 1) void svb_bucket_attn_dq_kernel(SvbBucketAtt
                 } else {
 #pragma unroll
                     for (int r = 0; r < 16; ++r) {
-                        const int rw = svbt_row(r, kb), o = max(-R, min(R, rw - qo)) + R;
+                        const int o = max(-R, min(R, o0 + svbt_reg(r))) + R;
                         float w = __builtin_amdgcn_exp2f(fmaf(s[r], c, s_bias[o]) - lse);
-                        if (edge) w = (su >> rw & 1u) && !(a.causal && rw > qo) ? w : 0.f;
+                        if (edge) w = (su >> svbt_reg(r) & 1u) && !(a.causal && o0 + svbt_reg(r) > 0) ? w : 0.f;
                         s[r] = svbt_ds(w, dp[r], delta);
                         if (g.part) atomicAdd(&s_sum[(int)s_idx[o] * 256 + threadIdx.x], s[r]);        // (this thread's own slot)
                     }
@@ -221,7 +220,7 @@ __global__ __launch_bounds__(256, 1) void svb_bucket_attn_dq_kernel(SvbBucketAtt
 
 // ---- dk, dv: 4 waves x 32 keys, queries of the heads that share them staged -----------------------------------------------------------
 template <typename T, int DKP, int KT, bool DOUBLE>
-__global__ __launch_bounds__(256, 1) void svb_bucket_attn_dkv_kernel(SvbBucketAttn a, SvbBattnBwd g, int ktiles) {
+__global__ __launch_bounds__(256, DKP <= (SvbtParts<T>::NS == 1 ? 64 : 32) ? 2 : 1) void svb_bucket_attn_dkv_kernel(SvbBucketAttn a, SvbBattnBwd g, int ktiles) {
     typedef SvbtTile<T, DKP, KT, 256> Tile;
     constexpr int NS = Tile::NS, NK = DKP / 16, NDB = DKP / 32, NSUB = KT / 32;
     constexpr int TILE = NS * 2 * (Tile::ROWS_BYTES + Tile::COLS_BYTES), BUF = TILE + 2 * KT * 4;
@@ -305,14 +304,14 @@ __global__ __launch_bounds__(256, 1) void svb_bucket_attn_dkv_kernel(SvbBucketAt
                     Tile::row_frag(drows, u, x, l31, kb, f);
                     svbt_mma<NS, true>(dp, f, vf[x]);
                 }
-                const int jo = j - (pt + 32 * u);                       // offset against query row 0 of the sub-tile
+                const int o0 = svbt_fresh(j - (pt + 32 * u + 4 * kb));   // offset of register row 0
 #pragma unroll
                 for (int r4 = 0; r4 < 4; ++r4) {
                     const float4 ls = *reinterpret_cast<const float4*>(stats + 32 * u + 8 * r4 + 4 * kb);
                     const float4 dl = *reinterpret_cast<const float4*>(stats + KT + 32 * u + 8 * r4 + 4 * kb);
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        const int r = 4 * r4 + e, o = jo - svbt_row(r, kb);
+                        const int r = 4 * r4 + e, o = o0 - svbt_reg(r);
                         float bias = flat;
                         if (!(behind || before)) bias = s_bias[max(-R, min(R, o)) + R];
                         float w = __builtin_amdgcn_exp2f(fmaf(s[r], c, bias) - ls[e]);

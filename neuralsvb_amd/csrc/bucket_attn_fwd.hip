@@ -12,6 +12,7 @@
 // The bias of a pair is that of its diagonal: a head's table is expanded to one value per offset in LDS.  A tile of keys that lies
 // further than the last bucket border from all queries of a wave has one bias for all its pairs and reads none.
 #include "attn_tiles.h"
+#include <type_traits>
 
 // softmax state and output of 32 queries in one wave
 template <int NDB> struct SvbtState {
@@ -20,16 +21,16 @@ template <int NDB> struct SvbtState {
 };
 
 // One 32-key sub-tile's scores -> t (log2 units) in place.  NEAR: the bias varies.  EDGE: some pair is hidden.
-// qo: offset of this lane's query against the first key of the sub-tile, p_i - j0 (keys j0 + row have offset row - qo).
+// o0: offset of register row 0 of this lane, j0 + 4 kb - p_i; seen: the sub-tile's key bits from 4 kb on.
 template <bool NEAR, bool EDGE>
-__device__ __forceinline__ void svbt_scores(f32x16& s, float c, const float* s_bias, int R, float flat, int qo, bool causal, unsigned seen, int kb) {
+__device__ __forceinline__ void svbt_scores(f32x16& s, float c, const float* s_bias, int R, float flat, int o0, bool causal, unsigned seen) {
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
-        const int row = svbt_row(r, kb);
+        const int o = o0 + svbt_reg(r);
         float bias = flat;
-        if (NEAR) bias = s_bias[max(-R, min(R, row - qo)) + R];
+        if (NEAR) bias = s_bias[max(-R, min(R, o)) + R];
         s[r] = fmaf(s[r], c, bias);
-        if (EDGE) s[r] = (seen >> row & 1u) && !(causal && row > qo) ? s[r] : -SVBT_INF;
+        if (EDGE) s[r] = (seen >> svbt_reg(r) & 1u) && !(causal && o > 0) ? s[r] : -SVBT_INF;
     }
 }
 
@@ -67,7 +68,7 @@ __device__ __forceinline__ void svbt_softmax(f32x16 (&s)[NSUB], SvbtState<NDB>& 
 // ---- query tiles: 4 waves x 32 queries, keys staged through LDS, the next tile's loads in flight during this one's products ------------
 // PP: parts of P
 template <typename T, int DKP, int KT, bool DOUBLE, int PP>
-__global__ __launch_bounds__(256, 1) void svb_bucket_attn_fwd_kernel(SvbBucketAttn a, int qtiles) {
+__global__ __launch_bounds__(256, DKP <= 64 ? 2 : 1) void svb_bucket_attn_fwd_kernel(SvbBucketAttn a, int qtiles) {
     typedef SvbtTile<T, DKP, KT, 256> Tile;
     constexpr int NS = Tile::NS, NK = DKP / 16, NDB = DKP / 32, NSUB = KT / 32;
     constexpr int BUF = NS * (Tile::ROWS_BYTES + Tile::COLS_BYTES);
@@ -150,14 +151,14 @@ __global__ __launch_bounds__(256, 1) void svb_bucket_attn_fwd_kernel(SvbBucketAt
             const float flat = behind ? past : ahead;
 #pragma unroll
             for (int u = 0; u < NSUB; ++u) {
-                const unsigned su = (unsigned)(now >> (32 * u));
-                const int qo = p - (j0 + 32 * u);
+                const unsigned su = (unsigned)(now >> (32 * u)) >> (4 * kb);
+                const int o0 = svbt_fresh(j0 + 32 * u + 4 * kb - p);
                 if (behind || before) {
-                    if (edge) svbt_scores<false, true>(s[u], c, s_bias, R, flat, qo, a.causal, su, kb);
-                    else svbt_scores<false, false>(s[u], c, s_bias, R, flat, qo, a.causal, su, kb);
+                    if (edge) svbt_scores<false, true>(s[u], c, s_bias, R, flat, o0, a.causal, su);
+                    else svbt_scores<false, false>(s[u], c, s_bias, R, flat, o0, a.causal, su);
                 } else {
-                    if (edge) svbt_scores<true, true>(s[u], c, s_bias, R, flat, qo, a.causal, su, kb);
-                    else svbt_scores<true, false>(s[u], c, s_bias, R, flat, qo, a.causal, su, kb);
+                    if (edge) svbt_scores<true, true>(s[u], c, s_bias, R, flat, o0, a.causal, su);
+                    else svbt_scores<true, false>(s[u], c, s_bias, R, flat, o0, a.causal, su);
                 }
             }
             svbt_softmax<NSUB, NDB>(s, st);
@@ -210,13 +211,278 @@ __global__ __launch_bounds__(256, 1) void svb_bucket_attn_fwd_kernel(SvbBucketAt
     if (a.lse && kb == 0) a.lse[((size_t)b * a.H + h) * a.Tq + i] = l > 0.f ? st.m + __log2f(l) : SVBT_INF;
 }
 
+// ---- few query rows: the cache's keys split over waves and workgroups ------------------------------------------------------------------
+// A new token per request reads each cached key and value once and computes little: HBM-bound, and one workgroup per head would leave
+// the chip empty.  The rows of a wave are the (query head, query) pairs that share a key / value head (at most 32, so a shared head is read
+// once); every wave takes its own run of keys in tiles of 64, straight from memory to operands:
+//   K: a lane loads the key pair 2 l31, 2 l31 + 1 of a channel (consecutive lanes, whole lines); a permutation makes the even and the odd
+//      keys' operands, two 32-key score tiles.  Register r of tile p is then key 2 row(r) + p, and the registers 4 g .. 4 g + 3 of both tiles,
+//      interleaved, are the eight consecutive keys 16 g + 8 kb + 0..7
+//   V: 16 bytes of consecutive keys of a channel per lane, in just that order.
+// Waves join in LDS, workgroups in a second launch from [split][row] parts (m, l, sum of P v) in memory, in order.
+struct SvbFewParts {
+    float *o, *ml;                 // [item][split][rows][dk], [item][split][rows][2]; NULL: one split, out is written
+    int splits;
+};
+
+// A tile whose 64 keys do not all count (the last one, one with hidden keys) reads 64 keys all the same: it steps back from the end of
+// the rows (Tk >= 64) and counts only what is its own.  Channels that do not exist read one that does: their q is 0, their outputs are
+// not written.
+// Addresses: a uniform row pointer and a 32-bit lane offset (8 channel pitches of at most 2^25 elements).
+template <typename T>
+struct SvbFewRows {
+    const char* row;                   // of channel d
+    long long step, dk, d;
+    unsigned off0, off1;               // this lane's byte offset without and with its 8 kb channels
+    // (opaque, and walked: the loop over tiles would otherwise keep pointers and conditions per row in more scalar registers than there are)
+    __device__ __forceinline__ SvbFewRows(const T* k, long long sc, int j, int kb, int dk_) : row((const char*)k), step(sc * (long long)sizeof(T)), dk(dk_), d(0) {
+        svb_opaque_uniform(step);
+        svb_opaque_uniform(dk);
+        off0 = (unsigned)sizeof(T) * (unsigned)j;
+        off1 = off0 + (unsigned)(8 * kb) * (unsigned)step;
+    }
+    __device__ __forceinline__ const char* next(bool skip8) {             // channel d + 8 kb; then the next (skip8: the next 16's first)
+        const char* p = row + (d + 8 < dk ? off1 : off0);
+        const int n = skip8 ? 9 : 1;
+#pragma unroll
+        for (int i = 0; i < n; ++i, ++d) row += d + 1 < dk ? step : 0;
+        return p;
+    }
+};
+template <typename T, int NK> struct SvbFewKeys;
+template <int NK> struct SvbFewKeys<unsigned short, NK> {
+    unsigned r[NK][8];                                                  // (even | odd << 16) of channel 16 s + 8 kb + e
+    __device__ __forceinline__ void load(SvbFewRows<unsigned short> rows) {
+#pragma unroll
+        for (int s = 0; s < NK; ++s)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) __builtin_memcpy(&r[s][e], rows.next(e == 7), 4);
+    }
+    __device__ __forceinline__ void frag(int s, int p, svbt_bf16x8 (&f)[1]) const {
+        unsigned u[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const unsigned a = r[s][2 * e], b = r[s][2 * e + 1];
+            u[e] = p ? a >> 16 | (b & 0xffff0000u) : (a & 0xffffu) | b << 16;
+        }
+        __builtin_memcpy(&f[0], u, 16);
+    }
+};
+template <int NK> struct SvbFewKeys<float, NK> {
+    float r[NK][8][2];
+    __device__ __forceinline__ void load(SvbFewRows<float> rows) {
+#pragma unroll
+        for (int s = 0; s < NK; ++s)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) __builtin_memcpy(r[s][e], rows.next(e == 7), 8);
+    }
+    __device__ __forceinline__ void frag(int s, int p, svbt_bf16x8 (&f)[3]) const {
+        float v[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = r[s][e][p];
+        svbt_frag8<3>(v, f);
+    }
+};
+// eight consecutive keys of one channel as loaded, and as operand; `seen`: the bits of those that count (the others become zero)
+template <typename T> struct SvbFewValues;
+template <> struct SvbFewValues<unsigned short> {
+    unsigned r[4];
+    __device__ __forceinline__ void load(const unsigned short* p) { __builtin_memcpy(r, p, 16); }
+    template <bool FULL>
+    __device__ __forceinline__ void frag(unsigned seen, svbt_bf16x8 (&f)[1]) const {
+        unsigned u[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            u[e] = FULL ? r[e] : r[e] & ((seen >> (2 * e) & 1 ? 0xffffu : 0u) | (seen >> (2 * e + 1) & 1 ? 0xffff0000u : 0u));
+        __builtin_memcpy(&f[0], u, 16);
+    }
+};
+template <> struct SvbFewValues<float> {
+    float r[8];
+    __device__ __forceinline__ void load(const float* p) { __builtin_memcpy(r, p, 32); }
+    template <bool FULL>
+    __device__ __forceinline__ void frag(unsigned seen, svbt_bf16x8 (&f)[3]) const {
+        float v[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = FULL || (seen >> e & 1) ? r[e] : 0.f;
+        svbt_frag8<3>(v, f);
+    }
+};
+
+template <typename T, int DKP>
+__global__ __launch_bounds__(256, DKP * SvbtParts<T>::NS > 192 || DKP == 128 ? 1 : 2) void svb_bucket_attn_few_kernel(SvbBucketAttn a, SvbFewParts parts) {
+    constexpr int NS = SvbtParts<T>::NS, NK = DKP / 16, NDB = DKP / 32;
+    HIP_DYNAMIC_SHARED(char, smem)
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l31 = lane & 31, kb = lane >> 5;
+    const int split = blockIdx.x, hk = blockIdx.y, b = blockIdx.z;
+    const int G = a.H / a.Hkv, rows = G * a.Tq, nb = a.buckets.n_buckets, R = svb_bucket_reach(a.buckets);
+    float* s_tab = (float*)smem;                                        // [G][nb]
+    unsigned char* s_idx = (unsigned char*)(s_tab + G * nb);             // [2 R + 1]
+    for (int e = threadIdx.x; e < G * nb; e += 256)
+        s_tab[e] = svb_ld_table(a.table, (size_t)(e % nb) * a.H + hk * G + e / nb, a.table_dtype == SVB_DT_BF16) * SVBT_LOG2E;
+    for (int o = threadIdx.x; o <= 2 * R; o += 256) s_idx[o] = (unsigned char)svb_bucket_of(a.buckets, o - R);
+
+    const bool has = l31 < rows;
+    const int hl = has ? l31 / a.Tq : 0, i = has ? l31 - hl * a.Tq : 0, h = hk * G + hl;
+    const T* q = (const T*)a.q + b * a.q_sb + (long long)h * a.dk * a.q_sc;
+    const T* k = (const T*)a.k + b * a.k_sb + (long long)hk * a.dk * a.k_sc;
+    const T* v = (const T*)a.v + b * a.v_sb + (long long)hk * a.dk * a.v_sc;
+    const float* keep = a.keep ? a.keep + (size_t)b * a.Tk : nullptr;
+    svbt_bf16x8 qf[NK][NS];
+#pragma unroll
+    for (int s = 0; s < NK; ++s) svbt_own_frag<T, NS>(q, a.q_sc, i, s, kb, a.dk, has, qf[s]);
+
+    const int start = svbt_start(a, b), p = start + i;
+    const int end = a.causal ? max(0, min(a.Tk, start + a.Tq)) : a.Tk;
+    // this wave's run of keys: whole tiles of 64, even over all waves of all splits
+    const int tiles = (end + 63) / 64, runs = parts.splits * 4, run = split * 4 + wave;
+    const int per = (tiles + runs - 1) / runs, t0 = min(run * per, tiles), t1 = min(t0 + per, tiles);
+    const float c = a.scale * SVBT_LOG2E;
+    SvbtState<NDB> st;
+#pragma unroll
+    for (int d = 0; d < NDB; ++d) svbt_zero(st.o[d]);
+    st.m = -SVBT_INF;
+    st.l = 0.f;
+    __syncthreads();
+    const float* tab = s_tab + hl * nb;
+    const float past = tab[s_idx[0]], ahead = tab[s_idx[2 * R]];
+
+    long long vrow[NDB];                                                // this lane's channel (one that exists) of V, from key 8 kb on
+#pragma unroll
+    for (int d = 0; d < NDB; ++d) vrow[d] = min(32 * d + l31, a.dk - 1) * a.v_sc + 8 * kb;
+    auto tile = [&](int t, auto full_c) {
+        constexpr bool FULL = decltype(full_c)::value;                   // 64 keys, all of them seen by every row
+        const int j0 = FULL ? 64 * t : min(64 * t, a.Tk - 64);
+        SvbFewKeys<T, NK> kt;
+        kt.load(SvbFewRows<T>(k, a.k_sc, j0 + 2 * l31, kb, a.dk));
+        unsigned long long seen = ~0ull;
+        if (!FULL) seen = __ballot(j0 + lane >= 64 * t && j0 + lane < end && (!keep || keep[j0 + lane] != 0.f));
+        SvbFewValues<T> vt[4][NDB];
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+#pragma unroll
+            for (int d = 0; d < NDB; ++d) {
+                vt[g][d].load(v + vrow[d] + (j0 + 16 * g));
+            }
+        if (seen == 0ull) return;                                       // (wave-uniform)
+        f32x16 s[2];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            svbt_zero(s[u]);
+#pragma unroll
+            for (int x = 0; x < NK; ++x) {
+                svbt_bf16x8 f[NS];
+                kt.frag(x, u, f);
+                svbt_mma<NS, false>(s[u], f, qf[x]);
+            }
+        }
+        const bool flat = j0 + 63 - start <= -R || j0 - (start + a.Tq - 1) >= R;
+        const float fb = j0 + 63 - start <= -R ? past : ahead;
+        // key of register r of tile u: 2 svbt_reg(r) + u + 8 kb
+        const int o0 = svbt_fresh(j0 + 8 * kb - p);
+        const unsigned w0 = (unsigned)seen >> (8 * kb), w1 = (unsigned)(seen >> 32) >> (8 * kb);
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                const int key = 2 * svbt_reg(r) + u, o = o0 + key;
+                float bias = fb;
+                if (!flat) bias = tab[s_idx[max(-R, min(R, o)) + R]];
+                s[u][r] = fmaf(s[u][r], c, bias);
+                if (!FULL) s[u][r] = ((r < 8 ? w0 : w1) >> (key & 31) & 1u) && !(a.causal && o > 0) ? s[u][r] : -SVBT_INF;
+            }
+        svbt_softmax<2, NDB>(s, st);
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            float w[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) w[e] = s[e & 1][4 * g + (e >> 1)];
+            svbt_bf16x8 pf[NS];
+            svbt_frag8<NS>(w, pf);
+#pragma unroll
+            for (int d = 0; d < NDB; ++d) {
+                svbt_bf16x8 f[NS];
+                vt[g][d].template frag<FULL>((unsigned)(seen >> (16 * g + 8 * kb)), f);
+                svbt_mma<NS, false>(st.o[d], f, pf);
+            }
+        }
+    };
+    // whole tiles first, the others behind them: two loops, since one with both bodies keeps both bodies' registers alive
+    const int whole = keep ? t0 : max(t0, min(t1, (a.causal ? min(end, start + 1) : end) / 64));
+    for (int t = t0; t < whole; ++t) tile(t, std::true_type{});
+    for (int t = whole; t < t1; ++t) tile(t, std::false_type{});
+    st.l += __shfl_xor(st.l, 32, 64);
+
+    // join of the four waves
+    __syncthreads();                                                    // (the tables are read)
+    float* s_ml = (float*)smem;                                         // [4][32][2]
+    float* s_o = s_ml + 256;                                            // [4][DKP][32]
+    if (kb == 0) { s_ml[(wave * 32 + l31) * 2] = st.m; s_ml[(wave * 32 + l31) * 2 + 1] = st.l; }
+#pragma unroll
+    for (int d = 0; d < NDB; ++d)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s_o[(wave * DKP + 32 * d + svbt_row(r, kb)) * 32 + l31] = st.o[d][r];
+    __syncthreads();
+    const size_t item = ((size_t)b * a.Hkv + hk) * parts.splits + split;
+    for (int e = threadIdx.x; e < rows * a.dk; e += 256) {
+        const int ch = e / rows, r = e - ch * rows;                     // (rows innermost: LDS in order)
+        float m = -SVBT_INF, l = 0.f, o = 0.f;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) m = fmaxf(m, s_ml[(w * 32 + r) * 2]);
+        const float m_use = m == -SVBT_INF ? 0.f : m;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            const float f = __builtin_amdgcn_exp2f(s_ml[(w * 32 + r) * 2] - m_use);
+            l = fmaf(s_ml[(w * 32 + r) * 2 + 1], f, l);
+            o = fmaf(s_o[(w * DKP + ch) * 32 + r], f, o);
+        }
+        const int g = r / a.Tq, i2 = r - g * a.Tq;
+        if (!parts.o) {
+            const float inv = l > 0.f ? 1.f / l : 0.f;
+            svbt_store((T*)a.out + (((size_t)b * a.H + hk * G + g) * a.dk + ch) * a.Tq + i2, o * inv);
+        } else {
+            parts.o[(item * rows + r) * a.dk + ch] = o;
+            if (ch == 0) { parts.ml[(item * rows + r) * 2] = m; parts.ml[(item * rows + r) * 2 + 1] = l; }
+        }
+    }
+}
+
+// out of one (batch entry, key / value head, row) from its splits: one wave, lanes along the channels
+template <typename T>
+__global__ __launch_bounds__(256) void svb_bucket_attn_join_kernel(SvbBucketAttn a, SvbFewParts parts, int total) {
+    const int id = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
+    if (id >= total) return;
+    const int G = a.H / a.Hkv, rows = G * a.Tq, r = id % rows, bh = id / rows, b = bh / a.Hkv, hk = bh - b * a.Hkv;
+    const float* ml = parts.ml + ((size_t)bh * parts.splits * rows + r) * 2;
+    float m = -SVBT_INF;
+    for (int s = lane; s < parts.splits; s += 64) m = fmaxf(m, ml[(size_t)s * rows * 2]);
+    m = svb_wave_max(m);
+    const float m_use = m == -SVBT_INF ? 0.f : m;
+    float l = 0.f, o[2] = {0.f, 0.f};
+    const float* po = parts.o + ((size_t)bh * parts.splits * rows + r) * a.dk;
+    for (int s = 0; s < parts.splits; ++s) {
+        const float f = __builtin_amdgcn_exp2f(ml[(size_t)s * rows * 2] - m_use);
+        l = fmaf(ml[(size_t)s * rows * 2 + 1], f, l);
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+            if (lane + 64 * u < a.dk) o[u] = fmaf(po[(size_t)s * rows * a.dk + lane + 64 * u], f, o[u]);
+    }
+    const float inv = l > 0.f ? 1.f / l : 0.f;
+    const int g = r / a.Tq, i = r - g * a.Tq;
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+        if (lane + 64 * u < a.dk) svbt_store((T*)a.out + (((size_t)b * a.H + hk * G + g) * a.dk + lane + 64 * u) * a.Tq + i, o[u] * inv);
+}
+
 // ---- host ------------------------------------------------------------------------------------------------------------------------
 int svb_bucket_attn_check(const SvbBucketAttn* a) {
     if (!a || !a->q || !a->k || !a->v || !a->table || !a->out) return SVB_ERR_ARG;
     if (a->B <= 0 || a->H <= 0 || a->Hkv <= 0 || a->dk <= 0 || a->Tq <= 0 || a->Tk <= 0 || a->H % a->Hkv) return SVB_ERR_ARG;
     if (!svb_bucket_valid(&a->buckets)) return SVB_ERR_ARG;
     if ((a->dtype != SVB_DT_F32 && a->dtype != SVB_DT_BF16) || (a->table_dtype != SVB_DT_F32 && a->table_dtype != SVB_DT_BF16)) return SVB_ERR_UNSUPPORTED;
-    if (a->dk > 128 || a->Tq > (1 << 28) || a->Tk > (1 << 28) || a->q_start < -(1 << 28) || a->q_start > (1 << 28)) return SVB_ERR_UNSUPPORTED;
+    // (channel pitches: a lane's offset over 16 channels stays in 32 bits)
+    if (a->q_sc < 0 || a->q_sc > (1 << 25) || a->k_sc < 0 || a->k_sc > (1 << 25) || a->v_sc < 0 || a->v_sc > (1 << 25)) return SVB_ERR_UNSUPPORTED;
+    if (a->dk > 128 || a->Tq > (1 << 25) || a->Tk > (1 << 25) || a->q_start < -(1 << 28) || a->q_start > (1 << 28)) return SVB_ERR_UNSUPPORTED;
     if ((long)a->B * a->H * ((a->Tq + 31) / 32) > 0x7fffffffL || (long)a->B * a->Hkv * ((a->Tk + 31) / 32) > 0x7fffffffL) return SVB_ERR_UNSUPPORTED;
     return SVB_OK;
 }
@@ -233,16 +499,54 @@ static int fwd_launch(const SvbBucketAttn* a, hipStream_t st) {
     return SVB_OK;
 }
 
+// Few rows: what a wave holds in its 32 columns, a tile of keys at least, and nothing kept for a backward.  Splits: enough workgroups for two per CU, at least
+// 256 keys (a tile for each wave) in each; 0: not this form.
+static int few_splits(const SvbBucketAttn* a) {
+    if (a->lse || (long)(a->H / a->Hkv) * a->Tq > 32 || a->Tk < 64 || a->B > 65535 || a->Hkv > 65535) return 0;
+    const int most = (a->Tk + 255) / 256, want = 512 / max(1, min(512, a->B * a->Hkv));
+    return max(1, min(most, want));
+}
+
 extern "C" size_t svb_bucket_attn_fwd_workspace_floats(const SvbBucketAttn* a) {
-    (void)a;
-    return 0;
+    if (!a || a->B <= 0 || a->H <= 0 || a->Hkv <= 0 || a->Tq <= 0 || a->Tk <= 0 || a->dk <= 0) return 0;
+    const int n = few_splits(a);
+    return n > 1 ? (size_t)a->B * a->H * a->Tq * n * (a->dk + 2) : 0;
+}
+
+template <typename T, int DKP>
+static int few_launch(const SvbBucketAttn* a, float* ws, int splits, hipStream_t st) {
+    const int G = a->H / a->Hkv, rows = G * a->Tq;
+    SvbFewParts parts = {nullptr, nullptr, splits};
+    if (splits > 1) {
+        parts.o = ws;
+        parts.ml = ws + (size_t)a->B * a->H * a->Tq * splits * a->dk;
+    }
+    const int tables = G * a->buckets.n_buckets * 4 + 2 * svb_bucket_reach(a->buckets) + 1, join = (256 + 4 * DKP * 32) * 4;
+    const int lds = tables > join ? tables : join;
+    auto* kern = svb_bucket_attn_few_kernel<T, DKP>;
+    if (lds > 65536 && hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024) != hipSuccess) return SVB_ERR_LAUNCH;
+    hipLaunchKernelGGL(kern, dim3((unsigned)splits, (unsigned)a->Hkv, (unsigned)a->B), dim3(256), lds, st, *a, parts);
+    SVB_CHECK_LAUNCH();
+    if (splits > 1) {
+        const int total = a->B * a->Hkv * rows;
+        hipLaunchKernelGGL((svb_bucket_attn_join_kernel<T>), dim3((unsigned)((total + 3) / 4)), dim3(256), 0, st, *a, parts, total);
+        SVB_CHECK_LAUNCH();
+    }
+    return SVB_OK;
 }
 
 extern "C" int svb_bucket_attn_fwd(const SvbBucketAttn* a, float* ws, void* stream) {
-    (void)ws;
     const int rc = svb_bucket_attn_check(a);
     if (rc != SVB_OK) return rc;
     hipStream_t st = (hipStream_t)stream;
+    const int splits = few_splits(a);
+    if (splits > 1 && !ws) return SVB_ERR_ARG;
+#define SVB_FEW_GO(T)                                                                                              \
+    return a->dk <= 32 ? few_launch<T, 32>(a, ws, splits, st) : a->dk <= 64 ? few_launch<T, 64>(a, ws, splits, st) \
+         : a->dk <= 96 ? few_launch<T, 96>(a, ws, splits, st) : few_launch<T, 128>(a, ws, splits, st)
+    if (splits && a->dtype == SVB_DT_F32) SVB_FEW_GO(float);
+    if (splits) SVB_FEW_GO(unsigned short);
+#undef SVB_FEW_GO
 #define SVB_FWD_GO(T, KT, PP)                                                                                     \
     return a->dk <= 32 ? fwd_launch<T, 32, KT, true, PP>(a, st) : a->dk <= 64 ? fwd_launch<T, 64, KT, true, PP>(a, st) \
          : a->dk <= 96 ? fwd_launch<T, 96, KT, true, PP>(a, st) : fwd_launch<T, 128, KT, true, PP>(a, st)
