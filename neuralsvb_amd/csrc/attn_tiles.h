@@ -101,35 +101,43 @@ __device__ __forceinline__ void svbt_store(float* p, float v) { *p = v; }
 __device__ __forceinline__ void svbt_store(unsigned short* p, float v) { *p = (unsigned short)svbt_pack2(v, v); }
 
 // Operand of this lane's own column t (position) for the channels 16 s + 8 kb + 0..7: read once per workgroup, 32 lanes along time.
-// `has` false or a channel beyond dk: zeros (whatever memory holds there).
+// `has` false or a channel beyond dk: zeros, whatever memory holds there.  Read without a branch (t has to exist, a channel that does
+// not exist reads the last one): a load under a condition is waited for before the next one, and a workgroup begins with dk of them.
+template <typename T>
+__device__ __forceinline__ void svbt_own8(const T* base, long long sc, int t, int s, int kb, int dk, bool has, float (&v)[8]) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = svbt_load(base + min(16 * s + 8 * kb + e, dk - 1) * sc + t);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = has && 16 * s + 8 * kb + e < dk ? v[e] : 0.f;
+}
 template <typename T, int NS>
 __device__ __forceinline__ void svbt_own_frag(const T* base, long long sc, int t, int s, int kb, int dk, bool has, svbt_bf16x8 (&f)[NS]) {
     float v[8];
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-        const int d = 16 * s + 8 * kb + e;
-        v[e] = has && d < dk ? svbt_load(base + d * sc + t) : 0.f;
-    }
+    svbt_own8(base, sc, t, s, kb, dk, has, v);
     svbt_frag8<NS>(v, f);
 }
 
 // ---- staged tiles ----------------------------------------------------------------------------------------------------------
-// One 4 channel x 4 position block as loaded.
+// One 4 channel x 4 position block as loaded.  row(c): the c-th channel's four elements, any element-aligned address.
 template <typename T> struct SvbtBlock;
 template <> struct SvbtBlock<unsigned short> {
     unsigned r[4][2];
-    __device__ __forceinline__ void load(const unsigned short* p, long long sc, int rows, int n) {      // rows, n: channels / positions that exist
+    __device__ __forceinline__ void row(int c, const unsigned short* p) {
+        const svbt_u2u t = *reinterpret_cast<const svbt_u2u*>(p);
+        r[c][0] = t.x;
+        r[c][1] = t.y;
+    }
+    __device__ __forceinline__ void row_n(int c, const unsigned short* p, int n) {                       // n < 4 elements
+        r[c][0] = (n > 0 ? (unsigned)p[0] : 0u) | (n > 1 ? (unsigned)p[1] << 16 : 0u);
+        r[c][1] = n > 2 ? (unsigned)p[2] : 0u;
+    }
+    // the block was loaded `by` elements too early (4 or more: nothing of it exists)
+    __device__ __forceinline__ void shift(int by) {
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
-            r[c][0] = r[c][1] = 0u;
-            if (c < rows) {
-                if (n >= 4) { const svbt_u2u t = *reinterpret_cast<const svbt_u2u*>(p + c * sc); r[c][0] = t.x; r[c][1] = t.y; }
-                else {
-                    if (n > 0) r[c][0] = p[c * sc];
-                    if (n > 1) r[c][0] |= (unsigned)p[c * sc + 1] << 16;
-                    if (n > 2) r[c][1] = p[c * sc + 2];
-                }
-            }
+            const unsigned long long v = by < 4 ? ((unsigned long long)r[c][1] << 32 | r[c][0]) >> (16 * by) : 0ull;
+            r[c][0] = (unsigned)v;
+            r[c][1] = (unsigned)(v >> 32);
         }
     }
     // positions whose bit is not set become zero
@@ -145,21 +153,22 @@ template <> struct SvbtBlock<unsigned short> {
 };
 template <> struct SvbtBlock<float> {
     float r[4][4];
-    __device__ __forceinline__ void load(const float* p, long long sc, int rows, int n) {
+    __device__ __forceinline__ void row(int c, const float* p) {
+        const svbt_f4u t = *reinterpret_cast<const svbt_f4u*>(p);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) r[c][e] = t[e];
+    }
+    __device__ __forceinline__ void row_n(int c, const float* p, int n) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) r[c][e] = e < n ? p[e] : 0.f;
+    }
+    __device__ __forceinline__ void shift(int by) {
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
+            if (by & 2) { r[c][0] = r[c][2]; r[c][1] = r[c][3]; r[c][2] = r[c][3] = 0.f; }
+            if (by & 1) { r[c][0] = r[c][1]; r[c][1] = r[c][2]; r[c][2] = r[c][3]; r[c][3] = 0.f; }
 #pragma unroll
-            for (int e = 0; e < 4; ++e) r[c][e] = 0.f;
-            if (c < rows) {
-                if (n >= 4) {
-                    const svbt_f4u t = *reinterpret_cast<const svbt_f4u*>(p + c * sc);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) r[c][e] = t[e];
-                } else {
-#pragma unroll
-                    for (int e = 0; e < 3; ++e) if (e < n) r[c][e] = p[c * sc + e];
-                }
-            }
+            for (int e = 0; e < 4; ++e) r[c][e] = by < 4 ? r[c][e] : 0.f;
         }
     }
     __device__ __forceinline__ void hide(unsigned seen) {
@@ -181,27 +190,46 @@ template <> struct SvbtBlock<float> {
     }
 };
 
-// KT positions x DKP channels of one tensor: NB blocks per thread of NT threads
-template <typename T, int DKP, int KT, int NT>
+// KT positions x DKP channels of one tensor: NB blocks per thread of NT threads.
+// A block that reaches over the end of the rows is loaded earlier, so that it ends with them, and moved into place before it is stored:
+// the loads have no branches and stay in flight together.  A channel >= dk reads channel dk - 1: own operands are 0 there, and result
+// rows of such channels are not written.
+// TINY: rows of less than 4 elements, read one by one (a form of its own: with both in one loop the loads are waited for where they join).
+template <typename T, int DKP, int KT, int NT, bool TINY>
 struct SvbtTile {
     static constexpr int NS = SvbtParts<T>::NS, JB = KT / 4, BLOCKS = JB * (DKP / 4), NB = (BLOCKS + NT - 1) / NT;
     static constexpr int ROWP = 2 * DKP + 16, COLP = 2 * KT + 16;                       // pitches, bytes
     static constexpr int ROWS_BYTES = KT * ROWP, COLS_BYTES = DKP * COLP;              // one part's plane
     SvbtBlock<T> b[NB];
 
-    // positions j0 .. j0 + KT - 1 of [dk][.] rows at `base`; positions >= T_ and channels >= dk read as zero
-    __device__ __forceinline__ void load(const T* base, long long sc, int j0, int T_, int dk) {
+    // positions j0 .. j0 + KT - 1 of rows of L elements at `base`, channel pitch sc (<= 2^25)
+    __device__ __forceinline__ void load(const T* base, long long sc, int j0, int L, int dk) {
 #pragma unroll
         for (int i = 0; i < NB; ++i) {
-            const int id = threadIdx.x + i * NT, d = id / JB * 4, j = j0 + id % JB * 4;
-            long long off = d * sc + j;
+            const int id = threadIdx.x + i * NT, j = j0 + id % JB * 4;
+            if (BLOCKS % NT != 0 && id >= BLOCKS) continue;
+            const int d = min(id / JB * 4, dk - 1), more = dk - 1 - d;
+            long long off = (long long)d * sc + max(0, min(j, L - 4));
             svb_opaque(off);                                            // (one offset per block through the loop, not one per row)
-            if (BLOCKS % NT == 0 || id < BLOCKS) b[i].load(base + off, sc, dk - d, T_ - j);
+            const T* p = base + off;
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                const T* pc = p + (size_t)(unsigned)min(c, more) * (unsigned)sc;
+                if (TINY) b[i].row_n(c, pc, L - j);
+                else b[i].row(c, pc);
+            }
         }
     }
-    __device__ __forceinline__ void hide(unsigned long long seen) {
+    // after the loads: blocks over the end into place, and positions whose bit is not set to zero (`seen` == ~0: all count)
+    __device__ __forceinline__ void settle(int j0, int L, unsigned long long seen) {
+        if (!TINY && j0 + KT > L) {                                     // (uniform, as the next)
 #pragma unroll
-        for (int i = 0; i < NB; ++i) b[i].hide((unsigned)(seen >> ((threadIdx.x + i * NT) % JB * 4)) & 15u);
+            for (int i = 0; i < NB; ++i) b[i].shift(max(0, j0 + (int)(threadIdx.x + i * NT) % JB * 4 - (L - 4)));
+        }
+        if (seen != ~0ull) {
+#pragma unroll
+            for (int i = 0; i < NB; ++i) b[i].hide((unsigned)(seen >> ((threadIdx.x + i * NT) % JB * 4)) & 15u);
+        }
     }
     template <bool ROWS, bool COLS>
     __device__ __forceinline__ void store(char* rows, char* cols) const {
@@ -260,10 +288,6 @@ __device__ __forceinline__ int svbt_start(const SvbBucketAttn& a, int b) {
 __device__ __forceinline__ void svbt_fill_bias(float* s_bias, const SvbBucketAttn& a, int h, int R, int nt) {
     for (int o = threadIdx.x; o <= 2 * R; o += nt)
         s_bias[o] = svb_ld_table(a.table, (size_t)svb_bucket_of(a.buckets, o - R) * a.H + h, a.table_dtype == SVB_DT_BF16) * SVBT_LOG2E;
-}
-// bits of the keys j0 .. j0 + 63 that exist (j < end) and are kept
-__device__ __forceinline__ unsigned long long svbt_keep_bits(float keep, int j0, int end, int lane) {
-    return __ballot(j0 + lane < end && keep != 0.f);
 }
 // last kept key + 1 of a batch entry (0: none), by one wave; 512 keys' loads in flight, from the end
 __device__ __forceinline__ int svbt_keep_end(const float* keep, int n, int lane) {

@@ -33,9 +33,9 @@ __device__ __forceinline__ float svbt_ds(float p, float dp, float delta) {
 }
 
 // ---- dq, dtable, delta: 4 waves x 32 queries, keys staged ----------------------------------------------------------------------------
-template <typename T, int DKP, int KT, bool DOUBLE>
+template <typename T, int DKP, int KT, bool DOUBLE, bool TINY>
 __global__ __launch_bounds__(256, DKP <= 64 ? 2 : 1) void svb_bucket_attn_dq_kernel(SvbBucketAttn a, SvbBattnBwd g, int qtiles) {
-    typedef SvbtTile<T, DKP, KT, 256> Tile;
+    typedef SvbtTile<T, DKP, KT, 256, TINY> Tile;
     constexpr int NS = Tile::NS, NK = DKP / 16, NDB = DKP / 32, NSUB = KT / 32;
     constexpr int BUF = NS * (2 * Tile::ROWS_BYTES + Tile::COLS_BYTES);
     HIP_DYNAMIC_SHARED(char, smem)
@@ -52,19 +52,19 @@ __global__ __launch_bounds__(256, DKP <= 64 ? 2 : 1) void svb_bucket_attn_dq_ker
     const size_t head = ((size_t)b * a.H + h) * a.dk * a.Tq;
     const T* dout = (const T*)g.dout + head;
     const float* out = (NS == 3 ? (const float*)a.out : a.out_f32) + head;
-    const size_t row = ((size_t)b * a.H + h) * a.Tq + (has ? i : 0);
+    const int ic = has ? i : 0;
+    const size_t row = ((size_t)b * a.H + h) * a.Tq + ic;
     svbt_bf16x8 qf[NK][NS], of[NK][NS];
     float delta = 0.f;
 #pragma unroll
     for (int s = 0; s < NK; ++s) {
-        svbt_own_frag<T, NS>(q, a.q_sc, i, s, kb, a.dk, has, qf[s]);
-        float v[8];
+        svbt_own_frag<T, NS>(q, a.q_sc, ic, s, kb, a.dk, has, qf[s]);
+        float v[8], o[8];
+        svbt_own8(dout, a.Tq, ic, s, kb, a.dk, has, v);
+        svbt_own8(out, a.Tq, ic, s, kb, a.dk, has, o);
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-            const int d = 16 * s + 8 * kb + e;
-            const bool in = has && d < a.dk;
-            v[e] = in ? svbt_load(dout + (size_t)d * a.Tq + i) : 0.f;
-            delta = fmaf(v[e], in ? out[(size_t)d * a.Tq + i] : 0.f, delta);
+            delta = fmaf(v[e], o[e], delta);
             if (s & 1) v[e] = -v[e];                                    // (see dp_neg below)
         }
         svbt_frag8<NS>(v, of[s]);
@@ -98,17 +98,19 @@ __global__ __launch_bounds__(256, DKP <= 64 ? 2 : 1) void svb_bucket_attn_dq_ker
     float sum_past = 0.f, sum_ahead = 0.f;
 
     Tile tk, tv;
-    unsigned long long seen = ~0ull;
+    unsigned long long seen = ~0ull;                                    // of the tile in LDS: the keys that exist and are kept
+    float kept = 1.f;
     constexpr unsigned long long ALL = KT == 64 ? ~0ull : 0xffffffffull;
     auto fetch = [&](int t) {
-        tk.load(k, a.k_sc, t * KT, end, a.dk);
-        tv.load(v, a.v_sc, t * KT, end, a.dk);
+        tk.load(k, a.k_sc, t * KT, a.Tk, a.dk);
+        tv.load(v, a.v_sc, t * KT, a.Tk, a.dk);
+        if (keep) kept = keep[min(t * KT + lane, a.Tk - 1)];
     };
-    auto bits = [&](int t) {
-        return ALL & (keep ? svbt_keep_bits(keep[min(t * KT + lane, a.Tk - 1)], t * KT, end, lane) : __ballot(t * KT + lane < end));
-    };
+    auto bits = [&](int t) { return ALL & __ballot(t * KT + lane < end && kept != 0.f); };
     auto put = [&](int t) {
-        if (keep) { tk.hide(seen); tv.hide(seen); }
+        const unsigned long long m = seen == ALL ? ~0ull : seen;
+        tk.settle(t * KT, a.Tk, m);
+        tv.settle(t * KT, a.Tk, m);
         char* buf = smem + (DOUBLE ? (t & 1) * BUF : 0);
         tk.template store<true, true>(buf, buf + 2 * NS * Tile::ROWS_BYTES);
         tv.template store<true, false>(buf + NS * Tile::ROWS_BYTES, nullptr);
@@ -219,9 +221,9 @@ __global__ __launch_bounds__(256, DKP <= 64 ? 2 : 1) void svb_bucket_attn_dq_ker
 }
 
 // ---- dk, dv: 4 waves x 32 keys, queries of the heads that share them staged -----------------------------------------------------------
-template <typename T, int DKP, int KT, bool DOUBLE>
+template <typename T, int DKP, int KT, bool DOUBLE, bool TINY>
 __global__ __launch_bounds__(256, DKP <= (SvbtParts<T>::NS == 1 ? 64 : 32) ? 2 : 1) void svb_bucket_attn_dkv_kernel(SvbBucketAttn a, SvbBattnBwd g, int ktiles) {
-    typedef SvbtTile<T, DKP, KT, 256> Tile;
+    typedef SvbtTile<T, DKP, KT, 256, TINY> Tile;
     constexpr int NS = Tile::NS, NK = DKP / 16, NDB = DKP / 32, NSUB = KT / 32;
     constexpr int TILE = NS * 2 * (Tile::ROWS_BYTES + Tile::COLS_BYTES), BUF = TILE + 2 * KT * 4;
     HIP_DYNAMIC_SHARED(char, smem)
@@ -238,8 +240,8 @@ __global__ __launch_bounds__(256, DKP <= (SvbtParts<T>::NS == 1 ? 64 : 32) ? 2 :
     svbt_bf16x8 kf[NK][NS], vf[NK][NS];
 #pragma unroll
     for (int s = 0; s < NK; ++s) {
-        svbt_own_frag<T, NS>(k, a.k_sc, j, s, kb, a.dk, kept, kf[s]);
-        svbt_own_frag<T, NS>(v, a.v_sc, j, s, kb, a.dk, kept, vf[s]);
+        svbt_own_frag<T, NS>(k, a.k_sc, has ? j : 0, s, kb, a.dk, kept, kf[s]);
+        svbt_own_frag<T, NS>(v, a.v_sc, has ? j : 0, s, kb, a.dk, kept, vf[s]);
     }
     const bool all_kept = __ballot(!kept) == 0ull, none_kept = __ballot(kept) == 0ull;
     f32x16 dk[NDB], dv[NDB];
@@ -266,6 +268,9 @@ __global__ __launch_bounds__(256, DKP <= (SvbtParts<T>::NS == 1 ? 64 : 32) ? 2 :
         }
     };
     auto put = [&](int n) {
+        const int i0 = (first + n % tiles) * KT;
+        tq.settle(i0, a.Tq, ~0ull);
+        td.settle(i0, a.Tq, ~0ull);
         char* buf = smem + (DOUBLE ? (n & 1) * BUF : 0);
         tq.template store<true, true>(buf, buf + 2 * NS * Tile::ROWS_BYTES);
         td.template store<true, true>(buf + NS * Tile::ROWS_BYTES, buf + NS * (2 * Tile::ROWS_BYTES + Tile::COLS_BYTES));
@@ -365,27 +370,28 @@ static int bwd_lds(K* kern, int lds) {
     return lds > 65536 && hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024) != hipSuccess;
 }
 
-template <typename T, int DKP, int KT, bool DOUBLE>
-static int bwd_launch(const SvbBucketAttn* a, const SvbBattnBwd& g, hipStream_t st) {
-    typedef SvbtTile<T, DKP, KT, 256> Tile;
-    const int nbuf = DOUBLE ? 2 : 1, span = 2 * svb_bucket_reach(a->buckets) + 1;
-    {
-        const int qtiles = (a->Tq + 127) / 128;
-        int lds = nbuf * Tile::NS * (2 * Tile::ROWS_BYTES + Tile::COLS_BYTES) + ((span + 3) & ~3) * 4;
-        if (g.part) lds += a->buckets.n_buckets * 1024 + span;
-        auto* kern = svb_bucket_attn_dq_kernel<T, DKP, KT, DOUBLE>;
-        if (bwd_lds(kern, lds)) return SVB_ERR_LAUNCH;
-        hipLaunchKernelGGL(kern, dim3((unsigned)(a->B * a->H * qtiles)), dim3(256), lds, st, *a, g, qtiles);
-        SVB_CHECK_LAUNCH();
-    }
-    if (g.dk) {
-        const int ktiles = (a->Tk + 127) / 128;
-        const int lds = nbuf * (2 * Tile::NS * (Tile::ROWS_BYTES + Tile::COLS_BYTES) + 2 * KT * 4) + span * 4;
-        auto* kern = svb_bucket_attn_dkv_kernel<T, DKP, KT, DOUBLE>;
-        if (bwd_lds(kern, lds)) return SVB_ERR_LAUNCH;
-        hipLaunchKernelGGL(kern, dim3((unsigned)(a->B * a->Hkv * ktiles)), dim3(256), lds, st, *a, g, ktiles);
-        SVB_CHECK_LAUNCH();
-    }
+template <typename T, int DKP, int KT, bool DOUBLE, bool TINY = false>
+static int dq_launch(const SvbBucketAttn* a, const SvbBattnBwd& g, hipStream_t st) {
+    typedef SvbtTile<T, DKP, KT, 256, TINY> Tile;
+    const int span = 2 * svb_bucket_reach(a->buckets) + 1, qtiles = (a->Tq + 127) / 128;
+    int lds = (DOUBLE ? 2 : 1) * Tile::NS * (2 * Tile::ROWS_BYTES + Tile::COLS_BYTES) + ((span + 3) & ~3) * 4;
+    if (g.part) lds += a->buckets.n_buckets * 1024 + span;
+    auto* kern = svb_bucket_attn_dq_kernel<T, DKP, KT, DOUBLE, TINY>;
+    if (bwd_lds(kern, lds)) return SVB_ERR_LAUNCH;
+    hipLaunchKernelGGL(kern, dim3((unsigned)(a->B * a->H * qtiles)), dim3(256), lds, st, *a, g, qtiles);
+    SVB_CHECK_LAUNCH();
+    return SVB_OK;
+}
+
+template <typename T, int DKP, int KT, bool DOUBLE, bool TINY = false>
+static int dkv_launch(const SvbBucketAttn* a, const SvbBattnBwd& g, hipStream_t st) {
+    typedef SvbtTile<T, DKP, KT, 256, TINY> Tile;
+    const int span = 2 * svb_bucket_reach(a->buckets) + 1, ktiles = (a->Tk + 127) / 128;
+    const int lds = (DOUBLE ? 2 : 1) * (2 * Tile::NS * (Tile::ROWS_BYTES + Tile::COLS_BYTES) + 2 * KT * 4) + span * 4;
+    auto* kern = svb_bucket_attn_dkv_kernel<T, DKP, KT, DOUBLE, TINY>;
+    if (bwd_lds(kern, lds)) return SVB_ERR_LAUNCH;
+    hipLaunchKernelGGL(kern, dim3((unsigned)(a->B * a->Hkv * ktiles)), dim3(256), lds, st, *a, g, ktiles);
+    SVB_CHECK_LAUNCH();
     return SVB_OK;
 }
 
@@ -402,16 +408,25 @@ extern "C" int svb_bucket_attn_bwd(const SvbBucketAttn* a, const SvbBucketAttnGr
     if (!g || !g->dout || !g->ws || !a->lse || (a->dtype == SVB_DT_BF16 && !a->out_f32) || (!g->d_k != !g->d_v)) return SVB_ERR_ARG;
     hipStream_t st = (hipStream_t)stream;
     SvbBattnBwd w = {g->dout, g->d_q, g->d_k, g->d_v, g->ws, g->d_table ? g->ws + delta_floats(a) : nullptr};
+    // (double buffers where two workgroups of them fit a CU)
     if (a->dtype == SVB_DT_BF16) {
-        if (a->dk <= 32) rc = bwd_launch<unsigned short, 32, 64, true>(a, w, st);
-        else if (a->dk <= 64) rc = bwd_launch<unsigned short, 64, 64, true>(a, w, st);
-        else if (a->dk <= 96) rc = bwd_launch<unsigned short, 96, 64, false>(a, w, st);
-        else rc = bwd_launch<unsigned short, 128, 64, false>(a, w, st);
+        typedef unsigned short T;
+        rc = a->Tk < 4 ? dq_launch<T, 128, 64, false, true>(a, w, st) : a->dk <= 32 ? dq_launch<T, 32, 64, true>(a, w, st)
+             : a->dk <= 64 ? dq_launch<T, 64, 64, true>(a, w, st) : a->dk <= 96 ? dq_launch<T, 96, 64, false>(a, w, st)
+             : dq_launch<T, 128, 64, false>(a, w, st);
+        if (rc == SVB_OK && w.dk)
+            rc = a->Tq < 4 ? dkv_launch<T, 128, 64, false, true>(a, w, st) : a->dk <= 32 ? dkv_launch<T, 32, 64, true>(a, w, st)
+                 : a->dk <= 64 ? dkv_launch<T, 64, 64, true>(a, w, st) : a->dk <= 96 ? dkv_launch<T, 96, 64, false>(a, w, st)
+                 : dkv_launch<T, 128, 64, false>(a, w, st);
     } else {
-        if (a->dk <= 32) rc = bwd_launch<float, 32, 32, true>(a, w, st);
-        else if (a->dk <= 64) rc = bwd_launch<float, 64, 32, false>(a, w, st);
-        else if (a->dk <= 96) rc = bwd_launch<float, 96, 32, false>(a, w, st);
-        else rc = bwd_launch<float, 128, 32, false>(a, w, st);
+        typedef float T;
+        rc = a->Tk < 4 ? dq_launch<T, 128, 32, false, true>(a, w, st) : a->dk <= 32 ? dq_launch<T, 32, 32, true>(a, w, st)
+             : a->dk <= 64 ? dq_launch<T, 64, 32, false>(a, w, st) : a->dk <= 96 ? dq_launch<T, 96, 32, false>(a, w, st)
+             : dq_launch<T, 128, 32, false>(a, w, st);
+        if (rc == SVB_OK && w.dk)
+            rc = a->Tq < 4 ? dkv_launch<T, 128, 32, false, true>(a, w, st) : a->dk <= 32 ? dkv_launch<T, 32, 32, true>(a, w, st)
+                 : a->dk <= 64 ? dkv_launch<T, 64, 32, false>(a, w, st) : a->dk <= 96 ? dkv_launch<T, 96, 32, false>(a, w, st)
+                 : dkv_launch<T, 128, 32, false>(a, w, st);
     }
     if (rc != SVB_OK || !g->d_table) return rc;
     return svb_bucket_table_reduce(w.part, g->d_table, a->B * ((a->Tq + 127) / 128), a->buckets.n_buckets, a->H, a->table_dtype, st);

@@ -67,9 +67,9 @@ __device__ __forceinline__ void svbt_softmax(f32x16 (&s)[NSUB], SvbtState<NDB>& 
 
 // ---- query tiles: 4 waves x 32 queries, keys staged through LDS, the next tile's loads in flight during this one's products ------------
 // PP: parts of P
-template <typename T, int DKP, int KT, bool DOUBLE, int PP>
+template <typename T, int DKP, int KT, bool DOUBLE, int PP, bool TINY>
 __global__ __launch_bounds__(256, DKP <= 64 ? 2 : 1) void svb_bucket_attn_fwd_kernel(SvbBucketAttn a, int qtiles) {
-    typedef SvbtTile<T, DKP, KT, 256> Tile;
+    typedef SvbtTile<T, DKP, KT, 256, TINY> Tile;
     constexpr int NS = Tile::NS, NK = DKP / 16, NDB = DKP / 32, NSUB = KT / 32;
     constexpr int BUF = NS * (Tile::ROWS_BYTES + Tile::COLS_BYTES);
     HIP_DYNAMIC_SHARED(char, smem)
@@ -90,7 +90,7 @@ __global__ __launch_bounds__(256, DKP <= 64 ? 2 : 1) void svb_bucket_attn_fwd_ke
     const float* keep = a.keep ? a.keep + (size_t)b * a.Tk : nullptr;
     svbt_bf16x8 qf[NK][NS];
 #pragma unroll
-    for (int s = 0; s < NK; ++s) svbt_own_frag<T, NS>(q, a.q_sc, i, s, kb, a.dk, has, qf[s]);
+    for (int s = 0; s < NK; ++s) svbt_own_frag<T, NS>(q, a.q_sc, has ? i : 0, s, kb, a.dk, has, qf[s]);
 
     // keys that anyone here sees end at `end`; this wave's queries are at positions p0 .. p1
     int end = keep ? svbt_keep_end(keep, a.Tk, lane) : a.Tk;
@@ -106,17 +106,19 @@ __global__ __launch_bounds__(256, DKP <= 64 ? 2 : 1) void svb_bucket_attn_fwd_ke
     const float c = a.scale * SVBT_LOG2E;
 
     Tile tk, tv;
-    unsigned long long seen = ~0ull;
+    unsigned long long seen = ~0ull;                                    // of the tile in LDS: the keys that exist and are kept
+    float kept = 1.f;
     auto fetch = [&](int t) {                                            // loads of tile t
-        tk.load(k, a.k_sc, t * KT, end, a.dk);
-        tv.load(v, a.v_sc, t * KT, end, a.dk);
+        tk.load(k, a.k_sc, t * KT, a.Tk, a.dk);
+        tv.load(v, a.v_sc, t * KT, a.Tk, a.dk);
+        if (keep) kept = keep[min(t * KT + lane, a.Tk - 1)];
     };
     constexpr unsigned long long ALL = KT == 64 ? ~0ull : 0xffffffffull;
-    auto bits = [&](int t) {
-        return ALL & (keep ? svbt_keep_bits(keep[min(t * KT + lane, a.Tk - 1)], t * KT, end, lane) : __ballot(t * KT + lane < end));
-    };
+    auto bits = [&](int t) { return ALL & __ballot(t * KT + lane < end && kept != 0.f); };
     auto put = [&](int t) {                                              // registers -> LDS
-        if (keep) { tk.hide(seen); tv.hide(seen); }
+        const unsigned long long m = seen == ALL ? ~0ull : seen;
+        tk.settle(t * KT, a.Tk, m);
+        tv.settle(t * KT, a.Tk, m);
         char* buf = smem + (DOUBLE ? (t & 1) * BUF : 0);
         tk.template store<true, false>(buf, nullptr);
         tv.template store<false, true>(nullptr, buf + NS * Tile::ROWS_BYTES);
@@ -487,11 +489,11 @@ int svb_bucket_attn_check(const SvbBucketAttn* a) {
     return SVB_OK;
 }
 
-template <typename T, int DKP, int KT, bool DOUBLE, int PP>
+template <typename T, int DKP, int KT, bool DOUBLE, int PP, bool TINY = false>
 static int fwd_launch(const SvbBucketAttn* a, hipStream_t st) {
-    typedef SvbtTile<T, DKP, KT, 256> Tile;
+    typedef SvbtTile<T, DKP, KT, 256, TINY> Tile;
     const int lds = (DOUBLE ? 2 : 1) * Tile::NS * (Tile::ROWS_BYTES + Tile::COLS_BYTES) + (2 * svb_bucket_reach(a->buckets) + 1) * 4;
-    auto* kern = svb_bucket_attn_fwd_kernel<T, DKP, KT, DOUBLE, PP>;
+    auto* kern = svb_bucket_attn_fwd_kernel<T, DKP, KT, DOUBLE, PP, TINY>;
     if (lds > 65536 && hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024) != hipSuccess) return SVB_ERR_LAUNCH;
     const int qtiles = (a->Tq + 127) / 128;
     hipLaunchKernelGGL(kern, dim3((unsigned)(a->B * a->H * qtiles)), dim3(256), lds, st, *a, qtiles);
@@ -548,7 +550,8 @@ extern "C" int svb_bucket_attn_fwd(const SvbBucketAttn* a, float* ws, void* stre
     if (splits) SVB_FEW_GO(unsigned short);
 #undef SVB_FEW_GO
 #define SVB_FWD_GO(T, KT, PP)                                                                                     \
-    return a->dk <= 32 ? fwd_launch<T, 32, KT, true, PP>(a, st) : a->dk <= 64 ? fwd_launch<T, 64, KT, true, PP>(a, st) \
+    return a->Tk < 4 ? fwd_launch<T, 128, KT, true, PP, true>(a, st)                                                   \
+         : a->dk <= 32 ? fwd_launch<T, 32, KT, true, PP>(a, st) : a->dk <= 64 ? fwd_launch<T, 64, KT, true, PP>(a, st) \
          : a->dk <= 96 ? fwd_launch<T, 96, KT, true, PP>(a, st) : fwd_launch<T, 128, KT, true, PP>(a, st)
     if (a->dtype == SVB_DT_F32) SVB_FWD_GO(float, 32, 3);
     if (a->lse) SVB_FWD_GO(unsigned short, 64, 3);
