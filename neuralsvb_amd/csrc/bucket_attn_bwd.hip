@@ -41,7 +41,7 @@ __global__ __launch_bounds__(256, DKP <= 64 ? 2 : 1) void svb_bucket_attn_dq_ker
     HIP_DYNAMIC_SHARED(char, smem)
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l31 = lane & 31, kb = lane >> 5;
     const int item = svbt_item(blockIdx.x, gridDim.x);
-    const int bh = item / qtiles, b = bh / a.H, h = bh - b * a.H, hk = h / (a.H / a.Hkv);
+    const int bh = svb_uniform(item / qtiles), b = svb_uniform(bh / a.H), h = bh - b * a.H, hk = svb_uniform(h / (a.H / a.Hkv));
     const int qt = a.causal ? qtiles - 1 - (item - bh * qtiles) : item - bh * qtiles;
     const int i0 = qt * 128, i = i0 + wave * 32 + l31;
     const bool has = i < a.Tq;
@@ -229,7 +229,7 @@ __global__ __launch_bounds__(256, DKP <= (SvbtParts<T>::NS == 1 ? 64 : 32) ? 2 :
     HIP_DYNAMIC_SHARED(char, smem)
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l31 = lane & 31, kb = lane >> 5;
     const int item = svbt_item(blockIdx.x, gridDim.x);
-    const int bk = item / ktiles, b = bk / a.Hkv, hk = bk - b * a.Hkv, G = a.H / a.Hkv;
+    const int bk = svb_uniform(item / ktiles), b = svb_uniform(bk / a.Hkv), hk = bk - b * a.Hkv, G = svb_uniform(a.H / a.Hkv);
     const int jt = (item - bk * ktiles) * 128, jw = jt + wave * 32, j = jw + l31;
     const bool has = j < a.Tk, kept = has && (!a.keep || a.keep[(size_t)b * a.Tk + j] != 0.f);
     const int start = svbt_start(a, b), R = svb_bucket_reach(a.buckets);
@@ -257,7 +257,7 @@ __global__ __launch_bounds__(256, DKP <= (SvbtParts<T>::NS == 1 ? 64 : 32) ? 2 :
     const int steps = G * tiles;
     const bool any_kept = none_kept ? false : true;
     auto fetch = [&](int n) {
-        const int hh = hk * G + n / tiles, i0 = (first + n % tiles) * KT;
+        const int hh = hk * G + svb_uniform(n / tiles), i0 = (first + n % tiles) * KT;
         const size_t hd = (size_t)b * a.H + hh;
         tq.load((const T*)a.q + b * a.q_sb + (long long)hh * a.dk * a.q_sc, a.q_sc, i0, a.Tq, a.dk);
         td.load((const T*)g.dout + hd * a.dk * a.Tq, a.Tq, i0, a.Tq, a.dk);

@@ -75,7 +75,7 @@ __global__ __launch_bounds__(256, DKP <= 64 ? 2 : 1) void svb_bucket_attn_fwd_ke
     HIP_DYNAMIC_SHARED(char, smem)
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l31 = lane & 31, kb = lane >> 5;
     const int item = svbt_item(blockIdx.x, gridDim.x);
-    const int bh = item / qtiles, b = bh / a.H, h = bh - b * a.H, hk = h / (a.H / a.Hkv);
+    const int bh = svb_uniform(item / qtiles), b = svb_uniform(bh / a.H), h = bh - b * a.H, hk = svb_uniform(h / (a.H / a.Hkv));
     const int qt = a.causal ? qtiles - 1 - (item - bh * qtiles) : item - bh * qtiles;      // (causal: the longest rows first)
     const int i0 = qt * 128, i = i0 + wave * 32 + l31;
     const bool has = i < a.Tq;
@@ -317,7 +317,7 @@ __global__ __launch_bounds__(256, DKP * SvbtParts<T>::NS > 192 || DKP == 128 ? 1
     HIP_DYNAMIC_SHARED(char, smem)
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l31 = lane & 31, kb = lane >> 5;
     const int split = blockIdx.x, hk = blockIdx.y, b = blockIdx.z;
-    const int G = a.H / a.Hkv, rows = G * a.Tq, nb = a.buckets.n_buckets, R = svb_bucket_reach(a.buckets);
+    const int G = svb_uniform(a.H / a.Hkv), rows = G * a.Tq, nb = a.buckets.n_buckets, R = svb_bucket_reach(a.buckets);
     float* s_tab = (float*)smem;                                        // [G][nb]
     unsigned char* s_idx = (unsigned char*)(s_tab + G * nb);             // [2 R + 1]
     for (int e = threadIdx.x; e < G * nb; e += 256)

@@ -119,7 +119,7 @@ __global__ __launch_bounds__(NT) void svb_ln_nct_fwd_kernel(SvbLnArgs a) {
     const int col = threadIdx.x & (LPR - 1), row = threadIdx.x / LPR;
     for (int c = threadIdx.x; c < a.C; c += NT)                         // (read behind the barriers of the reductions)
         affine[c] = make_float2(a.gamma ? svb_ld_table(a.gamma, c, a.affine_bf16) : 1.f, a.beta ? svb_ld_table(a.beta, c, a.affine_bf16) : 0.f);
-    const int b = blockIdx.x / a.tiles, t0 = min((blockIdx.x - b * a.tiles) * (LPR * VEC) + col * VEC, a.T - VEC);
+    const int b = svb_uniform((int)blockIdx.x / a.tiles), t0 = min(((int)blockIdx.x - b * a.tiles) * (LPR * VEC) + col * VEC, a.T - VEC);
     // uniform bases and 32-bit byte offsets inside one batch entry: the scalar-base form of the loads, one register per address
     const char* x = (const char*)((const T*)a.x + (size_t)b * a.C * a.T);
     char* y = (char*)((T*)a.y + (size_t)b * a.C * a.T);
@@ -191,7 +191,7 @@ __global__ __launch_bounds__(NT) void svb_ln_nct_bwd_kernel(SvbLnArgs a) {
     __syncthreads();
     const int all = a.B * a.tiles;
     for (int tile = blockIdx.x; tile < all; tile += gridDim.x) {
-        const int b = tile / a.tiles, want = (tile - b * a.tiles) * (LPR * VEC) + col * VEC;
+        const int b = svb_uniform(tile / a.tiles), want = (tile - b * a.tiles) * (LPR * VEC) + col * VEC;
         const int t0 = min(want, a.T - VEC), skip = want - t0;          // (skip >= VEC: nothing of its own)
         const size_t base = (size_t)b * a.C * a.T;
         const char *x = (const char*)((const T*)a.x + base), *dy = (const char*)((const T*)a.dy + base);
@@ -225,7 +225,8 @@ __global__ __launch_bounds__(NT) void svb_ln_nct_bwd_kernel(SvbLnArgs a) {
                 dg[p] = fmaf(own, e >= skip ? xh : 0.f, dg[p]);
                 db[p] += own;
             }
-            __builtin_amdgcn_sched_barrier(0);                          // (one pass's floats at a time)
+            svb_opaque(dg[p]);                                          // (summed here: moved down behind the reductions the sums would keep
+            svb_opaque(db[p]);                                          //  every pass's floats alive, 140 registers)
         }
         if (a.dx) {                                                     // (workgroup-uniform)
             svbl_rows_sum<VEC, LPR, NT>(s1, red, col);
@@ -244,7 +245,6 @@ __global__ __launch_bounds__(NT) void svb_ln_nct_bwd_kernel(SvbLnArgs a) {
                     }
                     svbl_store<VEC>((T*)(dx + (off + p * step)), o);
                 }
-                __builtin_amdgcn_sched_barrier(0);
             }
         }
     }
@@ -348,24 +348,25 @@ __global__ __launch_bounds__(256) void svb_ln_nct_bwd_wide_kernel(SvbLnArgs a) {
     }
 }
 
-// dgamma | dbeta = sums of the rows of part [rows][2 C]: 32 columns x 8 row groups per workgroup, four sums in flight per thread
-__global__ __launch_bounds__(256) void svb_ln_nct_affine_kernel(const float* part, int rows, int C, void* dgamma, void* dbeta, int is_bf16) {
-    __shared__ float red[8][32];
+// dgamma | dbeta = sums of the rows of part [rows][2 C]: 32 columns x 32 row groups per workgroup, four rows of each in flight
+__global__ __launch_bounds__(1024) void svb_ln_nct_affine_kernel(const float* part, int rows, int C, void* dgamma, void* dbeta, int is_bf16) {
+    __shared__ float red[32][33];
     const int cl = threadIdx.x & 31, rg = threadIdx.x >> 5, c = blockIdx.x * 32 + cl;
     float s[4] = {0.f, 0.f, 0.f, 0.f};
     if (c < 2 * C)
-        for (int r = rg; r < rows; r += 32)
+        for (int r = rg; r < rows; r += 128)
 #pragma unroll
             for (int u = 0; u < 4; ++u)
-                if (r + 8 * u < rows) s[u] += part[(size_t)(r + 8 * u) * 2 * C + c];
+                if (r + 32 * u < rows) s[u] += part[(size_t)(r + 32 * u) * 2 * C + c];
     red[rg][cl] = (s[0] + s[1]) + (s[2] + s[3]);
     __syncthreads();
-    if (rg == 0 && c < 2 * C) {
-        float t = 0.f;
+    float t = red[cl][rg];                                              // column rg's 32 groups, one per lane
 #pragma unroll
-        for (int q = 0; q < 8; ++q) t += red[q][cl];
-        if (c < C) { if (dgamma) svbl_st_affine(dgamma, c, t, is_bf16); }
-        else if (dbeta) svbl_st_affine(dbeta, c - C, t, is_bf16);
+    for (int o = 1; o < 32; o <<= 1) t += __shfl_xor(t, o, 64);
+    const int c2 = blockIdx.x * 32 + rg;
+    if (cl == 0 && c2 < 2 * C) {
+        if (c2 < C) { if (dgamma) svbl_st_affine(dgamma, c2, t, is_bf16); }
+        else if (dbeta) svbl_st_affine(dbeta, c2 - C, t, is_bf16);
     }
 }
 
@@ -445,7 +446,7 @@ extern "C" int svb_ln_nct_bwd(const void* x, const void* gamma, const void* dy, 
     else svbl_launch<float, 4>(false, a, p, (unsigned)grid, (hipStream_t)stream);
     SVB_CHECK_LAUNCH();
     if ((dgamma || dbeta) && (grid > 1 || p.rows == 0)) {
-        hipLaunchKernelGGL(svb_ln_nct_affine_kernel, dim3((unsigned)((2 * C + 31) / 32)), dim3(256), 0, (hipStream_t)stream, (const float*)ws,
+        hipLaunchKernelGGL(svb_ln_nct_affine_kernel, dim3((unsigned)((2 * C + 31) / 32)), dim3(1024), 0, (hipStream_t)stream, (const float*)ws,
                            grid, C, dgamma, dbeta, (int)a.affine_bf16);
         SVB_CHECK_LAUNCH();
     }

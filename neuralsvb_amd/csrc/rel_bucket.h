@@ -9,6 +9,10 @@
 #include "svb_common.h"
 #include "../../include/svb_hip.h"
 
+// A value that is the same in every lane but was computed by vector instructions (an integer division is), as a scalar: pointers built
+// from it are scalar then, and a load takes a scalar base and a 32-bit offset instead of a register pair per address.
+__device__ __forceinline__ int svb_uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
+
 // least distance from which a side's bucket stays the same
 static __host__ __device__ __forceinline__ int svb_bucket_reach(const SvbRelBuckets& b) {
     return b.n_edge > 0 ? b.edge[b.n_edge - 1] : b.near;

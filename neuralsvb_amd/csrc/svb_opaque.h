@@ -8,5 +8,6 @@
 #include <hip/hip_runtime.h>
 
 __device__ __forceinline__ void svb_opaque(unsigned& v) { asm volatile("" : "+v"(v)); }
+__device__ __forceinline__ void svb_opaque(float& v) { asm volatile("" : "+v"(v)); }
 __device__ __forceinline__ void svb_opaque(long long& v) { asm volatile("" : "+v"(v)); }      // (an offset: an opaque pointer would be a flat one)
 __device__ __forceinline__ void svb_opaque_uniform(long long& v) { asm volatile("" : "+s"(v)); }      // (the same in every lane)
