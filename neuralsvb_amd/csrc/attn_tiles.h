@@ -305,10 +305,3 @@ __device__ __forceinline__ int svbt_keep_end(const float* keep, int n, int lane)
     }
     return 0;
 }
-// work item of a workgroup: consecutive items on one XCD (workgroups go round the 8 XCDs in turn), so that the workgroups of one
-// head share their keys and values in one L2
-// (divisions of uniform values leave them in vector registers: svb_uniform brings them back)
-__device__ __forceinline__ int svbt_item(int id, int total) {
-    const int x = id & 7, q = total >> 3, r = total & 7;
-    return x * q + min(x, r) + (id >> 3);
-}

@@ -40,7 +40,7 @@ __global__ __launch_bounds__(256, DKP <= 64 ? 2 : 1) void svb_bucket_attn_dq_ker
     constexpr int BUF = NS * (2 * Tile::ROWS_BYTES + Tile::COLS_BYTES);
     HIP_DYNAMIC_SHARED(char, smem)
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l31 = lane & 31, kb = lane >> 5;
-    const int item = svbt_item(blockIdx.x, gridDim.x);
+    const int item = svb_xcd_item(blockIdx.x, gridDim.x);
     const int bh = svb_uniform(item / qtiles), b = svb_uniform(bh / a.H), h = bh - b * a.H, hk = svb_uniform(h / (a.H / a.Hkv));
     const int qt = a.causal ? qtiles - 1 - (item - bh * qtiles) : item - bh * qtiles;
     const int i0 = qt * 128, i = i0 + wave * 32 + l31;
@@ -228,7 +228,7 @@ __global__ __launch_bounds__(256, DKP <= (SvbtParts<T>::NS == 1 ? 64 : 32) ? 2 :
     constexpr int TILE = NS * 2 * (Tile::ROWS_BYTES + Tile::COLS_BYTES), BUF = TILE + 2 * KT * 4;
     HIP_DYNAMIC_SHARED(char, smem)
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l31 = lane & 31, kb = lane >> 5;
-    const int item = svbt_item(blockIdx.x, gridDim.x);
+    const int item = svb_xcd_item(blockIdx.x, gridDim.x);
     const int bk = svb_uniform(item / ktiles), b = svb_uniform(bk / a.Hkv), hk = bk - b * a.Hkv, G = svb_uniform(a.H / a.Hkv);
     const int jt = (item - bk * ktiles) * 128, jw = jt + wave * 32, j = jw + l31;
     const bool has = j < a.Tk, kept = has && (!a.keep || a.keep[(size_t)b * a.Tk + j] != 0.f);

@@ -74,7 +74,7 @@ __global__ __launch_bounds__(256, DKP <= 64 ? 2 : 1) void svb_bucket_attn_fwd_ke
     constexpr int BUF = NS * (Tile::ROWS_BYTES + Tile::COLS_BYTES);
     HIP_DYNAMIC_SHARED(char, smem)
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l31 = lane & 31, kb = lane >> 5;
-    const int item = svbt_item(blockIdx.x, gridDim.x);
+    const int item = svb_xcd_item(blockIdx.x, gridDim.x);
     const int bh = svb_uniform(item / qtiles), b = svb_uniform(bh / a.H), h = bh - b * a.H, hk = svb_uniform(h / (a.H / a.Hkv));
     const int qt = a.causal ? qtiles - 1 - (item - bh * qtiles) : item - bh * qtiles;      // (causal: the longest rows first)
     const int i0 = qt * 128, i = i0 + wave * 32 + l31;

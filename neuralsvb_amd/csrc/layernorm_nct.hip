@@ -16,7 +16,7 @@
 #include "rel_bucket.h"
 #include <svb_opaque.h>
 
-#define SVB_LN_MAX_WG 1024
+#define SVB_LN_MAX_WG 512
 
 typedef float svbl_f4 __attribute__((ext_vector_type(4), aligned(4)));
 typedef unsigned svbl_u4 __attribute__((ext_vector_type(4), aligned(2)));
@@ -119,7 +119,8 @@ __global__ __launch_bounds__(NT) void svb_ln_nct_fwd_kernel(SvbLnArgs a) {
     const int col = threadIdx.x & (LPR - 1), row = threadIdx.x / LPR;
     for (int c = threadIdx.x; c < a.C; c += NT)                         // (read behind the barriers of the reductions)
         affine[c] = make_float2(a.gamma ? svb_ld_table(a.gamma, c, a.affine_bf16) : 1.f, a.beta ? svb_ld_table(a.beta, c, a.affine_bf16) : 0.f);
-    const int b = svb_uniform((int)blockIdx.x / a.tiles), t0 = min(((int)blockIdx.x - b * a.tiles) * (LPR * VEC) + col * VEC, a.T - VEC);
+    const int item = svb_xcd_item(blockIdx.x, gridDim.x);
+    const int b = svb_uniform(item / a.tiles), t0 = min((item - b * a.tiles) * (LPR * VEC) + col * VEC, a.T - VEC);
     // uniform bases and 32-bit byte offsets inside one batch entry: the scalar-base form of the loads, one register per address
     const char* x = (const char*)((const T*)a.x + (size_t)b * a.C * a.T);
     char* y = (char*)((T*)a.y + (size_t)b * a.C * a.T);
@@ -190,7 +191,7 @@ __global__ __launch_bounds__(NT) void svb_ln_nct_bwd_kernel(SvbLnArgs a) {
     for (int p = 0; p < P; ++p) dg[p] = db[p] = 0.f;
     __syncthreads();
     const int all = a.B * a.tiles;
-    for (int tile = blockIdx.x; tile < all; tile += gridDim.x) {
+    for (int tile = svb_xcd_item(blockIdx.x, gridDim.x); tile < all; tile += gridDim.x) {
         const int b = svb_uniform(tile / a.tiles), want = (tile - b * a.tiles) * (LPR * VEC) + col * VEC;
         const int t0 = min(want, a.T - VEC), skip = want - t0;          // (skip >= VEC: nothing of its own)
         const size_t base = (size_t)b * a.C * a.T;

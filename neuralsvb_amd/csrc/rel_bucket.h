@@ -13,6 +13,13 @@
 // from it are scalar then, and a load takes a scalar base and a 32-bit offset instead of a register pair per address.
 __device__ __forceinline__ int svb_uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
 
+// Work item of workgroup `id` of `total`: workgroups go round the 8 XCDs in turn, each with an L2 of its own; consecutive items on one
+// XCD share what they read there (the keys of one head, the two halves of a line).
+__device__ __forceinline__ int svb_xcd_item(int id, int total) {
+    const int x = id & 7, q = total >> 3, r = total & 7;
+    return x * q + min(x, r) + (id >> 3);
+}
+
 // least distance from which a side's bucket stays the same
 static __host__ __device__ __forceinline__ int svb_bucket_reach(const SvbRelBuckets& b) {
     return b.n_edge > 0 ? b.edge[b.n_edge - 1] : b.near;
