@@ -877,15 +877,15 @@ class _LayerNormNCTFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, gamma, beta, eps):
         x, gamma, beta = _c(x), _c(gamma), _c(beta)
-        y, mean, rstd = K.ln_nct_fwd(x, gamma, beta, eps, save_stats=True)
+        y, stats = K.ln_nct_fwd(x, gamma, beta, eps, save_stats=True)
         ctx.affine_dtype = gamma.dtype if gamma is not None else beta.dtype if beta is not None else torch.float32
-        ctx.save_for_backward(x, gamma, mean, rstd)
+        ctx.save_for_backward(x, gamma, stats)
         return y
 
     @staticmethod
     def backward(ctx, dy):
-        x, gamma, mean, rstd = ctx.saved_tensors
-        return K.ln_nct_bwd(x, gamma, _c(dy), mean, rstd, *ctx.needs_input_grad[:3], affine_dtype=ctx.affine_dtype) + (None,)
+        x, gamma, stats = ctx.saved_tensors
+        return K.ln_nct_bwd(x, gamma, _c(dy), stats, *ctx.needs_input_grad[:3], ctx.affine_dtype) + (None,)
 
 
 def layer_norm_nct(x, gamma, beta, eps=1e-5):
@@ -977,7 +977,7 @@ class _BucketAttnFn(torch.autograd.Function):
 
 
 def _time_rows(t):
-    return t if t.dim() != 3 or t.shape[2] <= 1 or t.stride(2) == 1 else t.contiguous()
+    return t if t.dim() != 3 or t.stride(2) == 1 or t.shape[2] <= 1 else t.contiguous()
 
 
 def bucket_attention(q, k, v, table, buckets, n_head, keep=None, causal=False, scale=None, q_start=None):
@@ -1001,8 +1001,8 @@ def bucket_attention(q, k, v, table, buckets, n_head, keep=None, causal=False, s
         q_start = k.shape[-1] - q.shape[-1]
     elif isinstance(q_start, torch.Tensor):
         q_start = q_start.contiguous()
-    cfg = (buckets.c, n_head, bool(causal), float(scale))
-    if torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, v, table)):
+    cfg = (buckets.c, n_head, int(bool(causal)), float(scale))
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or table.requires_grad):
         return _BucketAttnFn.apply(q, k, v, table, keep, q_start, cfg)
     return K.bucket_attn_fwd(q, k, v, table, *cfg[:2], keep, q_start, *cfg[2:])
 

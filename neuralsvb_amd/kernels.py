@@ -1035,6 +1035,7 @@ def layernorm_nct_fwd(x, gamma, beta, eps=1e-5):
 
 
 _DT = {torch.float32: L.SVB_DT_F32, torch.bfloat16: L.SVB_DT_BF16}
+_byref = C.byref
 
 
 def _dt(t, what):
@@ -1044,52 +1045,61 @@ def _dt(t, what):
     return code
 
 
-def _issue(t, what, fn, *args):
-    """One C-ABI call that launches on t's device, whichever device is current."""
-    idx = t.get_device()
+def _issue(idx, what, fn, *args):
+    """One C-ABI call that launches on device idx (-1: the emulator), whichever device is current."""
     if idx < 0 or idx == torch._C._cuda_getDevice():
-        L.check(fn(*args), what)
+        rc = fn(*args)
     else:
         with torch.cuda.device(idx):
-            L.check(fn(*args), what)
+            rc = fn(*args)
+    if rc:
+        L.check(rc, what)
 
 
 def ln_nct_fwd(x, gamma, beta, eps=1e-5, save_stats=False):
-    """LayerNorm over dim 1 of [B, C, T], fp32 or bf16 -> y, and with save_stats mean, rstd [B, T].  gamma, beta [C] or None, both of
-    x's dtype or both float32."""
-    for t in (gamma, beta):
-        if t is not None and (tuple(t.shape) != (x.shape[1],) or t.dtype not in (x.dtype, torch.float32)):
-            raise ValueError(f"gamma, beta: [{x.shape[1]}] of {x.dtype} or float32, got {tuple(t.shape)} of {t.dtype}")
-    if gamma is not None and beta is not None and gamma.dtype != beta.dtype:
-        raise TypeError("gamma and beta must have one dtype")
-    dt, adt = _dt(x, "ln_nct_fwd"), _dt(gamma if gamma is not None else beta if beta is not None else x, "ln_nct_fwd")
-    lib, st = _prep(x, gamma, beta)
+    """LayerNorm over dim 1 of [B, C, T], fp32 or bf16 -> y, and with save_stats the statistics [2, B, T] (mean, 1 / deviation).
+    gamma, beta [C] or None, both of x's dtype or both float32."""
     B, c, t = x.shape
+    adt = None
+    for p in (gamma, beta):
+        if p is not None:
+            if p.dim() != 1 or p.shape[0] != c or (p.dtype is not torch.float32 and p.dtype is not x.dtype):
+                raise ValueError(f"gamma, beta: [{c}] of {x.dtype} or float32, got {tuple(p.shape)} of {p.dtype}")
+            if adt is not None and p.dtype is not adt:
+                raise TypeError("gamma and beta must have one dtype")
+            adt = p.dtype
+    dt = _dt(x, "ln_nct_fwd")
+    lib, st = _prep(x, gamma, beta)
     y = torch.empty_like(x)
-    mean = rstd = None
+    mean = rstd = stats = None
     if save_stats:
-        mean, rstd = (torch.empty((B, t), device=x.device, dtype=torch.float32) for _ in range(2))
+        stats = x.new_empty((2, B, t), dtype=torch.float32)
+        mean = stats.data_ptr()
+        rstd = mean + 4 * B * t
     if x.numel():
-        _issue(x, "svb_ln_nct_fwd", lib.svb_ln_nct_fwd, _ptr(x), _ptr(gamma), _ptr(beta), _ptr(y), _ptr(mean), _ptr(rstd), B, c, t,
-               float(eps), dt, adt, st)
-    return (y, mean, rstd) if save_stats else y
+        _issue(x.get_device(), "svb_ln_nct_fwd", lib.svb_ln_nct_fwd, x.data_ptr(), _ptr(gamma), _ptr(beta), y.data_ptr(), mean, rstd, B, c, t,
+               eps, dt, 0 if adt is None else _DT[adt], st)
+    return (y, stats) if save_stats else y
 
 
-def ln_nct_bwd(x, gamma, dy, mean, rstd, want_dx=True, want_dgamma=True, want_dbeta=True, affine_dtype=torch.float32):
-    """-> dx, dgamma, dbeta (None where not wanted); affine gradients in affine_dtype."""
-    if dy.shape != x.shape or dy.dtype != x.dtype:
+def ln_nct_bwd(x, gamma, dy, stats, want_dx=True, want_dgamma=True, want_dbeta=True, affine_dtype=torch.float32):
+    """-> dx, dgamma, dbeta (None where not wanted); affine gradients in affine_dtype.  stats: of ln_nct_fwd."""
+    if dy.shape != x.shape or dy.dtype is not x.dtype:
         raise ValueError("dy must have the shape and dtype of x")
-    lib, st = _prep(x, gamma, dy, mean, rstd)
+    lib, st = _prep(x, gamma, dy, stats)
     B, c, t = x.shape
     dx = torch.empty_like(x) if want_dx else None
-    dg, db = (torch.empty((c,), device=x.device, dtype=affine_dtype) if w else None for w in (want_dgamma, want_dbeta))
+    dg = x.new_empty((c,), dtype=affine_dtype) if want_dgamma else None
+    db = x.new_empty((c,), dtype=affine_dtype) if want_dbeta else None
     if not x.numel():
         return dx, dg.zero_() if want_dgamma else None, db.zero_() if want_dbeta else None
+    dt = _DT[x.dtype]
     ws = None
     if want_dgamma or want_dbeta:
-        ws = torch.empty((lib.svb_ln_nct_bwd_workspace_floats(B, c, t, _DT[x.dtype]),), device=x.device, dtype=torch.float32)
-    _issue(x, "svb_ln_nct_bwd", lib.svb_ln_nct_bwd, _ptr(x), _ptr(gamma), _ptr(dy), _ptr(mean), _ptr(rstd), _ptr(dx), _ptr(dg), _ptr(db),
-           _ptr(ws), B, c, t, _DT[x.dtype], _DT[affine_dtype], st)
+        ws = x.new_empty((lib.svb_ln_nct_bwd_workspace_floats(B, c, t, dt),), dtype=torch.float32)
+    mean = stats.data_ptr()
+    _issue(x.get_device(), "svb_ln_nct_bwd", lib.svb_ln_nct_bwd, x.data_ptr(), _ptr(gamma), dy.data_ptr(), mean, mean + 4 * B * t, _ptr(dx), _ptr(dg),
+           _ptr(db), _ptr(ws), B, c, t, dt, _DT[affine_dtype], st)
     return dx, dg, db
 
 
@@ -1103,10 +1113,11 @@ def bucket_bias_fwd(table, buckets, tq, tk, q_start):
     _table_shape(table, buckets, None, "bucket_bias")
     dt = _dt(table, "bucket_bias")
     lib, st = _prep(table)
-    out = torch.empty((table.shape[1], tq, tk), device=table.device, dtype=table.dtype)
+    h = table.shape[1]
+    out = table.new_empty((h, tq, tk))
     if out.numel():
-        _issue(table, "svb_bucket_bias_fwd", lib.svb_bucket_bias_fwd, _ptr(table), _ptr(out), C.byref(buckets), table.shape[1], tq, tk, q_start,
-               dt, st)
+        _issue(table.get_device(), "svb_bucket_bias_fwd", lib.svb_bucket_bias_fwd, table.data_ptr(), out.data_ptr(), _byref(buckets), h, tq, tk,
+               q_start, dt, st)
     return out
 
 
@@ -1115,48 +1126,56 @@ def bucket_bias_bwd(dbias, buckets, q_start):
     dt = _dt(dbias, "bucket_bias")
     lib, st = _prep(dbias)
     h, tq, tk = dbias.shape
-    dtable = torch.empty((buckets.n_buckets, h), device=dbias.device, dtype=dbias.dtype)
+    dtable = dbias.new_empty((buckets.n_buckets, h))
     if not dbias.numel():
         return dtable.zero_()
-    ws = torch.empty((lib.svb_bucket_bias_bwd_workspace_floats(h, tq, tk, buckets.n_buckets),), device=dbias.device, dtype=torch.float32)
-    _issue(dbias, "svb_bucket_bias_bwd", lib.svb_bucket_bias_bwd, _ptr(dbias), _ptr(dtable), C.byref(buckets), _ptr(ws), h, tq, tk, q_start, dt, st)
+    ws = dbias.new_empty((lib.svb_bucket_bias_bwd_workspace_floats(h, tq, tk, buckets.n_buckets),), dtype=torch.float32)
+    _issue(dbias.get_device(), "svb_bucket_bias_bwd", lib.svb_bucket_bias_bwd, dbias.data_ptr(), dtable.data_ptr(), _byref(buckets), ws.data_ptr(), h,
+           tq, tk, q_start, dt, st)
     return dtable
 
 
 def _bucket_attn_desc(q, k, v, table, buckets, n_head, keep, q_start, causal, scale):
-    """The checked call description (lib, stream, SvbBucketAttn without outputs)."""
+    """(lib, stream, SvbBucketAttn without outputs) of a checked call."""
     _table_shape(table, buckets, n_head, "bucket_attention")
     if q.dim() != 3 or k.dim() != 3 or k.shape != v.shape or q.shape[0] != k.shape[0] or q.shape[1] % n_head:
         raise ValueError(f"bucket_attention: q [B, H dk, Tq], k, v [B, Hkv dk, Tk] with {n_head} heads, got {tuple(q.shape)}, {tuple(k.shape)}, "
                          f"{tuple(v.shape)}")
     B, D, tq = q.shape
-    dk, tk = D // n_head, k.shape[2]
-    if not 1 <= dk <= 128 or k.shape[1] % dk or n_head % max(1, k.shape[1] // dk):
-        raise ValueError(f"bucket_attention: {k.shape[1]} key channels are no divisor of {n_head} heads of {dk} channels (at most 128)")
-    if not (q.dtype == k.dtype == v.dtype):
+    _, Dk, tk = k.shape
+    dk = D // n_head
+    if not 1 <= dk <= 128 or not Dk or Dk % dk or n_head % (Dk // dk):
+        raise ValueError(f"bucket_attention: {Dk} key channels are no divisor of {n_head} heads of {dk} channels (at most 128)")
+    if q.dtype is not k.dtype or q.dtype is not v.dtype:
         raise TypeError("bucket_attention: q, k and v must have one dtype")
-    for t in (q, k, v):
-        if (t.shape[2] > 1 and t.stride(2) != 1) or t.device != q.device:
-            raise ValueError("bucket_attention: q, k, v need unit time stride and one device")
     d = L.SvbBucketAttn()
     d.dtype, d.table_dtype = _dt(q, "bucket_attention"), _dt(table, "bucket_attention: table")
+    d.q_sb, d.q_sc, q_st = q.stride()
+    d.k_sb, d.k_sc, k_st = k.stride()
+    d.v_sb, d.v_sc, v_st = v.stride()
+    if (tq > 1 and q_st != 1) or (tk > 1 and (k_st != 1 or v_st != 1)):
+        raise ValueError("bucket_attention: q, k, v need unit time stride")
     if keep is not None:
         _f32(keep)
         if tuple(keep.shape) != (B, tk):
             raise ValueError(f"bucket_attention: keep must be [{B}, {tk}], got {tuple(keep.shape)}")
+        d.keep = keep.data_ptr()
+    starts = None
     if isinstance(q_start, torch.Tensor):
-        if q_start.dtype != torch.int32 or tuple(q_start.shape) != (B,):
+        starts = q_start
+        if starts.dtype != torch.int32 or tuple(starts.shape) != (B,):
             raise ValueError(f"bucket_attention: q_start must be an int or int32 [{B}]")
-        d.q_start_b, starts = _ptr(q_start), q_start
+        d.q_start_b = starts.data_ptr()
     else:
-        d.q_start, starts = int(q_start), None
+        # (beyond any key the start makes no difference any more; its distance fits the descriptor's 32 bits)
+        d.q_start = max(-(1 << 28), min(1 << 28, int(q_start)))
     lib, st = _prep(table, keep, starts)
-    if table.get_device() != q.get_device():
-        raise ValueError(f"tensors on different devices: {table.device} vs {q.device}")
-    d.q, d.k, d.v, d.table, d.keep = _ptr(q), _ptr(k), _ptr(v), _ptr(table), _ptr(keep)
-    d.q_sb, d.q_sc, d.k_sb, d.k_sc, d.v_sb, d.v_sc = q.stride(0), q.stride(1), k.stride(0), k.stride(1), v.stride(0), v.stride(1)
-    d.B, d.H, d.Hkv, d.dk, d.Tq, d.Tk = B, n_head, k.shape[1] // dk, dk, tq, tk
-    d.causal, d.scale, d.buckets = int(bool(causal)), float(scale), buckets
+    idx = q.get_device()
+    if table.get_device() != idx or k.get_device() != idx or v.get_device() != idx:
+        raise ValueError(f"tensors on different devices: {q.device}, {k.device}, {v.device}, {table.device}")
+    d.q, d.k, d.v, d.table = q.data_ptr(), k.data_ptr(), v.data_ptr(), table.data_ptr()
+    d.B, d.H, d.Hkv, d.dk, d.Tq, d.Tk = B, n_head, Dk // dk, dk, tq, tk
+    d.causal, d.scale, d.buckets = causal, scale, buckets
     return lib, st, d
 
 
@@ -1164,42 +1183,44 @@ def bucket_attn_fwd(q, k, v, table, buckets, n_head, keep, q_start, causal, scal
     """-> out [B, H dk, Tq]; with train also lse [B, H, Tq] and, for bf16 tensors, out in float32 (None for float32)."""
     lib, st, d = _bucket_attn_desc(q, k, v, table, buckets, n_head, keep, q_start, causal, scale)
     B, D, tq = q.shape
-    out = torch.empty((B, D, tq), device=q.device, dtype=q.dtype)
+    out = q.new_empty((B, D, tq))
     lse = o32 = None
     if train:
-        lse = torch.empty((B, n_head, tq), device=q.device, dtype=torch.float32)
-        if q.dtype != torch.float32:
-            o32 = torch.empty((B, D, tq), device=q.device, dtype=torch.float32)
+        lse = q.new_empty((B, n_head, tq), dtype=torch.float32)
+        d.lse = lse.data_ptr()
+        if q.dtype is not torch.float32:
+            o32 = q.new_empty((B, D, tq), dtype=torch.float32)
+            d.out_f32 = o32.data_ptr()
     if out.numel() and not k.shape[2]:
         out.zero_()                                    # (no key at all)
     elif out.numel():
-        d.out, d.lse, d.out_f32 = _ptr(out), _ptr(lse), _ptr(o32)
-        n = lib.svb_bucket_attn_fwd_workspace_floats(C.byref(d))
-        ws = torch.empty((n,), device=q.device, dtype=torch.float32) if n else None
-        _issue(q, "svb_bucket_attn_fwd", lib.svb_bucket_attn_fwd, C.byref(d), _ptr(ws), st)
+        d.out = out.data_ptr()
+        n = 0 if train else lib.svb_bucket_attn_fwd_workspace_floats(_byref(d))
+        ws = q.new_empty((n,), dtype=torch.float32) if n else None
+        _issue(q.get_device(), "svb_bucket_attn_fwd", lib.svb_bucket_attn_fwd, _byref(d), _ptr(ws), st)
     return (out, lse, o32) if train else out
 
 
 def bucket_attn_bwd(dout, q, k, v, table, buckets, n_head, keep, q_start, causal, scale, out, lse, o32, want_q=True, want_kv=True,
                     want_table=True):
-    """-> dq, (dk, dv), dtable, contiguous, None where not wanted.  out is read for float32 tensors, o32 for bfloat16 ones (the other may
+    """-> dq, dk, dv, dtable, contiguous, None where not wanted.  out is read for float32 tensors, o32 for bfloat16 ones (the other may
     be None)."""
     lib, st, d = _bucket_attn_desc(q, k, v, table, buckets, n_head, keep, q_start, causal, scale)
+    if dout.shape != q.shape or dout.dtype is not q.dtype:
+        raise ValueError("dout must have the shape and dtype of the output")
     _prep(dout, out, lse, o32)
-    dq = torch.empty(q.shape, device=q.device, dtype=q.dtype) if want_q else None
-    dk, dv = (torch.empty(k.shape, device=q.device, dtype=q.dtype) if want_kv else None for _ in range(2))
-    dt = torch.empty(table.shape, device=q.device, dtype=table.dtype) if want_table else None
+    dq = q.new_empty(q.shape) if want_q else None
+    dk, dv = (k.new_empty(k.shape), k.new_empty(k.shape)) if want_kv else (None, None)
+    dt = table.new_empty(table.shape) if want_table else None
     if not q.numel() or not k.numel():
         for t in (dq, dk, dv, dt):
             if t is not None:
                 t.zero_()
         return dq, dk, dv, dt
-    d.out, d.lse, d.out_f32 = _ptr(o32 if out is None else out), _ptr(lse), _ptr(o32)
-    g = L.SvbBucketAttnGrad()
-    g.dout, g.d_q, g.d_k, g.d_v, g.d_table = _ptr(dout), _ptr(dq), _ptr(dk), _ptr(dv), _ptr(dt)
-    ws = torch.empty((lib.svb_bucket_attn_bwd_workspace_floats(C.byref(d)),), device=q.device, dtype=torch.float32)
-    g.ws = _ptr(ws)
-    _issue(q, "svb_bucket_attn_bwd", lib.svb_bucket_attn_bwd, C.byref(d), C.byref(g), st)
+    d.out, d.lse, d.out_f32 = _ptr(o32 if out is None else out), lse.data_ptr(), _ptr(o32)
+    ws = q.new_empty((lib.svb_bucket_attn_bwd_workspace_floats(_byref(d)),), dtype=torch.float32)
+    g = L.SvbBucketAttnGrad(dout.data_ptr(), _ptr(dq), _ptr(dk), _ptr(dv), _ptr(dt), ws.data_ptr())
+    _issue(q.get_device(), "svb_bucket_attn_bwd", lib.svb_bucket_attn_bwd, _byref(d), _byref(g), st)
     return dq, dk, dv, dt
 
 
