@@ -284,11 +284,15 @@ __device__ __forceinline__ int svbt_start(const SvbBucketAttn& a, int b) {
     const int s = a.q_start_b ? a.q_start_b[b] : a.q_start;
     return max(-(1 << 29), min(1 << 29, s));
 }
-// bias of this head per offset o in [-R, R], times log2(e), into LDS (every thread of the workgroup; the caller synchronises)
+// Per-offset tables in LDS reach SVBT_PAD beyond the last bucket border R: a tile of up to 64 x 32 pairs that has any pair nearer than R
+// has none further than R + 94, so its pairs index them without a clamp -- one address per sub-tile, the rest in the instructions.
+#define SVBT_PAD 96
+// bias of this head per offset o in [-R - PAD, R + PAD], times log2(e) (every thread of the workgroup; the caller synchronises)
 __device__ __forceinline__ void svbt_fill_bias(float* s_bias, const SvbBucketAttn& a, int h, int R, int nt) {
-    for (int o = threadIdx.x; o <= 2 * R; o += nt)
-        s_bias[o] = svb_ld_table(a.table, (size_t)svb_bucket_of(a.buckets, o - R) * a.H + h, a.table_dtype == SVB_DT_BF16) * SVBT_LOG2E;
+    for (int o = threadIdx.x; o <= 2 * (R + SVBT_PAD); o += nt)
+        s_bias[o] = svb_ld_table(a.table, (size_t)svb_bucket_of(a.buckets, o - R - SVBT_PAD) * a.H + h, a.table_dtype == SVB_DT_BF16) * SVBT_LOG2E;
 }
+static inline int svbt_span(const SvbRelBuckets& b) { return (2 * (svb_bucket_reach(b) + SVBT_PAD) + 1 + 3) & ~3; }
 // last kept key + 1 of a batch entry (0: none), by one wave; 512 keys' loads in flight, from the end
 __device__ __forceinline__ int svbt_keep_end(const float* keep, int n, int lane) {
     for (int j0 = (n - 1) / 512 * 512; j0 >= 0; j0 -= 512) {

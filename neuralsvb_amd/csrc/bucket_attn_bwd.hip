@@ -14,8 +14,9 @@
 // averaged over the sum), and cut into three parts for fp32 tensors; dtable sums dS in fp32 before any rounding.
 // A row whose weight is all on one key (P == 1) has dS = 0: dP - delta is then rounding noise alone.
 //
-// dtable: dS of pairs further than the last bucket border is summed in registers; nearer pairs go to LDS, where each thread has its
-// own slot per bucket, and the slots are added in order at the end.
+// dtable: dS of pairs further than the last bucket border is summed in registers; nearer pairs are added per offset in LDS, in an array
+// for each half of each wave: the 32 lanes of a half have 32 different offsets for one register, so no two lanes of an instruction
+// meet, and the arrays are added in order at the end, then over the offsets of each bucket.
 #include "attn_tiles.h"
 
 int svb_bucket_attn_check(const SvbBucketAttn* a);
@@ -25,6 +26,8 @@ struct SvbBattnBwd {
     const void* dout;
     void *dq, *dk, *dv;
     float *delta, *part;           // [B][H][Tq]; [H][B * query tiles][n_buckets] or NULL
+    float* kv_part;                // [2][splits][B][Hkv dk][Tk] sums of dS q and P dout, or NULL: one split, dk and dv are written
+    int splits;
 };
 
 __device__ __forceinline__ float svbt_ds(float p, float dp, float delta) {
@@ -74,14 +77,13 @@ __global__ __launch_bounds__(256, DKP <= 64 ? 2 : 1) void svb_bucket_attn_dq_ker
     if (!g.dq && !g.part) return;                                       // (only delta is wanted; uniform)
     const float lse = has ? a.lse[row] : SVBT_INF;
 
+    const int span = (2 * (R + SVBT_PAD) + 1 + 3) & ~3;
     float* s_bias = (float*)(smem + (DOUBLE ? 2 : 1) * BUF);
-    float* s_sum = s_bias + ((2 * R + 1 + 3) & ~3);                      // [nb][256]
-    unsigned char* s_idx = (unsigned char*)(s_sum + (g.part ? nb * 256 : 0));
+    float* s_diag = s_bias + span;                                      // [8][span], by offset + R + PAD; then [2][4] far sums
     svbt_fill_bias(s_bias, a, h, R, 256);
-    if (g.part) {
-        for (int e = 0; e < nb; ++e) s_sum[e * 256 + threadIdx.x] = 0.f;
-        for (int o = threadIdx.x; o <= 2 * R; o += 256) s_idx[o] = (unsigned char)svb_bucket_of(a.buckets, o - R);
-    }
+    if (g.part)
+        for (int e = threadIdx.x; e < 8 * span; e += 256) s_diag[e] = 0.f;
+    float* my_diag = s_diag + (wave * 2 + kb) * span + R + SVBT_PAD;
 
     const T* k = (const T*)a.k + b * a.k_sb + (long long)hk * a.dk * a.k_sc;
     const T* v = (const T*)a.v + b * a.v_sb + (long long)hk * a.dk * a.v_sc;
@@ -121,7 +123,7 @@ __global__ __launch_bounds__(256, DKP <= 64 ? 2 : 1) void svb_bucket_attn_dq_ker
         put(0);
     }
     __syncthreads();
-    const float past = s_bias[0], ahead = s_bias[2 * R];
+    const float past = s_bias[0], ahead = s_bias[2 * (R + SVBT_PAD)];
     for (int t = 0; t < tiles; ++t) {
         const unsigned long long now = seen;
         const int j0 = t * KT;
@@ -133,7 +135,7 @@ __global__ __launch_bounds__(256, DKP <= 64 ? 2 : 1) void svb_bucket_attn_dq_ker
             const bool edge = now != ALL || (a.causal && j0 + KT - 1 > p0);
             const bool behind = j0 + KT - 1 - p0 <= -R, before = j0 - p1 >= R;
             const float flat = behind ? past : ahead;
-#pragma unroll
+#pragma unroll 1
             for (int u = 0; u < NSUB; ++u) {
                 // The matrix cores round the accumulator towards -inf.  In dP that is the same small offset for every pair, and a
                 // bucket's sum over millions of pairs shows it (1e-5 of the table's gradient): the odd steps go into an accumulator of
@@ -166,13 +168,17 @@ __global__ __launch_bounds__(256, DKP <= 64 ? 2 : 1) void svb_bucket_attn_dq_ker
                     if (behind) sum_past += sum;
                     else sum_ahead += sum;
                 } else {
+                    const float* bias0 = s_bias + (o0 + R + SVBT_PAD);
+                    float* diag0 = my_diag + o0;
 #pragma unroll
                     for (int r = 0; r < 16; ++r) {
-                        const int o = max(-R, min(R, o0 + svbt_reg(r))) + R;
-                        float w = __builtin_amdgcn_exp2f(fmaf(s[r], c, s_bias[o]) - lse);
+                        float w = __builtin_amdgcn_exp2f(fmaf(s[r], c, bias0[svbt_reg(r)]) - lse);
                         if (edge) w = (su >> svbt_reg(r) & 1u) && !(a.causal && o0 + svbt_reg(r) > 0) ? w : 0.f;
                         s[r] = svbt_ds(w, dp[r], delta);
-                        if (g.part) atomicAdd(&s_sum[(int)s_idx[o] * 256 + threadIdx.x], s[r]);        // (this thread's own slot)
+                    }
+                    if (g.part) {
+#pragma unroll
+                        for (int r = 0; r < 16; ++r) atomicAdd(&diag0[svbt_reg(r)], s[r]);
                     }
                 }
 #pragma unroll
@@ -199,14 +205,28 @@ __global__ __launch_bounds__(256, DKP <= 64 ? 2 : 1) void svb_bucket_attn_dq_ker
         __syncthreads();
     }
     if (g.part) {
-        atomicAdd(&s_sum[(int)s_idx[0] * 256 + threadIdx.x], sum_past);
-        atomicAdd(&s_sum[(int)s_idx[2 * R] * 256 + threadIdx.x], sum_ahead);
+        float* far = s_diag + 8 * span;
+        sum_past = svb_wave_sum(sum_past);
+        sum_ahead = svb_wave_sum(sum_ahead);
+        if (lane == 0) { far[wave] = sum_past; far[4 + wave] = sum_ahead; }
+        __syncthreads();
+        for (int e = threadIdx.x; e < span; e += 256) {
+            float t = 0.f;
+#pragma unroll
+            for (int u = 0; u < 8; ++u) t += s_diag[u * span + e];
+            s_diag[e] = t;
+        }
         __syncthreads();
         float* part = g.part + (((size_t)h * a.B + b) * qtiles + qt) * nb;
         for (int e = wave; e < nb; e += 4) {
-            const float* x = s_sum + e * 256 + lane;
-            const float w = svb_wave_sum((x[0] + x[64]) + (x[128] + x[192]));
-            if (lane == 0) part[e] = w;
+            int o_a, o_b;
+            svb_bucket_range(a.buckets, e, o_a, o_b);
+            float t = 0.f;
+            for (int o = max(o_a + R + SVBT_PAD, 0) + lane; o < min(o_b + R + SVBT_PAD, 2 * (R + SVBT_PAD) + 1); o += 64) t += s_diag[o];
+            t = svb_wave_sum(t);
+            if (o_a <= -R - SVBT_PAD && o_b > -R - SVBT_PAD) t += (far[0] + far[1]) + (far[2] + far[3]);
+            if (o_a <= R + SVBT_PAD && o_b > R + SVBT_PAD) t += (far[4] + far[5]) + (far[6] + far[7]);
+            if (lane == 0) part[e] = t;
         }
     }
     if (!has || !g.dq) return;
@@ -221,6 +241,7 @@ __global__ __launch_bounds__(256, DKP <= 64 ? 2 : 1) void svb_bucket_attn_dq_ker
 }
 
 // ---- dk, dv: 4 waves x 32 keys, queries of the heads that share them staged -----------------------------------------------------------
+// The (head, query tile) steps of a key tile can be split over workgroups: each then leaves its sums in memory, to be added in order.
 template <typename T, int DKP, int KT, bool DOUBLE, bool TINY>
 __global__ __launch_bounds__(256, DKP <= (SvbtParts<T>::NS == 1 ? 64 : 32) ? 2 : 1) void svb_bucket_attn_dkv_kernel(SvbBucketAttn a, SvbBattnBwd g, int ktiles) {
     typedef SvbtTile<T, DKP, KT, 256, TINY> Tile;
@@ -229,8 +250,9 @@ __global__ __launch_bounds__(256, DKP <= (SvbtParts<T>::NS == 1 ? 64 : 32) ? 2 :
     HIP_DYNAMIC_SHARED(char, smem)
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l31 = lane & 31, kb = lane >> 5;
     const int item = svb_xcd_item(blockIdx.x, gridDim.x);
-    const int bk = svb_uniform(item / ktiles), b = svb_uniform(bk / a.Hkv), hk = bk - b * a.Hkv, G = svb_uniform(a.H / a.Hkv);
-    const int jt = (item - bk * ktiles) * 128, jw = jt + wave * 32, j = jw + l31;
+    const int bkt = svb_uniform(item / g.splits), split = item - bkt * g.splits;
+    const int bk = svb_uniform(bkt / ktiles), b = svb_uniform(bk / a.Hkv), hk = bk - b * a.Hkv, G = svb_uniform(a.H / a.Hkv);
+    const int jt = (bkt - bk * ktiles) * 128, jw = jt + wave * 32, j = jw + l31;
     const bool has = j < a.Tk, kept = has && (!a.keep || a.keep[(size_t)b * a.Tk + j] != 0.f);
     const int start = svbt_start(a, b), R = svb_bucket_reach(a.buckets);
     float* s_bias = (float*)(smem + (DOUBLE ? 2 : 1) * BUF);
@@ -254,8 +276,7 @@ __global__ __launch_bounds__(256, DKP <= (SvbtParts<T>::NS == 1 ? 64 : 32) ? 2 :
     const float c = a.scale * SVBT_LOG2E;
     Tile tq, td;
     float stat = 0.f;                                                   // this thread's lse (threads < KT) or delta (KT .. 2 KT - 1)
-    const int steps = G * tiles;
-    const bool any_kept = none_kept ? false : true;
+    const int n0 = svb_uniform((int)((long long)G * tiles * split / g.splits)), n1 = svb_uniform((int)((long long)G * tiles * (split + 1) / g.splits));
     auto fetch = [&](int n) {
         const int hh = hk * G + svb_uniform(n / tiles), i0 = (first + n % tiles) * KT;
         const size_t hd = (size_t)b * a.H + hh;
@@ -277,26 +298,26 @@ __global__ __launch_bounds__(256, DKP <= (SvbtParts<T>::NS == 1 ? 64 : 32) ? 2 :
         if (threadIdx.x < 2 * KT) ((float*)(buf + TILE))[threadIdx.x] = stat;
     };
     float past = 0.f, ahead = 0.f;
-    if (steps > 0) { fetch(0); put(0); }
-    for (int n = 0; n < steps; ++n) {
-        if (n % tiles == 0) {                                           // a new head's bias (every thread is behind the last tile's barrier)
+    if (n0 < n1) { fetch(n0); put(n0); }
+    for (int n = n0; n < n1; ++n) {
+        if (n == n0 || n % tiles == 0) {                                           // a new head's bias (every thread is behind the last tile's barrier)
             svbt_fill_bias(s_bias, a, hk * G + n / tiles, R, 256);
             __syncthreads();
             past = s_bias[0];
-            ahead = s_bias[2 * R];
+            ahead = s_bias[2 * (R + SVBT_PAD)];
         }
-        if (n + 1 < steps) fetch(n + 1);
+        if (n + 1 < n1) fetch(n + 1);
         const char* qrows = smem + (DOUBLE ? (n & 1) * BUF : 0);
         const char* drows = qrows + NS * Tile::ROWS_BYTES;
         const char* qcols = drows + NS * Tile::ROWS_BYTES;
         const char* dcols = qcols + NS * Tile::COLS_BYTES;
         const float* stats = (const float*)(qrows + TILE);
         const int pt = start + (first + n % tiles) * KT;                // position of the tile's first query
-        if (any_kept && !(a.causal && jw > pt + KT - 1)) {              // (wave-uniform)
+        if (!none_kept && !(a.causal && jw > pt + KT - 1)) {              // (wave-uniform)
             const bool edge = !all_kept || (a.causal && jw + 31 > pt);
             const bool behind = jw + 31 - pt <= -R, before = jw - (pt + KT - 1) >= R;
             const float flat = behind ? past : ahead;
-#pragma unroll
+#pragma unroll 1
             for (int u = 0; u < NSUB; ++u) {
                 f32x16 s, dp;
                 svbt_zero(s);
@@ -310,6 +331,7 @@ __global__ __launch_bounds__(256, DKP <= (SvbtParts<T>::NS == 1 ? 64 : 32) ? 2 :
                     svbt_mma<NS, true>(dp, f, vf[x]);
                 }
                 const int o0 = svbt_fresh(j - (pt + 32 * u + 4 * kb));   // offset of register row 0
+                const float* bias0 = s_bias + (behind || before ? 0 : o0 + R + SVBT_PAD);
 #pragma unroll
                 for (int r4 = 0; r4 < 4; ++r4) {
                     const float4 ls = *reinterpret_cast<const float4*>(stats + 32 * u + 8 * r4 + 4 * kb);
@@ -318,7 +340,7 @@ __global__ __launch_bounds__(256, DKP <= (SvbtParts<T>::NS == 1 ? 64 : 32) ? 2 :
                     for (int e = 0; e < 4; ++e) {
                         const int r = 4 * r4 + e, o = o0 - svbt_reg(r);
                         float bias = flat;
-                        if (!(behind || before)) bias = s_bias[max(-R, min(R, o)) + R];
+                        if (!(behind || before)) bias = bias0[-svbt_reg(r)];
                         float w = __builtin_amdgcn_exp2f(fmaf(s[r], c, bias) - ls[e]);
                         if (edge) w = kept && !(a.causal && o > 0) ? w : 0.f;
                         s[r] = w;
@@ -344,27 +366,53 @@ __global__ __launch_bounds__(256, DKP <= (SvbtParts<T>::NS == 1 ? 64 : 32) ? 2 :
                 }
             }
         }
-        if (n + 1 < steps) {
+        if (n + 1 < n1) {
             if (!DOUBLE) __syncthreads();
             put(n + 1);
         }
         __syncthreads();
     }
     if (!has) return;
-    const size_t head = ((size_t)b * a.Hkv + hk) * a.dk * a.Tk + j;
+    const size_t head = ((size_t)b * a.Hkv + hk) * a.dk * a.Tk + j, all = (size_t)a.B * a.Hkv * a.dk * a.Tk;
+    float* pk = g.kv_part + split * all + head;
 #pragma unroll
     for (int d = 0; d < NDB; ++d)
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
             const int ch = 32 * d + svbt_row(r, kb);
-            if (ch < a.dk) {
+            if (ch >= a.dk) continue;
+            if (g.splits > 1) {
+                pk[(size_t)ch * a.Tk] = dk[d][r];
+                pk[g.splits * all + (size_t)ch * a.Tk] = dv[d][r];
+            } else {
                 svbt_store((T*)g.dk + head + (size_t)ch * a.Tk, dk[d][r] * a.scale);
                 svbt_store((T*)g.dv + head + (size_t)ch * a.Tk, dv[d][r]);
             }
         }
 }
 
+// dk (blockIdx.y 0, times scale) and dv (1) from their splits
+template <typename T>
+__global__ __launch_bounds__(256) void svb_bucket_attn_kv_sum_kernel(SvbBattnBwd g, size_t all, float scale) {
+    const float* part = g.kv_part + blockIdx.y * g.splits * all;
+    T* out = (T*)(blockIdx.y ? g.dv : g.dk);
+    const float f = blockIdx.y ? 1.f : scale;
+    for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < all; i += (size_t)gridDim.x * 256) {
+        float t = 0.f;
+        for (int s = 0; s < g.splits; ++s) t += part[s * all + i];
+        svbt_store(out + i, t * f);
+    }
+}
+
 // ---- host ------------------------------------------------------------------------------------------------------------------------
+// Splits of a key tile's steps: workgroups for two per CU (B2 H16/4 dk128 T2048 causal has 128 key tiles: 859 us with one split), of at
+// least four steps each.
+static int kv_splits(const SvbBucketAttn* a) {
+    const long tiles = (long)a->B * a->Hkv * ((a->Tk + 127) / 128), steps = (long)(a->H / a->Hkv) * ((a->Tq + 63) / 64);
+    const long want = (512 + tiles - 1) / tiles, most = steps / 4 < 8 ? steps / 4 : 8;
+    return (int)(want < most ? want : most > 1 ? most : 1);
+}
+
 template <typename K>
 static int bwd_lds(K* kern, int lds) {
     return lds > 65536 && hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024) != hipSuccess;
@@ -373,9 +421,8 @@ static int bwd_lds(K* kern, int lds) {
 template <typename T, int DKP, int KT, bool DOUBLE, bool TINY = false>
 static int dq_launch(const SvbBucketAttn* a, const SvbBattnBwd& g, hipStream_t st) {
     typedef SvbtTile<T, DKP, KT, 256, TINY> Tile;
-    const int span = 2 * svb_bucket_reach(a->buckets) + 1, qtiles = (a->Tq + 127) / 128;
-    int lds = (DOUBLE ? 2 : 1) * Tile::NS * (2 * Tile::ROWS_BYTES + Tile::COLS_BYTES) + ((span + 3) & ~3) * 4;
-    if (g.part) lds += a->buckets.n_buckets * 1024 + span;
+    const int span = svbt_span(a->buckets), qtiles = (a->Tq + 127) / 128;
+    const int lds = (DOUBLE ? 2 : 1) * Tile::NS * (2 * Tile::ROWS_BYTES + Tile::COLS_BYTES) + (g.part ? 9 * span + 8 : span) * 4;
     auto* kern = svb_bucket_attn_dq_kernel<T, DKP, KT, DOUBLE, TINY>;
     if (bwd_lds(kern, lds)) return SVB_ERR_LAUNCH;
     hipLaunchKernelGGL(kern, dim3((unsigned)(a->B * a->H * qtiles)), dim3(256), lds, st, *a, g, qtiles);
@@ -386,20 +433,30 @@ static int dq_launch(const SvbBucketAttn* a, const SvbBattnBwd& g, hipStream_t s
 template <typename T, int DKP, int KT, bool DOUBLE, bool TINY = false>
 static int dkv_launch(const SvbBucketAttn* a, const SvbBattnBwd& g, hipStream_t st) {
     typedef SvbtTile<T, DKP, KT, 256, TINY> Tile;
-    const int span = 2 * svb_bucket_reach(a->buckets) + 1, ktiles = (a->Tk + 127) / 128;
+    const int span = svbt_span(a->buckets), ktiles = (a->Tk + 127) / 128;
     const int lds = (DOUBLE ? 2 : 1) * (2 * Tile::NS * (Tile::ROWS_BYTES + Tile::COLS_BYTES) + 2 * KT * 4) + span * 4;
     auto* kern = svb_bucket_attn_dkv_kernel<T, DKP, KT, DOUBLE, TINY>;
     if (bwd_lds(kern, lds)) return SVB_ERR_LAUNCH;
-    hipLaunchKernelGGL(kern, dim3((unsigned)(a->B * a->Hkv * ktiles)), dim3(256), lds, st, *a, g, ktiles);
+    hipLaunchKernelGGL(kern, dim3((unsigned)(a->B * a->Hkv * ktiles * g.splits)), dim3(256), lds, st, *a, g, ktiles);
     SVB_CHECK_LAUNCH();
+    if (g.splits > 1) {
+        const size_t all = (size_t)a->B * a->Hkv * a->dk * a->Tk;
+        const unsigned grid = (unsigned)((all + 255) / 256 < 2048 ? (all + 255) / 256 : 2048);
+        hipLaunchKernelGGL((svb_bucket_attn_kv_sum_kernel<T>), dim3(grid, 2), dim3(256), 0, st, g, all, a->scale);
+        SVB_CHECK_LAUNCH();
+    }
     return SVB_OK;
 }
 
 static size_t delta_floats(const SvbBucketAttn* a) { return ((size_t)a->B * a->H * a->Tq + 3) & ~(size_t)3; }
+static size_t table_floats(const SvbBucketAttn* a) {
+    return ((size_t)a->H * a->B * ((a->Tq + 127) / 128) * a->buckets.n_buckets + 3) & ~(size_t)3;
+}
 
 extern "C" size_t svb_bucket_attn_bwd_workspace_floats(const SvbBucketAttn* a) {
-    if (!a || a->B <= 0 || a->H <= 0 || a->Tq <= 0) return 0;
-    return delta_floats(a) + (size_t)a->H * a->B * ((a->Tq + 127) / 128) * a->buckets.n_buckets;
+    if (svb_bucket_attn_check(a) != SVB_OK) return 0;
+    const int splits = kv_splits(a);
+    return delta_floats(a) + table_floats(a) + (splits > 1 ? 2 * (size_t)splits * a->B * a->Hkv * a->dk * a->Tk : 0);
 }
 
 extern "C" int svb_bucket_attn_bwd(const SvbBucketAttn* a, const SvbBucketAttnGrad* g, void* stream) {
@@ -407,7 +464,8 @@ extern "C" int svb_bucket_attn_bwd(const SvbBucketAttn* a, const SvbBucketAttnGr
     if (rc != SVB_OK) return rc;
     if (!g || !g->dout || !g->ws || !a->lse || (a->dtype == SVB_DT_BF16 && !a->out_f32) || (!g->d_k != !g->d_v)) return SVB_ERR_ARG;
     hipStream_t st = (hipStream_t)stream;
-    SvbBattnBwd w = {g->dout, g->d_q, g->d_k, g->d_v, g->ws, g->d_table ? g->ws + delta_floats(a) : nullptr};
+    SvbBattnBwd w = {g->dout, g->d_q, g->d_k, g->d_v, g->ws, g->d_table ? g->ws + delta_floats(a) : nullptr, nullptr, kv_splits(a)};
+    if (w.splits > 1) w.kv_part = g->ws + delta_floats(a) + table_floats(a);
     // (double buffers where two workgroups of them fit a CU)
     if (a->dtype == SVB_DT_BF16) {
         typedef unsigned short T;

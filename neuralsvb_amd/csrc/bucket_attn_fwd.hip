@@ -21,16 +21,13 @@ template <int NDB> struct SvbtState {
 };
 
 // One 32-key sub-tile's scores -> t (log2 units) in place.  NEAR: the bias varies.  EDGE: some pair is hidden.
-// o0: offset of register row 0 of this lane, j0 + 4 kb - p_i; seen: the sub-tile's key bits from 4 kb on.
+// o0: offset of register row 0 of this lane, j0 + 4 kb - p_i; bias0: the bias at o0; seen: the sub-tile's key bits from 4 kb on.
 template <bool NEAR, bool EDGE>
-__device__ __forceinline__ void svbt_scores(f32x16& s, float c, const float* s_bias, int R, float flat, int o0, bool causal, unsigned seen) {
+__device__ __forceinline__ void svbt_scores(f32x16& s, float c, const float* bias0, float flat, int o0, bool causal, unsigned seen) {
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
-        const int o = o0 + svbt_reg(r);
-        float bias = flat;
-        if (NEAR) bias = s_bias[max(-R, min(R, o)) + R];
-        s[r] = fmaf(s[r], c, bias);
-        if (EDGE) s[r] = (seen >> svbt_reg(r) & 1u) && !(causal && o > 0) ? s[r] : -SVBT_INF;
+        s[r] = fmaf(s[r], c, NEAR ? bias0[svbt_reg(r)] : flat);
+        if (EDGE) s[r] = (seen >> svbt_reg(r) & 1u) && !(causal && o0 + svbt_reg(r) > 0) ? s[r] : -SVBT_INF;
     }
 }
 
@@ -129,7 +126,7 @@ __global__ __launch_bounds__(256, DKP <= 64 ? 2 : 1) void svb_bucket_attn_fwd_ke
         put(0);
     }
     __syncthreads();
-    const float past = s_bias[0], ahead = s_bias[2 * R];
+    const float past = s_bias[0], ahead = s_bias[2 * (R + SVBT_PAD)];
     for (int t = 0; t < tiles; ++t) {
         const unsigned long long now = seen;
         const int j0 = t * KT;
@@ -156,11 +153,12 @@ __global__ __launch_bounds__(256, DKP <= 64 ? 2 : 1) void svb_bucket_attn_fwd_ke
                 const unsigned su = (unsigned)(now >> (32 * u)) >> (4 * kb);
                 const int o0 = svbt_fresh(j0 + 32 * u + 4 * kb - p);
                 if (behind || before) {
-                    if (edge) svbt_scores<false, true>(s[u], c, s_bias, R, flat, o0, a.causal, su);
-                    else svbt_scores<false, false>(s[u], c, s_bias, R, flat, o0, a.causal, su);
+                    if (edge) svbt_scores<false, true>(s[u], c, nullptr, flat, o0, a.causal, su);
+                    else svbt_scores<false, false>(s[u], c, nullptr, flat, o0, a.causal, su);
                 } else {
-                    if (edge) svbt_scores<true, true>(s[u], c, s_bias, R, flat, o0, a.causal, su);
-                    else svbt_scores<true, false>(s[u], c, s_bias, R, flat, o0, a.causal, su);
+                    const float* bias0 = s_bias + (o0 + R + SVBT_PAD);
+                    if (edge) svbt_scores<true, true>(s[u], c, bias0, flat, o0, a.causal, su);
+                    else svbt_scores<true, false>(s[u], c, bias0, flat, o0, a.causal, su);
                 }
             }
             svbt_softmax<NSUB, NDB>(s, st);
@@ -492,7 +490,7 @@ int svb_bucket_attn_check(const SvbBucketAttn* a) {
 template <typename T, int DKP, int KT, bool DOUBLE, int PP, bool TINY = false>
 static int fwd_launch(const SvbBucketAttn* a, hipStream_t st) {
     typedef SvbtTile<T, DKP, KT, 256, TINY> Tile;
-    const int lds = (DOUBLE ? 2 : 1) * Tile::NS * (Tile::ROWS_BYTES + Tile::COLS_BYTES) + (2 * svb_bucket_reach(a->buckets) + 1) * 4;
+    const int lds = (DOUBLE ? 2 : 1) * Tile::NS * (Tile::ROWS_BYTES + Tile::COLS_BYTES) + svbt_span(a->buckets) * 4;
     auto* kern = svb_bucket_attn_fwd_kernel<T, DKP, KT, DOUBLE, PP, TINY>;
     if (lds > 65536 && hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024) != hipSuccess) return SVB_ERR_LAUNCH;
     const int qtiles = (a->Tq + 127) / 128;

@@ -122,14 +122,8 @@ __global__ __launch_bounds__(256) void svb_bucket_bias_bwd_kernel(const T* dbias
     const int lane = threadIdx.x & 63;
     float* row = part + ((size_t)h * gridDim.y * gridDim.x + (size_t)blockIdx.y * gridDim.x + blockIdx.x) * bk.n_buckets;
     for (int k = threadIdx.x >> 6; k < bk.n_buckets; k += 4) {
-        const int side = bk.both ? bk.n_buckets / 2 : bk.n_buckets, m = bk.both && k >= side ? k - side : k;
-        // distances lo <= d < hi of the side's bucket m
-        const int far = 0x3fffffff;
-        const int lo = m <= bk.near ? m : (m - bk.near <= bk.n_edge ? bk.edge[m - bk.near - 1] : far);
-        const int hi = m < bk.near ? m + 1 : (m - bk.near < bk.n_edge ? bk.edge[m - bk.near] : far);
-        int a, b;                                                       // offsets a <= o < b
-        if (bk.both && k >= side) { a = max(lo, 1); b = hi; }
-        else { a = 1 - hi; b = 1 - lo; if (!bk.both && m == 0) b = far; }
+        int a, b;
+        svb_bucket_range(bk, k, a, b);
         a = max(a + start - tile0, 0);
         b = min(b + start - tile0, SVB_BB_OFFS);
         float t = 0.f;

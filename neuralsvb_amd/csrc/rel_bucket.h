@@ -34,6 +34,17 @@ __device__ __forceinline__ int svb_bucket_of(const SvbRelBuckets& b, int off) {
     return k;
 }
 
+// the offsets a <= o < b that bucket k holds (one run; empty where k is not used)
+#define SVB_REL_FAR 0x3fffffff
+__device__ __forceinline__ void svb_bucket_range(const SvbRelBuckets& bk, int k, int& a, int& b) {
+    const int side = bk.both ? bk.n_buckets / 2 : bk.n_buckets, m = bk.both && k >= side ? k - side : k;
+    // distances lo <= d < hi of the side's bucket m
+    const int lo = m <= bk.near ? m : (m - bk.near <= bk.n_edge ? bk.edge[m - bk.near - 1] : SVB_REL_FAR);
+    const int hi = m < bk.near ? m + 1 : (m - bk.near < bk.n_edge ? bk.edge[m - bk.near] : SVB_REL_FAR);
+    if (bk.both && k >= side) { a = max(lo, 1); b = hi; }
+    else { a = 1 - hi; b = !bk.both && m == 0 ? SVB_REL_FAR : 1 - lo; }
+}
+
 // host: is this a partition that the kernels can index with?
 static inline bool svb_bucket_valid(const SvbRelBuckets* b) {
     if (!b || b->n_buckets < 2 || b->n_buckets > SVB_REL_MAX_BUCKETS || (b->both && (b->n_buckets & 1))) return false;
