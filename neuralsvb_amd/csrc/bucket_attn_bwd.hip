@@ -14,9 +14,11 @@
 // averaged over the sum), and cut into three parts for fp32 tensors; dtable sums dS in fp32 before any rounding.
 // A row whose weight is all on one key (P == 1) has dS = 0: dP - delta is then rounding noise alone.
 //
-// dtable: dS of pairs further than the last bucket border is summed in registers; nearer pairs are added per offset in LDS, in an array
-// for each half of each wave: the 32 lanes of a half have 32 different offsets for one register, so no two lanes of an instruction
-// meet, and the arrays are added in order at the end, then over the offsets of each bucket.
+// dtable: dS of pairs further than the last bucket border is summed in registers.  Nearer pairs are summed along the diagonals of each
+// 32 x 32 sub-tile: the tile goes to LDS skewed, row (key - query) mod 32, which puts the diagonals d and d - 32 side by side into one row of
+// 32, and comes back one row half per lane.  That is 16 writes and 4 wide reads per lane; adding each value to its offset's sum with an LDS
+// atomic instead (87 cycles each, measured) took 37 of the 61 us of this kernel at B24 H4 dk48 T211.  The sums per offset stay in LDS, an
+// array per wave, and are added in order at the end, then over the offsets of each bucket.
 #include "attn_tiles.h"
 
 int svb_bucket_attn_check(const SvbBucketAttn* a);
@@ -33,6 +35,35 @@ struct SvbBattnBwd {
 __device__ __forceinline__ float svbt_ds(float p, float dp, float delta) {
     const float ds = p * (dp - delta);
     return p == 0.f || p == 1.f ? 0.f : ds;
+}
+
+// Adds a sub-tile's diagonal sums to diag[key - query], one wave.  s: register r is key svbt_row(r, kb) of query l31; skew: [32][36] floats
+// (rows of 36: the writes of 32 lanes, 35 words apart, and the 16-byte reads fall on different banks).
+#define SVBT_SKEW_P 36
+__device__ __forceinline__ void svbt_diag_add(float* skew, float* diag, const f32x16& s, int l31, int kb) {
+    const int t = svbt_fresh(4 * kb - l31);
+    __builtin_amdgcn_wave_barrier();                                    // (the last sub-tile's reads are done)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) skew[((svbt_reg(r) + t) & 31) * SVBT_SKEW_P + l31] = s[r];
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    // row l31, queries 16 kb .. 16 kb + 15: those up to 31 - l31 are of diagonal l31, the others of l31 - 32
+    const int last = 31 - l31 - 16 * kb;
+    float here = 0.f, there = 0.f;
+#pragma unroll
+    for (int m = 0; m < 4; ++m) {
+        const float4 v = *reinterpret_cast<const float4*>(skew + l31 * SVBT_SKEW_P + 16 * kb + 4 * m);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const float x = 4 * m + e <= last ? v[e] : 0.f;
+            here += x;
+            there += v[e] - x;                                          // (exactly v or 0)
+        }
+    }
+    here += __shfl_xor(here, 32, 64);
+    there += __shfl_xor(there, 32, 64);
+    diag[kb ? l31 - 32 : l31] += kb ? there : here;                     // (64 different offsets)
 }
 
 // ---- dq, dtable, delta: 4 waves x 32 queries, keys staged ----------------------------------------------------------------------------
@@ -79,11 +110,12 @@ __global__ __launch_bounds__(256, DKP <= 64 ? 2 : 1) void svb_bucket_attn_dq_ker
 
     const int span = (2 * (R + SVBT_PAD) + 1 + 3) & ~3;
     float* s_bias = (float*)(smem + (DOUBLE ? 2 : 1) * BUF);
-    float* s_diag = s_bias + span;                                      // [8][span], by offset + R + PAD; then [2][4] far sums
+    float* s_skew = s_bias + span;                                      // [4][32][SVBT_SKEW_P]
+    float* s_diag = s_skew + 4 * 32 * SVBT_SKEW_P;                       // [4][span], by offset + R + PAD; then [2][4] far sums
     svbt_fill_bias(s_bias, a, h, R, 256);
     if (g.part)
-        for (int e = threadIdx.x; e < 8 * span; e += 256) s_diag[e] = 0.f;
-    float* my_diag = s_diag + (wave * 2 + kb) * span + R + SVBT_PAD;
+        for (int e = threadIdx.x; e < 4 * span; e += 256) s_diag[e] = 0.f;
+    float *my_skew = s_skew + wave * 32 * SVBT_SKEW_P, *my_diag = s_diag + wave * span + R + SVBT_PAD;
 
     const T* k = (const T*)a.k + b * a.k_sb + (long long)hk * a.dk * a.k_sc;
     const T* v = (const T*)a.v + b * a.v_sb + (long long)hk * a.dk * a.v_sc;
@@ -169,17 +201,13 @@ __global__ __launch_bounds__(256, DKP <= 64 ? 2 : 1) void svb_bucket_attn_dq_ker
                     else sum_ahead += sum;
                 } else {
                     const float* bias0 = s_bias + (o0 + R + SVBT_PAD);
-                    float* diag0 = my_diag + o0;
 #pragma unroll
                     for (int r = 0; r < 16; ++r) {
                         float w = __builtin_amdgcn_exp2f(fmaf(s[r], c, bias0[svbt_reg(r)]) - lse);
                         if (edge) w = (su >> svbt_reg(r) & 1u) && !(a.causal && o0 + svbt_reg(r) > 0) ? w : 0.f;
                         s[r] = svbt_ds(w, dp[r], delta);
                     }
-                    if (g.part) {
-#pragma unroll
-                        for (int r = 0; r < 16; ++r) atomicAdd(&diag0[svbt_reg(r)], s[r]);
-                    }
+                    if (g.part) svbt_diag_add(my_skew, my_diag + (j0 + 32 * u - p0), s, l31, kb);
                 }
 #pragma unroll
                 for (int x = 0; x < 2; ++x) {
@@ -205,16 +233,13 @@ __global__ __launch_bounds__(256, DKP <= 64 ? 2 : 1) void svb_bucket_attn_dq_ker
         __syncthreads();
     }
     if (g.part) {
-        float* far = s_diag + 8 * span;
+        float* far = s_diag + 4 * span;
         sum_past = svb_wave_sum(sum_past);
         sum_ahead = svb_wave_sum(sum_ahead);
         if (lane == 0) { far[wave] = sum_past; far[4 + wave] = sum_ahead; }
         __syncthreads();
         for (int e = threadIdx.x; e < span; e += 256) {
-            float t = 0.f;
-#pragma unroll
-            for (int u = 0; u < 8; ++u) t += s_diag[u * span + e];
-            s_diag[e] = t;
+            s_diag[e] = (s_diag[e] + s_diag[span + e]) + (s_diag[2 * span + e] + s_diag[3 * span + e]);
         }
         __syncthreads();
         float* part = g.part + (((size_t)h * a.B + b) * qtiles + qt) * nb;
@@ -422,7 +447,7 @@ template <typename T, int DKP, int KT, bool DOUBLE, bool TINY = false>
 static int dq_launch(const SvbBucketAttn* a, const SvbBattnBwd& g, hipStream_t st) {
     typedef SvbtTile<T, DKP, KT, 256, TINY> Tile;
     const int span = svbt_span(a->buckets), qtiles = (a->Tq + 127) / 128;
-    const int lds = (DOUBLE ? 2 : 1) * Tile::NS * (2 * Tile::ROWS_BYTES + Tile::COLS_BYTES) + (g.part ? 9 * span + 8 : span) * 4;
+    const int lds = (DOUBLE ? 2 : 1) * Tile::NS * (2 * Tile::ROWS_BYTES + Tile::COLS_BYTES) + (g.part ? 5 * span + 4 * 32 * SVBT_SKEW_P + 8 : span) * 4;
     auto* kern = svb_bucket_attn_dq_kernel<T, DKP, KT, DOUBLE, TINY>;
     if (bwd_lds(kern, lds)) return SVB_ERR_LAUNCH;
     hipLaunchKernelGGL(kern, dim3((unsigned)(a->B * a->H * qtiles)), dim3(256), lds, st, *a, g, qtiles);
