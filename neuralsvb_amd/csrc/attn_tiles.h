@@ -100,22 +100,33 @@ __device__ __forceinline__ float svbt_load(const unsigned short* p) { return svb
 __device__ __forceinline__ void svbt_store(float* p, float v) { *p = v; }
 __device__ __forceinline__ void svbt_store(unsigned short* p, float v) { *p = (unsigned short)svbt_pack2(v, v); }
 
-// Operand of this lane's own column t (position) for the channels 16 s + 8 kb + 0..7: read once per workgroup, 32 lanes along time.
-// `has` false or a channel beyond dk: zeros, whatever memory holds there.  Read without a branch (t has to exist, a channel that does
-// not exist reads the last one): a load under a condition is waited for before the next one, and a workgroup begins with dk of them.
-template <typename T>
-__device__ __forceinline__ void svbt_own8(const T* base, long long sc, int t, int s, int kb, int dk, bool has, float (&v)[8]) {
+// Operands of this lane's own column t (position), channels 16 s + 8 kb + 0..7: read once per workgroup, 32 lanes along time.  Loaded
+// without a branch (t has to exist, a channel that does not exist reads the last one) -- a load under a condition is waited for before the
+// next one -- and taken apart later: a workgroup begins by issuing these, its first tile and its tables together, one memory latency in all.
+template <typename T, int NK>
+struct SvbtOwn {
+    T r[NK][8];
+    __device__ __forceinline__ void load(const T* base, long long sc, int t, int kb, int dk) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = svbt_load(base + min(16 * s + 8 * kb + e, dk - 1) * sc + t);
+        for (int s = 0; s < NK; ++s)
 #pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = has && 16 * s + 8 * kb + e < dk ? v[e] : 0.f;
-}
-template <typename T, int NS>
-__device__ __forceinline__ void svbt_own_frag(const T* base, long long sc, int t, int s, int kb, int dk, bool has, svbt_bf16x8 (&f)[NS]) {
-    float v[8];
-    svbt_own8(base, sc, t, s, kb, dk, has, v);
-    svbt_frag8<NS>(v, f);
-}
+            for (int e = 0; e < 8; ++e) r[s][e] = base[min(16 * s + 8 * kb + e, dk - 1) * sc + t];
+    }
+    // the values of step s; `has` false or a channel beyond dk: zeros, whatever memory holds there
+    __device__ __forceinline__ void get(int s, int kb, int dk, bool has, float (&v)[8]) const {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = has && 16 * s + 8 * kb + e < dk ? svbt_load(&r[s][e]) : 0.f;
+    }
+    template <int NS>
+    __device__ __forceinline__ void frags(int kb, int dk, bool has, svbt_bf16x8 (&f)[NK][NS]) const {
+#pragma unroll
+        for (int s = 0; s < NK; ++s) {
+            float v[8];
+            get(s, kb, dk, has, v);
+            svbt_frag8<NS>(v, f[s]);
+        }
+    }
+};
 
 // ---- staged tiles ----------------------------------------------------------------------------------------------------------
 // One 4 channel x 4 position block as loaded.  row(c): the c-th channel's four elements, any element-aligned address.
@@ -281,7 +292,8 @@ struct SvbtTile {
 // ---- positions and masks -----------------------------------------------------------------------------------------------------
 // position of query 0 of batch entry b; far beyond any key it makes no difference how far
 __device__ __forceinline__ int svbt_start(const SvbBucketAttn& a, int b) {
-    const int s = a.q_start_b ? a.q_start_b[b] : a.q_start;
+    int s = a.q_start;
+    if (a.q_start_b) s = a.q_start_b[b];                                // (a branch: a choice between the two addresses is a flat load)
     return max(-(1 << 29), min(1 << 29, s));
 }
 // Per-offset tables in LDS reach SVBT_PAD beyond the last bucket border R: a tile of up to 64 x 32 pairs that has any pair nearer than R

@@ -81,27 +81,43 @@ __global__ __launch_bounds__(256, DKP <= 64 ? 2 : 1) void svb_bucket_attn_dq_ker
     const bool has = i < a.Tq;
     const int start = svbt_start(a, b), R = svb_bucket_reach(a.buckets), nb = a.buckets.n_buckets;
 
+    const T* k = (const T*)a.k + b * a.k_sb + (long long)hk * a.dk * a.k_sc;
+    const T* v = (const T*)a.v + b * a.v_sb + (long long)hk * a.dk * a.v_sc;
+    const float* keep = a.keep ? a.keep + (size_t)b * a.Tk : nullptr;
+    Tile tk, tv;
+    float kept = 1.f;
+    auto fetch = [&](int t) {
+        tk.load(k, a.k_sc, t * KT, a.Tk, a.dk);
+        tv.load(v, a.v_sc, t * KT, a.Tk, a.dk);
+        if (keep) kept = keep[min(t * KT + lane, a.Tk - 1)];
+    };
     // own operands, and delta on the way
     const T* q = (const T*)a.q + b * a.q_sb + (long long)h * a.dk * a.q_sc;
     const size_t head = ((size_t)b * a.H + h) * a.dk * a.Tq;
-    const T* dout = (const T*)g.dout + head;
-    const float* out = (NS == 3 ? (const float*)a.out : a.out_f32) + head;
     const int ic = has ? i : 0;
     const size_t row = ((size_t)b * a.H + h) * a.Tq + ic;
     svbt_bf16x8 qf[NK][NS], of[NK][NS];
     float delta = 0.f;
+    {
+        SvbtOwn<T, NK> own_q, own_do;
+        SvbtOwn<float, NK> own_o;
+        own_do.load((const T*)g.dout + head, a.Tq, ic, kb, a.dk);
+        own_o.load((NS == 3 ? (const float*)a.out : a.out_f32) + head, a.Tq, ic, kb, a.dk);
+        own_q.load(q, a.q_sc, ic, kb, a.dk);
+        if (g.dq || g.part) fetch(0);                                   // (uniform)
 #pragma unroll
-    for (int s = 0; s < NK; ++s) {
-        svbt_own_frag<T, NS>(q, a.q_sc, ic, s, kb, a.dk, has, qf[s]);
-        float v[8], o[8];
-        svbt_own8(dout, a.Tq, ic, s, kb, a.dk, has, v);
-        svbt_own8(out, a.Tq, ic, s, kb, a.dk, has, o);
+        for (int s = 0; s < NK; ++s) {
+            float v8[8], o8[8];
+            own_do.get(s, kb, a.dk, has, v8);
+            own_o.get(s, kb, a.dk, has, o8);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            delta = fmaf(v[e], o[e], delta);
-            if (s & 1) v[e] = -v[e];                                    // (see dp_neg below)
+            for (int e = 0; e < 8; ++e) {
+                delta = fmaf(v8[e], o8[e], delta);
+                if (s & 1) v8[e] = -v8[e];                              // (see dp_neg below)
+            }
+            svbt_frag8<NS>(v8, of[s]);
         }
-        svbt_frag8<NS>(v, of[s]);
+        own_q.frags(kb, a.dk, has, qf);
     }
     delta += __shfl_xor(delta, 32, 64);
     if (has && kb == 0) g.delta[row] = delta;
@@ -117,9 +133,6 @@ __global__ __launch_bounds__(256, DKP <= 64 ? 2 : 1) void svb_bucket_attn_dq_ker
         for (int e = threadIdx.x; e < 4 * span; e += 256) s_diag[e] = 0.f;
     float *my_skew = s_skew + wave * 32 * SVBT_SKEW_P, *my_diag = s_diag + wave * span + R + SVBT_PAD;
 
-    const T* k = (const T*)a.k + b * a.k_sb + (long long)hk * a.dk * a.k_sc;
-    const T* v = (const T*)a.v + b * a.v_sb + (long long)hk * a.dk * a.v_sc;
-    const float* keep = a.keep ? a.keep + (size_t)b * a.Tk : nullptr;
     int end = keep ? svbt_keep_end(keep, a.Tk, lane) : a.Tk;
     if (a.causal) end = max(0, min(end, start + min(i0 + 128, a.Tq)));
     const int p0 = start + i0 + wave * 32, p1 = p0 + 31, p = start + i;
@@ -131,15 +144,8 @@ __global__ __launch_bounds__(256, DKP <= 64 ? 2 : 1) void svb_bucket_attn_dq_ker
     for (int d = 0; d < NDB; ++d) svbt_zero(acc[d]);
     float sum_past = 0.f, sum_ahead = 0.f;
 
-    Tile tk, tv;
     unsigned long long seen = ~0ull;                                    // of the tile in LDS: the keys that exist and are kept
-    float kept = 1.f;
     constexpr unsigned long long ALL = KT == 64 ? ~0ull : 0xffffffffull;
-    auto fetch = [&](int t) {
-        tk.load(k, a.k_sc, t * KT, a.Tk, a.dk);
-        tv.load(v, a.v_sc, t * KT, a.Tk, a.dk);
-        if (keep) kept = keep[min(t * KT + lane, a.Tk - 1)];
-    };
     auto bits = [&](int t) { return ALL & __ballot(t * KT + lane < end && kept != 0.f); };
     auto put = [&](int t) {
         const unsigned long long m = seen == ALL ? ~0ull : seen;
@@ -150,7 +156,6 @@ __global__ __launch_bounds__(256, DKP <= 64 ? 2 : 1) void svb_bucket_attn_dq_ker
         tv.template store<true, false>(buf + NS * Tile::ROWS_BYTES, nullptr);
     };
     if (tiles > 0) {
-        fetch(0);
         seen = bits(0);
         put(0);
     }
@@ -284,12 +289,9 @@ __global__ __launch_bounds__(256, DKP <= (SvbtParts<T>::NS == 1 ? 64 : 32) ? 2 :
 
     const T* k = (const T*)a.k + b * a.k_sb + (long long)hk * a.dk * a.k_sc;
     const T* v = (const T*)a.v + b * a.v_sb + (long long)hk * a.dk * a.v_sc;
-    svbt_bf16x8 kf[NK][NS], vf[NK][NS];
-#pragma unroll
-    for (int s = 0; s < NK; ++s) {
-        svbt_own_frag<T, NS>(k, a.k_sc, has ? j : 0, s, kb, a.dk, kept, kf[s]);
-        svbt_own_frag<T, NS>(v, a.v_sc, has ? j : 0, s, kb, a.dk, kept, vf[s]);
-    }
+    SvbtOwn<T, NK> own_k, own_v;
+    own_k.load(k, a.k_sc, has ? j : 0, kb, a.dk);
+    own_v.load(v, a.v_sc, has ? j : 0, kb, a.dk);
     const bool all_kept = __ballot(!kept) == 0ull, none_kept = __ballot(kept) == 0ull;
     f32x16 dk[NDB], dv[NDB];
 #pragma unroll
@@ -323,7 +325,11 @@ __global__ __launch_bounds__(256, DKP <= (SvbtParts<T>::NS == 1 ? 64 : 32) ? 2 :
         if (threadIdx.x < 2 * KT) ((float*)(buf + TILE))[threadIdx.x] = stat;
     };
     float past = 0.f, ahead = 0.f;
-    if (n0 < n1) { fetch(n0); put(n0); }
+    if (n0 < n1) fetch(n0);
+    svbt_bf16x8 kf[NK][NS], vf[NK][NS];
+    own_k.frags(kb, a.dk, kept, kf);
+    own_v.frags(kb, a.dk, kept, vf);
+    if (n0 < n1) put(n0);
     for (int n = n0; n < n1; ++n) {
         if (n == n0 || n % tiles == 0) {                                           // a new head's bias (every thread is behind the last tile's barrier)
             svbt_fill_bias(s_bias, a, hk * G + n / tiles, R, 256);
@@ -484,9 +490,12 @@ extern "C" size_t svb_bucket_attn_bwd_workspace_floats(const SvbBucketAttn* a) {
     return delta_floats(a) + table_floats(a) + (splits > 1 ? 2 * (size_t)splits * a->B * a->Hkv * a->dk * a->Tk : 0);
 }
 
-extern "C" int svb_bucket_attn_bwd(const SvbBucketAttn* a, const SvbBucketAttnGrad* g, void* stream) {
-    int rc = svb_bucket_attn_check(a);
+extern "C" int svb_bucket_attn_bwd(const SvbBucketAttn* call, const SvbBucketAttnGrad* g, void* stream) {
+    int rc = svb_bucket_attn_check(call);
     if (rc != SVB_OK) return rc;
+    SvbBucketAttn filled = *call;
+    svb_bucket_fill(&filled.buckets);
+    const SvbBucketAttn* a = &filled;
     if (!g || !g->dout || !g->ws || !a->lse || (a->dtype == SVB_DT_BF16 && !a->out_f32) || (!g->d_k != !g->d_v)) return SVB_ERR_ARG;
     hipStream_t st = (hipStream_t)stream;
     SvbBattnBwd w = {g->dout, g->d_q, g->d_k, g->d_v, g->ws, g->d_table ? g->ws + delta_floats(a) : nullptr, nullptr, kv_splits(a)};

@@ -76,24 +76,32 @@ __global__ __launch_bounds__(256, DKP <= 64 ? 2 : 1) void svb_bucket_attn_fwd_ke
     const int qt = a.causal ? qtiles - 1 - (item - bh * qtiles) : item - bh * qtiles;      // (causal: the longest rows first)
     const int i0 = qt * 128, i = i0 + wave * 32 + l31;
     const bool has = i < a.Tq;
-    const int start = svbt_start(a, b);
-    const int R = svb_bucket_reach(a.buckets);
-    float* s_bias = (float*)(smem + (DOUBLE ? 2 : 1) * BUF);
-    svbt_fill_bias(s_bias, a, h, R, 256);
-
     const T* q = (const T*)a.q + b * a.q_sb + (long long)h * a.dk * a.q_sc;
     const T* k = (const T*)a.k + b * a.k_sb + (long long)hk * a.dk * a.k_sc;
     const T* v = (const T*)a.v + b * a.v_sb + (long long)hk * a.dk * a.v_sc;
     const float* keep = a.keep ? a.keep + (size_t)b * a.Tk : nullptr;
-    svbt_bf16x8 qf[NK][NS];
-#pragma unroll
-    for (int s = 0; s < NK; ++s) svbt_own_frag<T, NS>(q, a.q_sc, has ? i : 0, s, kb, a.dk, has, qf[s]);
+    Tile tk, tv;
+    float kept = 1.f;
+    auto fetch = [&](int t) {                                            // loads of tile t
+        tk.load(k, a.k_sc, t * KT, a.Tk, a.dk);
+        tv.load(v, a.v_sc, t * KT, a.Tk, a.dk);
+        if (keep) kept = keep[min(t * KT + lane, a.Tk - 1)];
+    };
+    fetch(0);
+    SvbtOwn<T, NK> own;
+    own.load(q, a.q_sc, has ? i : 0, kb, a.dk);
+    const int start = svbt_start(a, b);
+    const int R = svb_bucket_reach(a.buckets);
+    float* s_bias = (float*)(smem + (DOUBLE ? 2 : 1) * BUF);
+    svbt_fill_bias(s_bias, a, h, R, 256);
 
     // keys that anyone here sees end at `end`; this wave's queries are at positions p0 .. p1
     int end = keep ? svbt_keep_end(keep, a.Tk, lane) : a.Tk;
     if (a.causal) end = max(0, min(end, start + min(i0 + 128, a.Tq)));
     const int p0 = start + i0 + wave * 32, p1 = p0 + 31, p = start + i;
     const int tiles = (end + KT - 1) / KT;
+    svbt_bf16x8 qf[NK][NS];
+    own.frags(kb, a.dk, has, qf);
 
     SvbtState<NDB> st;
 #pragma unroll
@@ -102,14 +110,7 @@ __global__ __launch_bounds__(256, DKP <= 64 ? 2 : 1) void svb_bucket_attn_fwd_ke
     st.l = 0.f;
     const float c = a.scale * SVBT_LOG2E;
 
-    Tile tk, tv;
     unsigned long long seen = ~0ull;                                    // of the tile in LDS: the keys that exist and are kept
-    float kept = 1.f;
-    auto fetch = [&](int t) {                                            // loads of tile t
-        tk.load(k, a.k_sc, t * KT, a.Tk, a.dk);
-        tv.load(v, a.v_sc, t * KT, a.Tk, a.dk);
-        if (keep) kept = keep[min(t * KT + lane, a.Tk - 1)];
-    };
     constexpr unsigned long long ALL = KT == 64 ? ~0ull : 0xffffffffull;
     auto bits = [&](int t) { return ALL & __ballot(t * KT + lane < end && kept != 0.f); };
     auto put = [&](int t) {                                              // registers -> LDS
@@ -121,7 +122,6 @@ __global__ __launch_bounds__(256, DKP <= 64 ? 2 : 1) void svb_bucket_attn_fwd_ke
         tv.template store<false, true>(nullptr, buf + NS * Tile::ROWS_BYTES);
     };
     if (tiles > 0) {
-        fetch(0);
         seen = bits(0);
         put(0);
     }
@@ -316,27 +316,47 @@ __global__ __launch_bounds__(256, DKP * SvbtParts<T>::NS > 192 || DKP == 128 ? 1
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l31 = lane & 31, kb = lane >> 5;
     const int split = blockIdx.x, hk = blockIdx.y, b = blockIdx.z;
     const int G = svb_uniform(a.H / a.Hkv), rows = G * a.Tq, nb = a.buckets.n_buckets, R = svb_bucket_reach(a.buckets);
-    float* s_tab = (float*)smem;                                        // [G][nb]
-    unsigned char* s_idx = (unsigned char*)(s_tab + G * nb);             // [2 R + 1]
-    for (int e = threadIdx.x; e < G * nb; e += 256)
-        s_tab[e] = svb_ld_table(a.table, (size_t)(e % nb) * a.H + hk * G + e / nb, a.table_dtype == SVB_DT_BF16) * SVBT_LOG2E;
-    for (int o = threadIdx.x; o <= 2 * R; o += 256) s_idx[o] = (unsigned char)svb_bucket_of(a.buckets, o - R);
-
     const bool has = l31 < rows;
     const int hl = has ? l31 / a.Tq : 0, i = has ? l31 - hl * a.Tq : 0, h = hk * G + hl;
     const T* q = (const T*)a.q + b * a.q_sb + (long long)h * a.dk * a.q_sc;
     const T* k = (const T*)a.k + b * a.k_sb + (long long)hk * a.dk * a.k_sc;
     const T* v = (const T*)a.v + b * a.v_sb + (long long)hk * a.dk * a.v_sc;
     const float* keep = a.keep ? a.keep + (size_t)b * a.Tk : nullptr;
-    svbt_bf16x8 qf[NK][NS];
-#pragma unroll
-    for (int s = 0; s < NK; ++s) svbt_own_frag<T, NS>(q, a.q_sc, i, s, kb, a.dk, has, qf[s]);
-
     const int start = svbt_start(a, b), p = start + i;
     const int end = a.causal ? max(0, min(a.Tk, start + a.Tq)) : a.Tk;
     // this wave's run of keys: whole tiles of 64, even over all waves of all splits
     const int tiles = (end + 63) / 64, runs = parts.splits * 4, run = split * 4 + wave;
     const int per = (tiles + runs - 1) / runs, t0 = min(run * per, tiles), t1 = min(t0 + per, tiles);
+    // A tile's K registers are free once its scores are made, its V registers at its end: the next tile's loads go there and then.
+    SvbFewKeys<T, NK> kt;
+    SvbFewValues<T> vt[4][NDB];
+    float kept = 1.f;
+    long long vrow[NDB];                                                // this lane's channel (one that exists) of V, from key 8 kb on
+#pragma unroll
+    for (int d = 0; d < NDB; ++d) vrow[d] = min(32 * d + l31, a.dk - 1) * a.v_sc + 8 * kb;
+    auto load_k = [&](int t) {                                          // (any t: the tile that ends with the rows is the last one)
+        const int j0 = min(64 * t, a.Tk - 64);
+        kt.load(SvbFewRows<T>(k, a.k_sc, j0 + 2 * l31, kb, a.dk));
+        if (keep) kept = keep[j0 + lane];
+    };
+    auto load_v = [&](int t) {
+        const int j0 = min(64 * t, a.Tk - 64);
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+#pragma unroll
+            for (int d = 0; d < NDB; ++d) vt[g][d].load(v + vrow[d] + (j0 + 16 * g));
+    };
+    SvbtOwn<T, NK> own;
+    own.load(q, a.q_sc, i, kb, a.dk);
+    if (NS == 1) { load_k(t0); load_v(t0); }                             // (fp32: two tiles' values spill, a tile loads its own)
+
+    float* s_tab = (float*)smem;                                        // [G][nb]
+    unsigned char* s_idx = (unsigned char*)(s_tab + G * nb);             // [2 R + 1]
+    for (int e = threadIdx.x; e < G * nb; e += 256)
+        s_tab[e] = svb_ld_table(a.table, (size_t)(e % nb) * a.H + hk * G + e / nb, a.table_dtype == SVB_DT_BF16) * SVBT_LOG2E;
+    for (int o = threadIdx.x; o <= 2 * R; o += 256) s_idx[o] = (unsigned char)svb_bucket_of(a.buckets, o - R);
+    svbt_bf16x8 qf[NK][NS];
+    own.frags(kb, a.dk, has, qf);
     const float c = a.scale * SVBT_LOG2E;
     SvbtState<NDB> st;
 #pragma unroll
@@ -347,24 +367,12 @@ __global__ __launch_bounds__(256, DKP * SvbtParts<T>::NS > 192 || DKP == 128 ? 1
     const float* tab = s_tab + hl * nb;
     const float past = tab[s_idx[0]], ahead = tab[s_idx[2 * R]];
 
-    long long vrow[NDB];                                                // this lane's channel (one that exists) of V, from key 8 kb on
-#pragma unroll
-    for (int d = 0; d < NDB; ++d) vrow[d] = min(32 * d + l31, a.dk - 1) * a.v_sc + 8 * kb;
     auto tile = [&](int t, auto full_c) {
         constexpr bool FULL = decltype(full_c)::value;                   // 64 keys, all of them seen by every row
         const int j0 = FULL ? 64 * t : min(64 * t, a.Tk - 64);
-        SvbFewKeys<T, NK> kt;
-        kt.load(SvbFewRows<T>(k, a.k_sc, j0 + 2 * l31, kb, a.dk));
+        if (NS != 1) { load_k(t); load_v(t); }
         unsigned long long seen = ~0ull;
-        if (!FULL) seen = __ballot(j0 + lane >= 64 * t && j0 + lane < end && (!keep || keep[j0 + lane] != 0.f));
-        SvbFewValues<T> vt[4][NDB];
-#pragma unroll
-        for (int g = 0; g < 4; ++g)
-#pragma unroll
-            for (int d = 0; d < NDB; ++d) {
-                vt[g][d].load(v + vrow[d] + (j0 + 16 * g));
-            }
-        if (seen == 0ull) return;                                       // (wave-uniform)
+        if (!FULL) seen = __ballot(j0 + lane >= 64 * t && j0 + lane < end && kept != 0.f);
         f32x16 s[2];
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
@@ -376,6 +384,7 @@ __global__ __launch_bounds__(256, DKP * SvbtParts<T>::NS > 192 || DKP == 128 ? 1
                 svbt_mma<NS, false>(s[u], f, qf[x]);
             }
         }
+        if (NS == 1 && t + 1 < t1) load_k(t + 1);
         const bool flat = j0 + 63 - start <= -R || j0 - (start + a.Tq - 1) >= R;
         const float fb = j0 + 63 - start <= -R ? past : ahead;
         // key of register r of tile u: 2 svbt_reg(r) + u + 8 kb
@@ -406,10 +415,13 @@ __global__ __launch_bounds__(256, DKP * SvbtParts<T>::NS > 192 || DKP == 128 ? 1
                 svbt_mma<NS, false>(st.o[d], f, pf);
             }
         }
+        if (NS == 1 && t + 1 < t1) load_v(t + 1);
     };
-    // whole tiles first, the others behind them: two loops, since one with both bodies keeps both bodies' registers alive
-    const int whole = keep ? t0 : max(t0, min(t1, (a.causal ? min(end, start + 1) : end) / 64));
-    for (int t = t0; t < whole; ++t) tile(t, std::true_type{});
+    // Whole tiles first, the others behind them: two loops, since one with both bodies keeps both bodies' registers alive.  bf16: without the
+    // masks 28 us instead of 33 (16 requests, 8192 cached keys); fp32 is bound by its six products, and one body is the shorter code.
+    const int whole = NS != 1 || keep ? t0 : max(t0, min(t1, (a.causal ? min(end, start + 1) : end) / 64));
+    if constexpr (NS == 1)
+        for (int t = t0; t < whole; ++t) tile(t, std::true_type{});
     for (int t = whole; t < t1; ++t) tile(t, std::false_type{});
     st.l += __shfl_xor(st.l, 32, 64);
 
@@ -535,9 +547,12 @@ static int few_launch(const SvbBucketAttn* a, float* ws, int splits, hipStream_t
     return SVB_OK;
 }
 
-extern "C" int svb_bucket_attn_fwd(const SvbBucketAttn* a, float* ws, void* stream) {
-    const int rc = svb_bucket_attn_check(a);
+extern "C" int svb_bucket_attn_fwd(const SvbBucketAttn* call, float* ws, void* stream) {
+    const int rc = svb_bucket_attn_check(call);
     if (rc != SVB_OK) return rc;
+    SvbBucketAttn filled = *call;
+    svb_bucket_fill(&filled.buckets);
+    const SvbBucketAttn* a = &filled;
     hipStream_t st = (hipStream_t)stream;
     const int splits = few_splits(a);
     if (splits > 1 && !ws) return SVB_ERR_ARG;

@@ -174,12 +174,14 @@ extern "C" int svb_bucket_bias_fwd(const void* table, void* bias, const SvbRelBu
     const int chunks = (Tq + SVB_BB_ROWS - 1) / SVB_BB_ROWS;
     if ((dtype != SVB_DT_F32 && dtype != SVB_DT_BF16) || (long)H * chunks > 0x7fffffffL) return SVB_ERR_UNSUPPORTED;
     const dim3 grid((unsigned)(H * chunks));
+    SvbRelBuckets bk = *buckets;
+    svb_bucket_fill(&bk);
     if (dtype == SVB_DT_BF16)
         hipLaunchKernelGGL((svb_bucket_bias_fwd_kernel<unsigned short>), grid, dim3(256), 0, (hipStream_t)stream, (const unsigned short*)table,
-                           (unsigned short*)bias, *buckets, H, Tq, Tk, q_start, chunks);
+                           (unsigned short*)bias, bk, H, Tq, Tk, q_start, chunks);
     else
         hipLaunchKernelGGL((svb_bucket_bias_fwd_kernel<float>), grid, dim3(256), 0, (hipStream_t)stream, (const float*)table, (float*)bias,
-                           *buckets, H, Tq, Tk, q_start, chunks);
+                           bk, H, Tq, Tk, q_start, chunks);
     SVB_CHECK_LAUNCH();
     return SVB_OK;
 }

@@ -29,9 +29,15 @@ __device__ __forceinline__ int svb_bucket_of(const SvbRelBuckets& b, int off) {
     int base = 0, m = off < 0 ? -off : 0;
     if (b.both && off > 0) { base = b.n_buckets / 2; m = off; }
     if (m < b.near) return base + m;
+    // all of the edges, unused ones never reached (svb_bucket_fill): a loop up to n_edge waits for a scalar load in each round
     int k = base + b.near;
-    for (int t = 0; t < b.n_edge; ++t) k += b.edge[t] <= m ? 1 : 0;
+#pragma unroll
+    for (int t = 0; t < SVB_REL_MAX_EDGES; ++t) k += b.edge[t] <= m ? 1 : 0;
     return k;
+}
+// host: the edges beyond n_edge, for svb_bucket_of
+static inline void svb_bucket_fill(SvbRelBuckets* b) {
+    for (int t = b->n_edge; t < SVB_REL_MAX_EDGES; ++t) b->edge[t] = 0x7fffffff;
 }
 
 // the offsets a <= o < b that bucket k holds (one run; empty where k is not used)
