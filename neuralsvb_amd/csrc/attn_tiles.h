@@ -212,12 +212,15 @@ struct SvbtTile {
     static constexpr int ROWP = 2 * DKP + 16, COLP = 2 * KT + 16;                       // pitches, bytes
     static constexpr int ROWS_BYTES = KT * ROWP, COLS_BYTES = DKP * COLP;              // one part's plane
     SvbtBlock<T> b[NB];
+    int tid;                           // this thread's first block
+    // second: of two tiles staged together, the one that begins where the first ends (small tiles leave threads without a block)
+    __device__ __forceinline__ explicit SvbtTile(bool second) : tid(second && 2 * BLOCKS <= NT ? (threadIdx.x + NT - BLOCKS) % NT : threadIdx.x) {}
 
     // positions j0 .. j0 + KT - 1 of rows of L elements at `base`, channel pitch sc (<= 2^25)
     __device__ __forceinline__ void load(const T* base, long long sc, int j0, int L, int dk) {
 #pragma unroll
         for (int i = 0; i < NB; ++i) {
-            const int id = threadIdx.x + i * NT, j = j0 + id % JB * 4;
+            const int id = tid + i * NT, j = j0 + id % JB * 4;
             if (BLOCKS % NT != 0 && id >= BLOCKS) continue;
             const int d = min(id / JB * 4, dk - 1), more = dk - 1 - d;
             long long off = (long long)d * sc + max(0, min(j, L - 4));
@@ -235,18 +238,18 @@ struct SvbtTile {
     __device__ __forceinline__ void settle(int j0, int L, unsigned long long seen) {
         if (!TINY && j0 + KT > L) {                                     // (uniform, as the next)
 #pragma unroll
-            for (int i = 0; i < NB; ++i) b[i].shift(max(0, j0 + (int)(threadIdx.x + i * NT) % JB * 4 - (L - 4)));
+            for (int i = 0; i < NB; ++i) b[i].shift(max(0, j0 + (tid + i * NT) % JB * 4 - (L - 4)));
         }
         if (seen != ~0ull) {
 #pragma unroll
-            for (int i = 0; i < NB; ++i) b[i].hide((unsigned)(seen >> ((threadIdx.x + i * NT) % JB * 4)) & 15u);
+            for (int i = 0; i < NB; ++i) b[i].hide((unsigned)(seen >> ((tid + i * NT) % JB * 4)) & 15u);
         }
     }
     template <bool ROWS, bool COLS>
     __device__ __forceinline__ void store(char* rows, char* cols) const {
 #pragma unroll
         for (int i = 0; i < NB; ++i) {
-            const int id = threadIdx.x + i * NT, d = id / JB * 4, j = id % JB * 4;
+            const int id = tid + i * NT, d = id / JB * 4, j = id % JB * 4;
             if (BLOCKS % NT == 0 || id < BLOCKS) {
                 unsigned o[NS][4][2];
                 b[i].parts(o);
@@ -320,4 +323,23 @@ __device__ __forceinline__ int svbt_keep_end(const float* keep, int n, int lane)
         if (last) return last;
     }
     return 0;
+}
+// (group, tile) of workgroup `id` of groups x tiles.  A group's workgroups read the same keys or queries, so they belong on one XCD
+// (workgroups go round the 8 in turn).  LONG_FIRST: tile 0 of every group is the longest, the last is short; a group's tiles one after the
+// other would leave the long ones of the last groups to the end (B2 H16 dk128 T2048 causal, dk and dv: 364 us that way).
+__device__ __forceinline__ void svbt_item(int id, int groups, int tiles, bool long_first, int& group, int& tile) {
+    if (long_first) {
+        if ((groups & 7) == 0) {                                         // the groups of this XCD, tile by tile
+            const int n = groups >> 3, r = id >> 3;
+            tile = svb_uniform(r / n);
+            group = (id & 7) * n + r - tile * n;
+        } else {
+            tile = svb_uniform(id / groups);
+            group = id - tile * groups;
+        }
+    } else {
+        const int item = svb_xcd_item(id, groups * tiles);
+        group = svb_uniform(item / tiles);
+        tile = item - group * tiles;
+    }
 }

@@ -68,15 +68,16 @@ __device__ __forceinline__ void svbt_diag_add(float* skew, float* diag, const f3
 
 // ---- dq, dtable, delta: 4 waves x 32 queries, keys staged ----------------------------------------------------------------------------
 template <typename T, int DKP, int KT, bool DOUBLE, bool TINY>
-__global__ __launch_bounds__(256, DKP <= 64 ? 2 : 1) void svb_bucket_attn_dq_kernel(SvbBucketAttn a, SvbBattnBwd g, int qtiles) {
+__global__ __launch_bounds__(256, SvbtParts<T>::NS == 1 || DKP <= 64 ? 2 : 1) void svb_bucket_attn_dq_kernel(SvbBucketAttn a, SvbBattnBwd g, int qtiles) {
     typedef SvbtTile<T, DKP, KT, 256, TINY> Tile;
     constexpr int NS = Tile::NS, NK = DKP / 16, NDB = DKP / 32, NSUB = KT / 32;
     constexpr int BUF = NS * (2 * Tile::ROWS_BYTES + Tile::COLS_BYTES);
     HIP_DYNAMIC_SHARED(char, smem)
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l31 = lane & 31, kb = lane >> 5;
-    const int item = svb_xcd_item(blockIdx.x, gridDim.x);
-    const int bh = svb_uniform(item / qtiles), b = svb_uniform(bh / a.H), h = bh - b * a.H, hk = svb_uniform(h / (a.H / a.Hkv));
-    const int qt = a.causal ? qtiles - 1 - (item - bh * qtiles) : item - bh * qtiles;
+    int bh, qt;
+    svbt_item(blockIdx.x, a.B * a.H, qtiles, a.causal, bh, qt);
+    if (a.causal) qt = qtiles - 1 - qt;
+    const int b = svb_uniform(bh / a.H), h = bh - b * a.H, hk = svb_uniform(h / (a.H / a.Hkv));
     const int i0 = qt * 128, i = i0 + wave * 32 + l31;
     const bool has = i < a.Tq;
     const int start = svbt_start(a, b), R = svb_bucket_reach(a.buckets), nb = a.buckets.n_buckets;
@@ -84,7 +85,7 @@ __global__ __launch_bounds__(256, DKP <= 64 ? 2 : 1) void svb_bucket_attn_dq_ker
     const T* k = (const T*)a.k + b * a.k_sb + (long long)hk * a.dk * a.k_sc;
     const T* v = (const T*)a.v + b * a.v_sb + (long long)hk * a.dk * a.v_sc;
     const float* keep = a.keep ? a.keep + (size_t)b * a.Tk : nullptr;
-    Tile tk, tv;
+    Tile tk(false), tv(true);
     float kept = 1.f;
     auto fetch = [&](int t) {
         tk.load(k, a.k_sc, t * KT, a.Tk, a.dk);
@@ -279,10 +280,11 @@ __global__ __launch_bounds__(256, DKP <= (SvbtParts<T>::NS == 1 ? 64 : 32) ? 2 :
     constexpr int TILE = NS * 2 * (Tile::ROWS_BYTES + Tile::COLS_BYTES), BUF = TILE + 2 * KT * 4;
     HIP_DYNAMIC_SHARED(char, smem)
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l31 = lane & 31, kb = lane >> 5;
-    const int item = svb_xcd_item(blockIdx.x, gridDim.x);
-    const int bkt = svb_uniform(item / g.splits), split = item - bkt * g.splits;
-    const int bk = svb_uniform(bkt / ktiles), b = svb_uniform(bk / a.Hkv), hk = bk - b * a.Hkv, G = svb_uniform(a.H / a.Hkv);
-    const int jt = (bkt - bk * ktiles) * 128, jw = jt + wave * 32, j = jw + l31;
+    int bk, ks;
+    svbt_item(blockIdx.x, a.B * a.Hkv, ktiles * g.splits, a.causal, bk, ks);
+    const int kt = svb_uniform(ks / g.splits), split = ks - kt * g.splits;
+    const int b = svb_uniform(bk / a.Hkv), hk = bk - b * a.Hkv, G = svb_uniform(a.H / a.Hkv);
+    const int jt = kt * 128, jw = jt + wave * 32, j = jw + l31;
     const bool has = j < a.Tk, kept = has && (!a.keep || a.keep[(size_t)b * a.Tk + j] != 0.f);
     const int start = svbt_start(a, b), R = svb_bucket_reach(a.buckets);
     float* s_bias = (float*)(smem + (DOUBLE ? 2 : 1) * BUF);
@@ -301,7 +303,7 @@ __global__ __launch_bounds__(256, DKP <= (SvbtParts<T>::NS == 1 ? 64 : 32) ? 2 :
     const int first = a.causal ? max(0, min(jt - start, a.Tq)) / KT : 0;
     const int tiles = max(0, (a.Tq + KT - 1) / KT - first);
     const float c = a.scale * SVBT_LOG2E;
-    Tile tq, td;
+    Tile tq(false), td(true);
     float stat = 0.f;                                                   // this thread's lse (threads < KT) or delta (KT .. 2 KT - 1)
     const int n0 = svb_uniform((int)((long long)G * tiles * split / g.splits)), n1 = svb_uniform((int)((long long)G * tiles * (split + 1) / g.splits));
     auto fetch = [&](int n) {
@@ -503,9 +505,9 @@ extern "C" int svb_bucket_attn_bwd(const SvbBucketAttn* call, const SvbBucketAtt
     // (double buffers where two workgroups of them fit a CU)
     if (a->dtype == SVB_DT_BF16) {
         typedef unsigned short T;
-        rc = a->Tk < 4 ? dq_launch<T, 128, 64, false, true>(a, w, st) : a->dk <= 32 ? dq_launch<T, 32, 64, true>(a, w, st)
-             : a->dk <= 64 ? dq_launch<T, 64, 64, true>(a, w, st) : a->dk <= 96 ? dq_launch<T, 96, 64, false>(a, w, st)
-             : dq_launch<T, 128, 64, false>(a, w, st);
+        rc = a->Tk < 4 ? dq_launch<T, 128, 32, false, true>(a, w, st) : a->dk <= 32 ? dq_launch<T, 32, 64, true>(a, w, st)
+             : a->dk <= 64 ? dq_launch<T, 64, 64, true>(a, w, st) : a->dk <= 96 ? dq_launch<T, 96, 32, false>(a, w, st)
+             : dq_launch<T, 128, 32, false>(a, w, st);
         if (rc == SVB_OK && w.dk)
             rc = a->Tq < 4 ? dkv_launch<T, 128, 64, false, true>(a, w, st) : a->dk <= 32 ? dkv_launch<T, 32, 64, true>(a, w, st)
                  : a->dk <= 64 ? dkv_launch<T, 64, 64, true>(a, w, st) : a->dk <= 96 ? dkv_launch<T, 96, 64, false>(a, w, st)

@@ -65,22 +65,23 @@ __device__ __forceinline__ void svbt_softmax(f32x16 (&s)[NSUB], SvbtState<NDB>& 
 // ---- query tiles: 4 waves x 32 queries, keys staged through LDS, the next tile's loads in flight during this one's products ------------
 // PP: parts of P
 template <typename T, int DKP, int KT, bool DOUBLE, int PP, bool TINY>
-__global__ __launch_bounds__(256, DKP <= 64 ? 2 : 1) void svb_bucket_attn_fwd_kernel(SvbBucketAttn a, int qtiles) {
+__global__ __launch_bounds__(256, SvbtParts<T>::NS == 3 && DKP == 128 ? 1 : 2) void svb_bucket_attn_fwd_kernel(SvbBucketAttn a, int qtiles) {
     typedef SvbtTile<T, DKP, KT, 256, TINY> Tile;
     constexpr int NS = Tile::NS, NK = DKP / 16, NDB = DKP / 32, NSUB = KT / 32;
     constexpr int BUF = NS * (Tile::ROWS_BYTES + Tile::COLS_BYTES);
     HIP_DYNAMIC_SHARED(char, smem)
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l31 = lane & 31, kb = lane >> 5;
-    const int item = svb_xcd_item(blockIdx.x, gridDim.x);
-    const int bh = svb_uniform(item / qtiles), b = svb_uniform(bh / a.H), h = bh - b * a.H, hk = svb_uniform(h / (a.H / a.Hkv));
-    const int qt = a.causal ? qtiles - 1 - (item - bh * qtiles) : item - bh * qtiles;      // (causal: the longest rows first)
+    int bh, qt;
+    svbt_item(blockIdx.x, a.B * a.H, qtiles, a.causal, bh, qt);
+    if (a.causal) qt = qtiles - 1 - qt;                                 // (the longest rows first)
+    const int b = svb_uniform(bh / a.H), h = bh - b * a.H, hk = svb_uniform(h / (a.H / a.Hkv));
     const int i0 = qt * 128, i = i0 + wave * 32 + l31;
     const bool has = i < a.Tq;
     const T* q = (const T*)a.q + b * a.q_sb + (long long)h * a.dk * a.q_sc;
     const T* k = (const T*)a.k + b * a.k_sb + (long long)hk * a.dk * a.k_sc;
     const T* v = (const T*)a.v + b * a.v_sb + (long long)hk * a.dk * a.v_sc;
     const float* keep = a.keep ? a.keep + (size_t)b * a.Tk : nullptr;
-    Tile tk, tv;
+    Tile tk(false), tv(true);
     float kept = 1.f;
     auto fetch = [&](int t) {                                            // loads of tile t
         tk.load(k, a.k_sc, t * KT, a.Tk, a.dk);
@@ -562,12 +563,13 @@ extern "C" int svb_bucket_attn_fwd(const SvbBucketAttn* call, float* ws, void* s
     if (splits && a->dtype == SVB_DT_F32) SVB_FEW_GO(float);
     if (splits) SVB_FEW_GO(unsigned short);
 #undef SVB_FEW_GO
-#define SVB_FWD_GO(T, KT, PP)                                                                                     \
+    // (double buffers where two workgroups of them fit a CU)
+#define SVB_FWD_GO(T, KT, PP, D96)                                                                                 \
     return a->Tk < 4 ? fwd_launch<T, 128, KT, true, PP, true>(a, st)                                                   \
          : a->dk <= 32 ? fwd_launch<T, 32, KT, true, PP>(a, st) : a->dk <= 64 ? fwd_launch<T, 64, KT, true, PP>(a, st) \
-         : a->dk <= 96 ? fwd_launch<T, 96, KT, true, PP>(a, st) : fwd_launch<T, 128, KT, true, PP>(a, st)
-    if (a->dtype == SVB_DT_F32) SVB_FWD_GO(float, 32, 3);
-    if (a->lse) SVB_FWD_GO(unsigned short, 64, 3);
-    SVB_FWD_GO(unsigned short, 64, 1);
+         : a->dk <= 96 ? fwd_launch<T, 96, KT, D96, PP>(a, st) : fwd_launch<T, 128, KT, true, PP>(a, st)
+    if (a->dtype == SVB_DT_F32) SVB_FWD_GO(float, 32, 3, false);
+    if (a->lse) SVB_FWD_GO(unsigned short, 64, 3, true);
+    SVB_FWD_GO(unsigned short, 64, 1, true);
 #undef SVB_FWD_GO
 }
