@@ -519,7 +519,7 @@ extern "C" int svb_bucket_attn_bwd(const SvbBucketAttn* call, const SvbBucketAtt
              : dq_launch<T, 128, 32, false>(a, w, st);
         if (rc == SVB_OK && w.dk)
             rc = a->Tq < 4 ? dkv_launch<T, 128, 32, false, true>(a, w, st) : a->dk <= 32 ? dkv_launch<T, 32, 32, true>(a, w, st)
-                 : a->dk <= 64 ? dkv_launch<T, 64, 32, false>(a, w, st) : a->dk <= 96 ? dkv_launch<T, 96, 32, false>(a, w, st)
+                 : a->dk <= 64 ? dkv_launch<T, 64, 64, false>(a, w, st) : a->dk <= 96 ? dkv_launch<T, 96, 32, false>(a, w, st)
                  : dkv_launch<T, 128, 32, false>(a, w, st);
     }
     if (rc != SVB_OK || !g->d_table) return rc;
