@@ -234,15 +234,18 @@ struct SvbtTile {
             }
         }
     }
-    // after the loads: blocks over the end into place, and positions whose bit is not set to zero (`seen` == ~0: all count)
-    __device__ __forceinline__ void settle(int j0, int L, unsigned long long seen) {
+    // after the loads: blocks over the end into place, and positions whose bit is not set to zero (`seen` == ~0: all count; seen2: from 64 on)
+    __device__ __forceinline__ void settle(int j0, int L, unsigned long long seen, unsigned long long seen2 = ~0ull) {
         if (!TINY && j0 + KT > L) {                                     // (uniform, as the next)
 #pragma unroll
             for (int i = 0; i < NB; ++i) b[i].shift(max(0, j0 + (tid + i * NT) % JB * 4 - (L - 4)));
         }
-        if (seen != ~0ull) {
+        if ((seen & seen2) != ~0ull) {
 #pragma unroll
-            for (int i = 0; i < NB; ++i) b[i].hide((unsigned)(seen >> ((tid + i * NT) % JB * 4)) & 15u);
+            for (int i = 0; i < NB; ++i) {
+                const int at = (tid + i * NT) % JB * 4;
+                b[i].hide((unsigned)((at < 64 ? seen : seen2) >> (at & 63)) & 15u);
+            }
         }
     }
     template <bool ROWS, bool COLS>

@@ -4,7 +4,7 @@
 // over the keys that query i sees, one pass over the keys with the running maximum m and sum l; nothing of size Tq x Tk exists.
 // Scores are computed transposed, S^T = K Q^T, one query per lane column: a query's maximum and sum are 16 registers and one exchange
 // with the other half of the wave, and S^T turns into the B operand of  O^T = V^T P^T  without moving (attn_tiles.h).
-// P is rounded to bf16 for bf16 tensors (relative 2^-9 per weight, averaged over the keys; l sums what was not rounded) and cut into
+// P is rounded to bf16 for bf16 tensors (relative 2^-8 per weight at most, averaged over the keys; l sums what was not rounded) and cut into
 // three parts for fp32 tensors.  A training forward of bf16 tensors takes P in three parts too: the backward gets delta_i = dout_i . out_i
 // from this output, and the sums of dS over a bucket cancel down to delta's error (B2 H16/4 dk128 T2048: the table's gradient is 5e-4
 // off with one part, 1e-6 with two, 2e-7 with three, as with 32-bit arithmetic throughout).
@@ -62,12 +62,12 @@ __device__ __forceinline__ void svbt_softmax(f32x16 (&s)[NSUB], SvbtState<NDB>& 
     st.l += sum;
 }
 
-// ---- query tiles: 4 waves x 32 queries, keys staged through LDS, the next tile's loads in flight during this one's products ------------
-// PP: parts of P
-template <typename T, int DKP, int KT, bool DOUBLE, int PP, bool TINY>
+// ---- query tiles: 4 waves, keys staged through LDS, the next tile's loads in flight during this one's products --------------------------
+// PP: parts of P.  KG: the waves are 4 / KG groups of 32 queries, each tile's keys are split over KG waves, which join at the end.
+template <typename T, int DKP, int KT, bool DOUBLE, int PP, int KG, bool TINY>
 __global__ __launch_bounds__(256, SvbtParts<T>::NS == 3 && DKP == 128 ? 1 : 2) void svb_bucket_attn_fwd_kernel(SvbBucketAttn a, int qtiles) {
     typedef SvbtTile<T, DKP, KT, 256, TINY> Tile;
-    constexpr int NS = Tile::NS, NK = DKP / 16, NDB = DKP / 32, NSUB = KT / 32;
+    constexpr int NS = Tile::NS, NK = DKP / 16, NDB = DKP / 32, NSUB = KT / 32 / KG, QW = 4 / KG;
     constexpr int BUF = NS * (Tile::ROWS_BYTES + Tile::COLS_BYTES);
     HIP_DYNAMIC_SHARED(char, smem)
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l31 = lane & 31, kb = lane >> 5;
@@ -75,18 +75,25 @@ __global__ __launch_bounds__(256, SvbtParts<T>::NS == 3 && DKP == 128 ? 1 : 2) v
     svbt_item(blockIdx.x, a.B * a.H, qtiles, a.causal, bh, qt);
     if (a.causal) qt = qtiles - 1 - qt;                                 // (the longest rows first)
     const int b = svb_uniform(bh / a.H), h = bh - b * a.H, hk = svb_uniform(h / (a.H / a.Hkv));
-    const int i0 = qt * 128, i = i0 + wave * 32 + l31;
+    const int qw = wave % QW, k0 = wave / QW * (NSUB * 32);             // this wave's queries, and its keys of a tile
+    const int i0 = qt * (32 * QW), i = i0 + qw * 32 + l31;
     const bool has = i < a.Tq;
     const T* q = (const T*)a.q + b * a.q_sb + (long long)h * a.dk * a.q_sc;
     const T* k = (const T*)a.k + b * a.k_sb + (long long)hk * a.dk * a.k_sc;
     const T* v = (const T*)a.v + b * a.v_sb + (long long)hk * a.dk * a.v_sc;
     const float* keep = a.keep ? a.keep + (size_t)b * a.Tk : nullptr;
     Tile tk(false), tv(true);
-    float kept = 1.f;
+    constexpr int NB64 = (KT + 63) / 64;
+    float kept[NB64];
+#pragma unroll
+    for (int w = 0; w < NB64; ++w) kept[w] = 1.f;
     auto fetch = [&](int t) {                                            // loads of tile t
         tk.load(k, a.k_sc, t * KT, a.Tk, a.dk);
         tv.load(v, a.v_sc, t * KT, a.Tk, a.dk);
-        if (keep) kept = keep[min(t * KT + lane, a.Tk - 1)];
+        if (keep) {
+#pragma unroll
+            for (int w = 0; w < NB64; ++w) kept[w] = keep[min(t * KT + 64 * w + lane, a.Tk - 1)];
+        }
     };
     fetch(0);
     SvbtOwn<T, NK> own;
@@ -98,8 +105,8 @@ __global__ __launch_bounds__(256, SvbtParts<T>::NS == 3 && DKP == 128 ? 1 : 2) v
 
     // keys that anyone here sees end at `end`; this wave's queries are at positions p0 .. p1
     int end = keep ? svbt_keep_end(keep, a.Tk, lane) : a.Tk;
-    if (a.causal) end = max(0, min(end, start + min(i0 + 128, a.Tq)));
-    const int p0 = start + i0 + wave * 32, p1 = p0 + 31, p = start + i;
+    if (a.causal) end = max(0, min(end, start + min(i0 + 32 * QW, a.Tq)));
+    const int p0 = start + i0 + qw * 32, p1 = p0 + 31, p = start + i;
     const int tiles = (end + KT - 1) / KT;
     svbt_bf16x8 qf[NK][NS];
     own.frags(kb, a.dk, has, qf);
@@ -111,26 +118,25 @@ __global__ __launch_bounds__(256, SvbtParts<T>::NS == 3 && DKP == 128 ? 1 : 2) v
     st.l = 0.f;
     const float c = a.scale * SVBT_LOG2E;
 
-    unsigned long long seen = ~0ull;                                    // of the tile in LDS: the keys that exist and are kept
-    constexpr unsigned long long ALL = KT == 64 ? ~0ull : 0xffffffffull;
-    auto bits = [&](int t) { return ALL & __ballot(t * KT + lane < end && kept != 0.f); };
+    unsigned long long seen[NB64];                                      // of the tile in LDS: the keys that exist and are kept
+    constexpr unsigned long long ALL = KT == 32 ? 0xffffffffull : ~0ull;
     auto put = [&](int t) {                                              // registers -> LDS
-        const unsigned long long m = seen == ALL ? ~0ull : seen;
-        tk.settle(t * KT, a.Tk, m);
-        tv.settle(t * KT, a.Tk, m);
+#pragma unroll
+        for (int w = 0; w < NB64; ++w) seen[w] = ALL & __ballot(t * KT + 64 * w + lane < end && kept[w] != 0.f);
+        const unsigned long long m = seen[0] == ALL ? ~0ull : seen[0];
+        tk.settle(t * KT, a.Tk, m, seen[NB64 - 1] | ~ALL);
+        tv.settle(t * KT, a.Tk, m, seen[NB64 - 1] | ~ALL);
         char* buf = smem + (DOUBLE ? (t & 1) * BUF : 0);
         tk.template store<true, false>(buf, nullptr);
         tv.template store<false, true>(nullptr, buf + NS * Tile::ROWS_BYTES);
     };
-    if (tiles > 0) {
-        seen = bits(0);
-        put(0);
-    }
+    if (tiles > 0) put(0);
     __syncthreads();
     const float past = s_bias[0], ahead = s_bias[2 * (R + SVBT_PAD)];
     for (int t = 0; t < tiles; ++t) {
-        const unsigned long long now = seen;
-        const int j0 = t * KT;
+        constexpr unsigned long long MINE = NSUB == 2 ? ~0ull : 0xffffffffull;
+        const unsigned long long now = (NB64 == 2 ? seen[wave / QW] : seen[0] >> k0) & MINE;
+        const int j0 = t * KT + k0;
         if (t + 1 < tiles) fetch(t + 1);
         const char* rows = smem + (DOUBLE ? (t & 1) * BUF : 0);
         const char* cols = rows + NS * Tile::ROWS_BYTES;
@@ -142,12 +148,12 @@ __global__ __launch_bounds__(256, SvbtParts<T>::NS == 3 && DKP == 128 ? 1 : 2) v
 #pragma unroll
                 for (int x = 0; x < NK; ++x) {
                     svbt_bf16x8 f[NS];
-                    Tile::row_frag(rows, u, x, l31, kb, f);
+                    Tile::row_frag(rows, k0 / 32 + u, x, l31, kb, f);
                     svbt_mma<NS, false>(s[u], f, qf[x]);
                 }
             }
-            const bool edge = now != ALL || (a.causal && j0 + KT - 1 > p0);
-            const bool behind = j0 + KT - 1 - p0 <= -R, before = j0 - p1 >= R;
+            const bool edge = now != MINE || (a.causal && j0 + 32 * NSUB - 1 > p0);
+            const bool behind = j0 + 32 * NSUB - 1 - p0 <= -R, before = j0 - p1 >= R;
             const float flat = behind ? past : ahead;
 #pragma unroll
             for (int u = 0; u < NSUB; ++u) {
@@ -175,7 +181,7 @@ __global__ __launch_bounds__(256, SvbtParts<T>::NS == 3 && DKP == 128 ? 1 : 2) v
 #pragma unroll
                     for (int d = 0; d < NDB; ++d) {
                         svbt_bf16x8 f[NS];
-                        Tile::col_frag(cols, d, u, x, l31, kb, f);
+                        Tile::col_frag(cols, d, k0 / 32 + u, x, l31, kb, f);
                         if constexpr (PP == NS) svbt_mma<NS, false>(st.o[d], f, pf);
                         else {
 #pragma unroll
@@ -186,12 +192,34 @@ __global__ __launch_bounds__(256, SvbtParts<T>::NS == 3 && DKP == 128 ? 1 : 2) v
         }
         if (t + 1 < tiles) {
             if (!DOUBLE) __syncthreads();                               // (this tile's fragments are read)
-            seen = bits(t + 1);
             put(t + 1);
         }
         __syncthreads();
     }
 
+    if constexpr (KG == 2) {                                            // (the last tile is read)
+        constexpr int N = 16 * NDB + 2;                                 // a lane's state, lanes innermost
+        static_assert(QW * N * 256 <= BUF, "the tile's LDS holds the states");
+        float* s_st = (float*)smem + qw * N * 64 + lane;
+        if (wave >= QW) {
+#pragma unroll
+            for (int d = 0; d < NDB; ++d)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) s_st[(16 * d + r) * 64] = st.o[d][r];
+            s_st[(N - 2) * 64] = st.m;
+            s_st[(N - 1) * 64] = st.l;
+        }
+        __syncthreads();
+        if (wave >= QW) return;
+        const float m1 = s_st[(N - 2) * 64], m = fmaxf(st.m, m1), m_use = m == -SVBT_INF ? 0.f : m;
+        const float f0 = __builtin_amdgcn_exp2f(st.m - m_use), f1 = __builtin_amdgcn_exp2f(m1 - m_use);
+        st.m = m;
+        st.l = st.l * f0 + s_st[(N - 1) * 64] * f1;
+#pragma unroll
+        for (int d = 0; d < NDB; ++d)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) st.o[d][r] = st.o[d][r] * f0 + s_st[(16 * d + r) * 64] * f1;
+    }
     const float l = st.l + __shfl_xor(st.l, 32, 64);
     const float inv = l > 0.f ? 1.f / l : 0.f;                          // (no key: zeros)
     if (!has) return;
@@ -500,13 +528,14 @@ int svb_bucket_attn_check(const SvbBucketAttn* a) {
     return SVB_OK;
 }
 
-template <typename T, int DKP, int KT, bool DOUBLE, int PP, bool TINY = false>
+template <typename T, int DKP, int KT, bool DOUBLE, int PP, int KG, bool TINY = false>
 static int fwd_launch(const SvbBucketAttn* a, hipStream_t st) {
     typedef SvbtTile<T, DKP, KT, 256, TINY> Tile;
     const int lds = (DOUBLE ? 2 : 1) * Tile::NS * (Tile::ROWS_BYTES + Tile::COLS_BYTES) + svbt_span(a->buckets) * 4;
-    auto* kern = svb_bucket_attn_fwd_kernel<T, DKP, KT, DOUBLE, PP, TINY>;
+    auto* kern = svb_bucket_attn_fwd_kernel<T, DKP, KT, DOUBLE, PP, KG, TINY>;
     if (lds > 65536 && hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024) != hipSuccess) return SVB_ERR_LAUNCH;
-    const int qtiles = (a->Tq + 127) / 128;
+    constexpr int ROWS = 128 / KG;
+    const int qtiles = (a->Tq + ROWS - 1) / ROWS;
     hipLaunchKernelGGL(kern, dim3((unsigned)(a->B * a->H * qtiles)), dim3(256), lds, st, *a, qtiles);
     SVB_CHECK_LAUNCH();
     return SVB_OK;
@@ -564,12 +593,19 @@ extern "C" int svb_bucket_attn_fwd(const SvbBucketAttn* call, float* ws, void* s
     if (splits) SVB_FEW_GO(unsigned short);
 #undef SVB_FEW_GO
     // (double buffers where two workgroups of them fit a CU)
-#define SVB_FWD_GO(T, KT, PP, D96)                                                                                 \
-    return a->Tk < 4 ? fwd_launch<T, 128, KT, true, PP, true>(a, st)                                                   \
-         : a->dk <= 32 ? fwd_launch<T, 32, KT, true, PP>(a, st) : a->dk <= 64 ? fwd_launch<T, 64, KT, true, PP>(a, st) \
-         : a->dk <= 96 ? fwd_launch<T, 96, KT, D96, PP>(a, st) : fwd_launch<T, 128, KT, true, PP>(a, st)
-    if (a->dtype == SVB_DT_F32) SVB_FWD_GO(float, 32, 3, false);
-    if (a->lse) SVB_FWD_GO(unsigned short, 64, 3, true);
-    SVB_FWD_GO(unsigned short, 64, 1, true);
+#define SVB_FWD_GO(T, K64, KT, PP, D96, KG)                                                                                \
+    return a->Tk < 4 ? fwd_launch<T, 128, KT, true, PP, 1, true>(a, st)                                                        \
+         : a->dk <= 32 ? fwd_launch<T, 32, K64, true, PP, KG>(a, st) : a->dk <= 64 ? fwd_launch<T, 64, K64, true, PP, KG>(a, st) \
+         : a->dk <= 96 ? fwd_launch<T, 96, KT, D96, PP, KG>(a, st) : fwd_launch<T, 128, KT, true, PP, KG>(a, st)
+    if (a->dtype == SVB_DT_F32) SVB_FWD_GO(float, 32, 32, 3, false, 1);
+    // At most one workgroup of 128 queries per CU and several tiles of keys: workgroups of 64 queries, twice as many, the keys of a tile over
+    // two waves, tiles of 128 keys up to dk 64.  B2 H8 dk64 T2000 causal (256 workgroups): 52 -> 41 us, training 72 -> 48; B4 H8 dk96 T1000
+    // causal: 38 -> 34; B24 H4 dk48 T211, where a join and a bigger tile save nothing: 14.5 -> 16.5.  Between one and two workgroups per CU
+    // (B7 H8 dk64 T1100 causal) the forward takes 39 us this way instead of 36.  fp32 tensors have six products per tile to wait behind.
+    const bool thin = a->Tk > 256 && (long)a->B * a->H * ((a->Tq + 127) / 128) <= 256;
+    if (a->lse && thin) SVB_FWD_GO(unsigned short, 128, 64, 3, true, 2);
+    if (a->lse) SVB_FWD_GO(unsigned short, 64, 64, 3, true, 1);
+    if (thin) SVB_FWD_GO(unsigned short, 128, 64, 1, true, 2);
+    SVB_FWD_GO(unsigned short, 64, 64, 1, true, 1);
 #undef SVB_FWD_GO
 }
