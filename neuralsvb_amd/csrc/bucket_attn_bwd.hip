@@ -10,7 +10,7 @@
 // their registers are the next product's operand (attn_tiles.h), so dS never moves between lanes.
 //
 // delta needs what rounding the output to bf16 destroys -- the sums over a bucket cancel, and the table's gradient is fp32 --, so the
-// forward keeps the output in fp32 for bf16 tensors.  P and dS are rounded to bf16 as operands for bf16 tensors (relative 2^-9 each,
+// forward keeps the output in fp32 for bf16 tensors.  P and dS are rounded to bf16 as operands for bf16 tensors (relative 2^-8 each at most,
 // averaged over the sum), and cut into three parts for fp32 tensors; dtable sums dS in fp32 before any rounding.
 // A row whose weight is all on one key (P == 1) has dS = 0: dP - delta is then rounding noise alone.
 //
@@ -285,8 +285,9 @@ __global__ __launch_bounds__(256, DKP <= (SvbtParts<T>::NS == 1 ? 64 : 32) ? 2 :
     const int kt = svb_uniform(ks / g.splits), split = ks - kt * g.splits;
     const int b = svb_uniform(bk / a.Hkv), hk = bk - b * a.Hkv, G = svb_uniform(a.H / a.Hkv);
     const int jt = kt * 128, jw = jt + wave * 32, j = jw + l31;
-    const bool has = j < a.Tk, kept = has && (!a.keep || a.keep[(size_t)b * a.Tk + j] != 0.f);
     const int start = svbt_start(a, b), R = svb_bucket_reach(a.buckets);
+    const bool has = j < a.Tk;                                          // kept: some query sees the key (rows of a tile beyond the last query do not count)
+    const bool kept = has && (!a.keep || a.keep[(size_t)b * a.Tk + j] != 0.f) && !(a.causal && j >= start + a.Tq);
     float* s_bias = (float*)(smem + (DOUBLE ? 2 : 1) * BUF);
 
     const T* k = (const T*)a.k + b * a.k_sb + (long long)hk * a.dk * a.k_sc;
@@ -304,7 +305,7 @@ __global__ __launch_bounds__(256, DKP <= (SvbtParts<T>::NS == 1 ? 64 : 32) ? 2 :
     const int tiles = max(0, (a.Tq + KT - 1) / KT - first);
     const float c = a.scale * SVBT_LOG2E;
     Tile tq(false), td(true);
-    float stat = 0.f;                                                   // this thread's lse (threads < KT) or delta (KT .. 2 KT - 1)
+    float stat = 0.f, row_lse = 0.f;                                    // this thread's lse (threads < KT) or delta (KT .. 2 KT - 1); lane's lse
     const int n0 = svb_uniform((int)((long long)G * tiles * split / g.splits)), n1 = svb_uniform((int)((long long)G * tiles * (split + 1) / g.splits));
     auto fetch = [&](int n) {
         const int hh = hk * G + svb_uniform(n / tiles), i0 = (first + n % tiles) * KT;
@@ -316,11 +317,15 @@ __global__ __launch_bounds__(256, DKP <= (SvbtParts<T>::NS == 1 ? 64 : 32) ? 2 :
             const float none = threadIdx.x < KT ? SVBT_INF : 0.f;       // (a query that does not exist has P = 0)
             stat = i < a.Tq ? (threadIdx.x < KT ? a.lse : g.delta)[hd * a.Tq + i] : none;
         }
+        row_lse = a.lse[hd * a.Tq + min(i0 + lane, a.Tq - 1)];
     };
     auto put = [&](int n) {
         const int i0 = (first + n % tiles) * KT;
-        tq.settle(i0, a.Tq, ~0ull);
-        td.settle(i0, a.Tq, ~0ull);
+        // a query that sees no key has no part in dk and dv, whatever q and dout hold there
+        constexpr unsigned long long OTHERS = KT == 64 ? 0ull : ~0xffffffffull;
+        const unsigned long long seen = OTHERS | __ballot(row_lse != SVBT_INF);
+        tq.settle(i0, a.Tq, seen);
+        td.settle(i0, a.Tq, seen);
         char* buf = smem + (DOUBLE ? (n & 1) * BUF : 0);
         tq.template store<true, true>(buf, buf + 2 * NS * Tile::ROWS_BYTES);
         td.template store<true, true>(buf + NS * Tile::ROWS_BYTES, buf + NS * (2 * Tile::ROWS_BYTES + Tile::COLS_BYTES));
@@ -439,7 +444,7 @@ __global__ __launch_bounds__(256) void svb_bucket_attn_kv_sum_kernel(SvbBattnBwd
 
 // ---- host ------------------------------------------------------------------------------------------------------------------------
 // Splits of a key tile's steps: workgroups for two per CU (B2 H16/4 dk128 T2048 causal has 128 key tiles: 859 us with one split), of at
-// least four steps each.
+// least four steps each.  (With splits the same case took 191 us and 15 us for the sums.)
 static int kv_splits(const SvbBucketAttn* a) {
     const long tiles = (long)a->B * a->Hkv * ((a->Tk + 127) / 128), steps = (long)(a->H / a->Hkv) * ((a->Tq + 63) / 64);
     const long want = (512 + tiles - 1) / tiles, most = steps / 4 < 8 ? steps / 4 : 8;

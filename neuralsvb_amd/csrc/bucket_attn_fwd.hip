@@ -524,7 +524,9 @@ int svb_bucket_attn_check(const SvbBucketAttn* a) {
     // (channel pitches: a lane's offset over 16 channels stays in 32 bits)
     if (a->q_sc < 0 || a->q_sc > (1 << 25) || a->k_sc < 0 || a->k_sc > (1 << 25) || a->v_sc < 0 || a->v_sc > (1 << 25)) return SVB_ERR_UNSUPPORTED;
     if (a->dk > 128 || a->Tq > (1 << 25) || a->Tk > (1 << 25) || a->q_start < -(1 << 28) || a->q_start > (1 << 28)) return SVB_ERR_UNSUPPORTED;
-    if ((long)a->B * a->H * ((a->Tq + 31) / 32) > 0x7fffffffL || (long)a->B * a->Hkv * ((a->Tk + 31) / 32) > 0x7fffffffL) return SVB_ERR_UNSUPPORTED;
+    // (a launch has less than 2^32 threads; dk and dv take up to 8 workgroups per 128 keys)
+    if (a->B > (1 << 24) || a->H > (1 << 24) || (long)a->B * a->H * ((a->Tq + 63) / 64) >= (1 << 24) || (long)a->B * a->Hkv * ((a->Tk + 127) / 128) >= (1 << 24))
+        return SVB_ERR_UNSUPPORTED;
     return SVB_OK;
 }
 

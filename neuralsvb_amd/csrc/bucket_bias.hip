@@ -76,13 +76,14 @@ __global__ __launch_bounds__(256) void svb_bucket_bias_fwd_kernel(const T* table
     }
 }
 
-// grid: (offset tiles, row chunks, H).  Offsets are counted without `start` here (column = row + offset); those that a chunk's rows
+// grid: (row chunks * offset tiles, H).  Offsets are counted without `start` here (column = row + offset); those that a chunk's rows
 // meet run from -(last row) on: tile0 .. tile0 + SVB_BB_OFFS - 1.  part [H][row chunks * offset tiles][n_buckets].
 template <typename T>
-__global__ __launch_bounds__(256) void svb_bucket_bias_bwd_kernel(const T* dbias, float* part, SvbRelBuckets bk, int Tq, int Tk, int start) {
+__global__ __launch_bounds__(256) void svb_bucket_bias_bwd_kernel(const T* dbias, float* part, SvbRelBuckets bk, int Tq, int Tk, int start,
+                                                                  int otiles) {
     __shared__ float sums[SVB_BB_OFFS];
-    const int h = blockIdx.z, i0 = blockIdx.y * SVB_BB_BROWS, i1 = min(i0 + SVB_BB_BROWS, Tq);
-    const int tile0 = -(i0 + SVB_BB_BROWS - 1) + (int)blockIdx.x * SVB_BB_OFFS;
+    const int h = blockIdx.y, chunk = svb_uniform(blockIdx.x / otiles), i0 = chunk * SVB_BB_BROWS, i1 = min(i0 + SVB_BB_BROWS, Tq);
+    const int tile0 = -(i0 + SVB_BB_BROWS - 1) + ((int)blockIdx.x - chunk * otiles) * SVB_BB_OFFS;
     const int o = tile0 + (int)threadIdx.x * 4;
     float s[4] = {0.f, 0.f, 0.f, 0.f};
     const T* base = dbias + (size_t)h * Tq * Tk;
@@ -120,7 +121,7 @@ __global__ __launch_bounds__(256) void svb_bucket_bias_bwd_kernel(const T* dbias
     __syncthreads();
     // a bucket's offsets are one run: find its ends in this tile, one wave per bucket in turn
     const int lane = threadIdx.x & 63;
-    float* row = part + ((size_t)h * gridDim.y * gridDim.x + (size_t)blockIdx.y * gridDim.x + blockIdx.x) * bk.n_buckets;
+    float* row = part + ((size_t)h * gridDim.x + blockIdx.x) * bk.n_buckets;
     for (int k = threadIdx.x >> 6; k < bk.n_buckets; k += 4) {
         int a, b;
         svb_bucket_range(bk, k, a, b);
@@ -165,14 +166,14 @@ int svb_bucket_table_reduce(const float* part, void* dtable, int rows, int nb, i
 
 // offsets j - i and start + i stay far inside 32 bits
 static bool svbb_sizes(int H, int Tq, int Tk, int start) {
-    return H > 0 && Tq > 0 && Tk > 0 && Tq < (1 << 28) && Tk < (1 << 28) && start > -(1 << 28) && start < (1 << 28);
+    return H > 0 && Tq > 0 && Tk > 0 && Tq <= (1 << 27) && Tk <= (1 << 27) && start >= -(1 << 28) && start <= (1 << 28);
 }
 
 extern "C" int svb_bucket_bias_fwd(const void* table, void* bias, const SvbRelBuckets* buckets, int H, int Tq, int Tk, int q_start, int dtype,
                                    void* stream) {
     if (!table || !bias || !svb_bucket_valid(buckets) || !svbb_sizes(H, Tq, Tk, q_start)) return SVB_ERR_ARG;
     const int chunks = (Tq + SVB_BB_ROWS - 1) / SVB_BB_ROWS;
-    if ((dtype != SVB_DT_F32 && dtype != SVB_DT_BF16) || (long)H * chunks > 0x7fffffffL) return SVB_ERR_UNSUPPORTED;
+    if ((dtype != SVB_DT_F32 && dtype != SVB_DT_BF16) || (long)H * chunks >= (1 << 24)) return SVB_ERR_UNSUPPORTED;
     const dim3 grid((unsigned)(H * chunks));
     SvbRelBuckets bk = *buckets;
     svb_bucket_fill(&bk);
@@ -203,14 +204,14 @@ extern "C" int svb_bucket_bias_bwd(const void* dbias, void* dtable, const SvbRel
     if (!dbias || !dtable || !ws || !svb_bucket_valid(buckets) || !svbb_sizes(H, Tq, Tk, q_start)) return SVB_ERR_ARG;
     long x, y;
     svbb_bwd_grid(Tq, Tk, &x, &y);
-    if ((dtype != SVB_DT_F32 && dtype != SVB_DT_BF16) || y > 65535 || H > 65535 || x * y > 0x7fffffffL) return SVB_ERR_UNSUPPORTED;
-    const dim3 grid((unsigned)x, (unsigned)y, (unsigned)H);
+    if ((dtype != SVB_DT_F32 && dtype != SVB_DT_BF16) || H > 65535 || H * x * y >= (1 << 24)) return SVB_ERR_UNSUPPORTED;
+    const dim3 grid((unsigned)(x * y), (unsigned)H);
     if (dtype == SVB_DT_BF16)
         hipLaunchKernelGGL((svb_bucket_bias_bwd_kernel<unsigned short>), grid, dim3(256), 0, (hipStream_t)stream, (const unsigned short*)dbias, ws,
-                           *buckets, Tq, Tk, q_start);
+                           *buckets, Tq, Tk, q_start, (int)x);
     else
         hipLaunchKernelGGL((svb_bucket_bias_bwd_kernel<float>), grid, dim3(256), 0, (hipStream_t)stream, (const float*)dbias, ws, *buckets, Tq, Tk,
-                           q_start);
+                           q_start, (int)x);
     SVB_CHECK_LAUNCH();
     return svb_bucket_table_reduce(ws, dtable, (int)(x * y), buckets->n_buckets, H, dtype, (hipStream_t)stream);
 }

@@ -13,6 +13,7 @@ import functools
 import weakref
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import _lib as L_
 from . import kernels as K
@@ -883,6 +884,7 @@ class _LayerNormNCTFn(torch.autograd.Function):
         return y
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dy):
         x, gamma, stats = ctx.saved_tensors
         return K.ln_nct_bwd(x, gamma, _c(dy), stats, *ctx.needs_input_grad[:3], ctx.affine_dtype) + (None,)
@@ -896,7 +898,10 @@ def layer_norm_nct(x, gamma, beta, eps=1e-5):
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, gamma, beta)):
         return _LayerNormNCTFn.apply(x, gamma, beta, float(eps))
     if x.dtype == torch.float32 and x.numel():
-        return K.layernorm_nct_fwd(x.contiguous(), gamma, beta, eps)
+        for p in (gamma, beta):
+            if p is not None and p.numel() != x.shape[1]:
+                raise ValueError(f"gamma, beta: [{x.shape[1]}], got {tuple(p.shape)}")
+        return K.layernorm_nct_fwd(x.contiguous(), _c(gamma), _c(beta), eps)
     return K.ln_nct_fwd(_c(x), _c(gamma), _c(beta), eps)
 
 
@@ -941,6 +946,7 @@ class _BucketBiasFn(torch.autograd.Function):
         return K.bucket_bias_fwd(_c(table), buckets, tq, tk, q_start)
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dbias):
         buckets, q_start = ctx.cfg
         return K.bucket_bias_bwd(_c(dbias), buckets, q_start), None, None, None, None
@@ -967,6 +973,7 @@ class _BucketAttnFn(torch.autograd.Function):
         return out
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dout):
         q, k, v, table, keep, starts, out, lse, o32 = ctx.saved_tensors
         nq, nk, nv, nt = ctx.needs_input_grad[:4]

@@ -1060,6 +1060,8 @@ def ln_nct_fwd(x, gamma, beta, eps=1e-5, save_stats=False):
     """LayerNorm over dim 1 of [B, C, T], fp32 or bf16 -> y, and with save_stats the statistics [2, B, T] (mean, 1 / deviation).
     gamma, beta [C] or None, both of x's dtype or both float32."""
     B, c, t = x.shape
+    if max(B, c, t) >= 1 << 31:
+        raise ValueError(f"ln_nct_fwd: {tuple(x.shape)}")
     adt = None
     for p in (gamma, beta):
         if p is not None:
@@ -1103,6 +1105,11 @@ def ln_nct_bwd(x, gamma, dy, stats, want_dx=True, want_dgamma=True, want_dbeta=T
     return dx, dg, db
 
 
+def _far_start(q_start):
+    """q_start in the C ABI's 32 bits: beyond any key it makes no difference how far."""
+    return max(-(1 << 28), min(1 << 28, int(q_start)))
+
+
 def _table_shape(table, buckets, n_head, what):
     if table.dim() != 2 or table.shape[0] != buckets.n_buckets or (n_head is not None and table.shape[1] != n_head):
         raise ValueError(f"{what}: table must be [{buckets.n_buckets}, {'heads' if n_head is None else n_head}], got {tuple(table.shape)}")
@@ -1111,8 +1118,11 @@ def _table_shape(table, buckets, n_head, what):
 def bucket_bias_fwd(table, buckets, tq, tk, q_start):
     """table [n_buckets, H] -> bias [H, tq, tk]: table[bucket(j - (q_start + i))].  buckets: an _lib.SvbRelBuckets."""
     _table_shape(table, buckets, None, "bucket_bias")
+    if max(tq, tk) > 1 << 27:
+        raise ValueError(f"bucket_bias: lengths {tq}, {tk} beyond {1 << 27}")
     dt = _dt(table, "bucket_bias")
     lib, st = _prep(table)
+    q_start = _far_start(q_start)
     h = table.shape[1]
     out = table.new_empty((h, tq, tk))
     if out.numel():
@@ -1125,6 +1135,7 @@ def bucket_bias_bwd(dbias, buckets, q_start):
     """dbias [H, tq, tk] -> dtable [n_buckets, H]."""
     dt = _dt(dbias, "bucket_bias")
     lib, st = _prep(dbias)
+    q_start = _far_start(q_start)
     h, tq, tk = dbias.shape
     dtable = dbias.new_empty((buckets.n_buckets, h))
     if not dbias.numel():
@@ -1144,6 +1155,8 @@ def _bucket_attn_desc(q, k, v, table, buckets, n_head, keep, q_start, causal, sc
     B, D, tq = q.shape
     _, Dk, tk = k.shape
     dk = D // n_head
+    if max(B, tq, tk) > 1 << 25:
+        raise ValueError(f"bucket_attention: batch {B}, lengths {tq}, {tk} beyond {1 << 25}")
     if not 1 <= dk <= 128 or not Dk or Dk % dk or n_head % (Dk // dk):
         raise ValueError(f"bucket_attention: {Dk} key channels are no divisor of {n_head} heads of {dk} channels (at most 128)")
     if q.dtype is not k.dtype or q.dtype is not v.dtype:
@@ -1167,8 +1180,7 @@ def _bucket_attn_desc(q, k, v, table, buckets, n_head, keep, q_start, causal, sc
             raise ValueError(f"bucket_attention: q_start must be an int or int32 [{B}]")
         d.q_start_b = starts.data_ptr()
     else:
-        # (beyond any key the start makes no difference any more; its distance fits the descriptor's 32 bits)
-        d.q_start = max(-(1 << 28), min(1 << 28, int(q_start)))
+        d.q_start = _far_start(q_start)
     lib, st = _prep(table, keep, starts)
     idx = q.get_device()
     if table.get_device() != idx or k.get_device() != idx or v.get_device() != idx:

@@ -440,3 +440,287 @@ def test_bias_tensor_is_the_bias_inside(dev):
     v = torch.eye(40)[:32].reshape(1, 32, 40).to(dev)
     out = SF.bucket_attention(torch.zeros(1, 32, 6, device=dev), torch.zeros(1, 32, 40, device=dev), v, table, bk, 1)
     near(out[0], torch.softmax(bias.double().cpu(), 1)[:, :32].t(), 128 * U32, "weights")
+
+
+# ---- forms, masks and limits ---------------------------------------------------------------------------------------------
+# few query rows over a cache that several workgroups share: heads in one wave, widths of every padded form, one and several queries
+@_dt
+@pytest.mark.parametrize("shape", [(3, 4, 2, 20, 1, 700), (1, 6, 1, 97, 2, 300), (1, 2, 2, 64, 16, 300), (1, 8, 1, 33, 4, 65)])
+def test_attention_cached_tokens(dev, dt, shape):
+    """One start per request; behind it the cache holds anything; some cached keys hidden."""
+    B, H, Hkv, dk, tq, tk = shape
+    *t, do = case(sum(shape), dt, *shape)
+    starts = torch.tensor([tk - tq, 66, 0][:B], dtype=torch.int32)
+    for x in (t[1], t[2]):
+        for b in range(B):
+            x[b, :, int(starts[b]) + tq:] = float("nan")
+    keep = torch.ones(B, tk)
+    keep[:, 5:60:7] = 0
+    keep[0, 200:290] = 0
+    for mask in (None, keep):
+        compare(dev, dt, t, do, SF.RelativeBuckets(16, 40, False), H, keep=mask, causal=True, q_start=starts, what=f"masked {mask is not None}")
+    *t, do = case(sum(shape) + 1, dt, *shape)
+    compare(dev, dt, t, do, SF.RelativeBuckets(16, 40, True), H, what="all keys")
+
+
+# keys of a tile over two waves (bf16), steps of a key tile over workgroups (8 heads to one), rows of less than 4, lengths behind whole tiles
+@_dt
+@pytest.mark.parametrize("shape", [(1, 1, 1, 33, 70, 300), (1, 2, 1, 100, 65, 270), (1, 1, 1, 128, 40, 385), (1, 8, 1, 16, 130, 40), (1, 2, 1, 100, 2, 3),
+                                   (2, 3, 1, 72, 64, 259)])
+def test_attention_split_work(dev, dt, shape):
+    B, H, Hkv, dk, tq, tk = shape
+    *t, do = case(sum(shape), dt, *shape)
+    keep = torch.ones(B, tk)
+    keep[0, 60:200] = 0
+    keep[0, tk - 1] = 0
+    compare(dev, dt, t, do, SF.RelativeBuckets(16, 40, True), H, keep=keep, what="masked")
+    compare(dev, dt, t, do, SF.RelativeBuckets(16, 40, False), H, causal=True, what="causal")
+
+
+@_dt
+def test_attention_widest_tables(dev, dt):
+    """The furthest border with the widest heads: the most LDS that a call takes."""
+    *t, do = case(31, dt, 1, 2, 1, 128, 50, 50, n=64)
+    compare(dev, dt, t, do, SF.RelativeBuckets(64, 1024, True), 2, what="64 buckets to 1024")
+    compare(dev, dt, t, do, SF.RelativeBuckets(64, 1024, False), 2, causal=True, q_start=600, what="past only")
+
+
+@_dt
+def test_attention_queries_that_see_nothing(dev, dt):
+    """Whatever q and dout hold in rows without a key, no gradient shows it."""
+    bk = SF.RelativeBuckets(16, 24, True)
+    *t, do = case(32, dt, 2, 2, 1, 24, 45, 70)
+    keep = torch.ones(2, 70)
+    keep[1] = 0
+    t[0][0, :, :9] = float("nan")                                         # (q_start = -9, causal: queries 0 .. 8 see nothing)
+    t[0][1] = float("inf")
+    do[0, :, 3] = float("nan")
+    do[1, 0] = float("inf")
+    ls = [x.to(dev).requires_grad_() for x in t]
+    out = SF.bucket_attention(*ls, bk, 2, keep=keep.to(dev), causal=True, q_start=-9)
+    assert not out[0, :, :9].any() and not out[1].any()
+    grads = torch.autograd.grad(out, ls, do.to(dev))
+    clean = [t[0].clone(), *t[1:]]
+    clean[0][0, :, :9] = 1.0
+    clean[0][1] = 1.0
+    do = torch.nan_to_num(do.clone(), 0.0, 0.0, 0.0)
+    lc = [x.to(dev).requires_grad_() for x in clean]
+    want = torch.autograd.grad(SF.bucket_attention(*lc, bk, 2, keep=keep.to(dev), causal=True, q_start=-9), lc, do.to(dev))
+    for g, w in zip(grads, want):
+        assert torch.equal(g, w)
+
+
+@_dt
+@pytest.mark.parametrize("low", [-math.inf, torch.finfo(torch.float32).min])
+def test_attention_buckets_without_weight(dev, dt, low):
+    """A table entry of -inf or the type's lowest value hides its bucket's pairs, as `keep` would."""
+    bk = SF.RelativeBuckets(16, 24, True)
+    for tq, tk in ((40, 70), (1, 130)):
+        *t, do = case(33, dt, 1, 2, 2, 24, tq, tk)
+        t[3][7, 0] = low                                                 # (head 0: the keys far in the past)
+        t[3][8:, 1] = low                                                # (head 1: all keys behind the query)
+        compare(dev, dt, t, do, bk, 2, q_start=30, what=f"{tq}")
+
+
+def test_second_derivatives_are_refused(dev):
+    gen = torch.Generator().manual_seed(34)
+    bk = SF.RelativeBuckets(8, 20)
+    x = torch.randn(1, 16, 9, generator=gen).to(dev).requires_grad_()
+    table = torch.randn(8, 2, generator=gen).to(dev).requires_grad_()
+    for out in (SF.layer_norm_nct(x, None, None), SF.bucket_attention(x, x, x, table, bk, 2), SF.bucket_bias(table, bk, 3, 4)):
+        leaf = x if out.shape == x.shape else table
+        g, = torch.autograd.grad(out.square().sum(), leaf, create_graph=True)
+        with pytest.raises(RuntimeError):
+            torch.autograd.grad(g.sum(), leaf)
+
+
+def test_far_positions_and_lengths(dev):
+    """Starts beyond the ABI's 32 bits are as far as can be; lengths beyond them are refused before anything is allocated."""
+    bk = SF.RelativeBuckets(8, 20)
+    table = torch.randn(8, 2, generator=torch.Generator().manual_seed(35)).to(dev).requires_grad_()
+    for start, bucket in ((1 << 40, 3), (-(1 << 40), 7)):
+        bias = SF.bucket_bias(table, bk, 3, 5, q_start=start)
+        assert torch.equal(bias, table[bucket][:, None, None].expand(2, 3, 5))
+        g, = torch.autograd.grad(bias.sum(), table)
+        want = torch.zeros(8, 2)
+        want[bucket] = 15
+        assert torch.equal(g.cpu(), want)
+        q = torch.randn(1, 8, 3, generator=torch.Generator().manual_seed(36)).to(dev)
+        assert torch.equal(SF.bucket_attention(q, q, q, table, bk, 2, q_start=start), SF.bucket_attention(q, q, q, table, bk, 2, q_start=99 * (1 if start > 0 else -1)))
+    with pytest.raises(ValueError):
+        SF.bucket_bias(table, bk, 1 << 40, 0)
+    with pytest.raises(ValueError):
+        SF.bucket_attention(torch.zeros(1, 2, 1, device=dev).expand(1, 2, (1 << 32) + 5)[:, :, :0], *[torch.zeros(1, 2, 0, device=dev).expand((1 << 32) + 1, 2, 0)] * 2,
+                            table, bk, 2)
+
+
+def test_layer_norm_nct_affine_sizes(dev):
+    """gamma and beta of another size are refused with and without gradients; any stride of them is taken."""
+    x = torch.randn(2, 12, 9, generator=torch.Generator().manual_seed(37)).to(dev)
+    wide = torch.randn(24, generator=torch.Generator().manual_seed(38)).to(dev)
+    for leaf in (x, x.clone().requires_grad_()):
+        for bad in (wide, wide[:11]):
+            with pytest.raises(ValueError):
+                SF.layer_norm_nct(leaf, bad, None)
+            with pytest.raises(ValueError):
+                SF.layer_norm_nct(leaf, wide[:12], bad)
+        assert torch.equal(SF.layer_norm_nct(leaf, wide[::2], wide[1::2]), SF.layer_norm_nct(leaf, wide[::2].clone(), wide[1::2].clone()))
+
+
+# ---- on the GPU: real lengths, streams, graphs ----------------------------------------------------------------------------
+@pytest.mark.gpu
+@_dt
+@pytest.mark.parametrize("shape", [(1, 4, 2, 64, 2000, 2000), (2, 2, 2, 128, 1030, 1500), (9, 8, 8, 16, 600, 513), (3, 2, 1, 96, 777, 1025)])
+def test_attention_long(gpu_only, dt, shape):
+    B, H, Hkv, dk, tq, tk = shape
+    *t, do = case(sum(shape), dt, *shape, n=32)
+    keep = torch.ones(B, tk)
+    keep[0, tk - 77:] = 0
+    keep[0, 300:420] = 0
+    compare("cuda", dt, t, do, SF.RelativeBuckets(32, 128, True), H, keep=keep, what="masked")
+    compare("cuda", dt, t, do, SF.RelativeBuckets(32, 128, False), H, causal=True, what="causal")
+
+
+@pytest.mark.gpu
+def test_attention_cache_beyond_32_bits(gpu_only):
+    """The last entry of a cache of more than 2^32 elements: one token, several (another form), and its gradients."""
+    B, H, Hkv, dk, tk = 5, 8, 8, 128, 1 << 20
+    gen = torch.Generator(device="cuda").manual_seed(41)
+    k, v = (torch.randn(B, Hkv * dk, tk, generator=gen, device="cuda", dtype=torch.bfloat16) for _ in range(2))
+    assert k.numel() > 1 << 32
+    table = torch.randn(32, H, generator=gen, device="cuda")
+    bk = SF.RelativeBuckets(32, 128, False)
+    for tq in (1, 40):
+        q = torch.randn(B, H * dk, tq, generator=gen, device="cuda", dtype=torch.bfloat16)
+        do = torch.randn(B, H * dk, tq, generator=gen, device="cuda", dtype=torch.bfloat16)
+        ls = [x.detach().requires_grad_() for x in (q, k, v)] if tq > 1 else [q, k, v]
+        out = SF.bucket_attention(*ls, table, bk, H, causal=True)
+        grads = torch.autograd.grad(out, ls, do) if tq > 1 else None
+        for b, h in ((0, 0), (B - 1, H - 1)):
+            qh, kh, vh, dh = (x[b, h * dk:(h + 1) * dk].detach().double() for x in (q, k, v, do))
+            off = torch.arange(tk, device="cuda")[None] - (tk - tq + torch.arange(tq, device="cuda")[:, None])
+            lut = bucket_index(bk, 1, 400, 399)[0].to("cuda")              # offsets -399 .. 0
+            s = qh.t() @ kh * dk ** -0.5 + table[:, h].double()[lut[(off.clamp(-399, 0) + 399)]]
+            p = torch.softmax(s.masked_fill(off > 0, -math.inf), 1)
+            near(out[b, h * dk:(h + 1) * dk], (vh @ p.t()).cpu(), 3 * UBF, f"out {tq} {b}")
+            if grads:
+                dp = dh.t() @ vh
+                ds = p * (dp - (p * dp).sum(1, keepdim=True)) * dk ** -0.5
+                near(grads[0][b, h * dk:(h + 1) * dk], (kh @ ds.t()).cpu(), 3 * UBF, f"dq {b}")
+                near(grads[1][b, h * dk:(h + 1) * dk], (qh @ ds).cpu(), 3 * UBF, f"dk {b}")
+                near(grads[2][b, h * dk:(h + 1) * dk], (dh @ p).cpu(), 3 * UBF, f"dv {b}")
+
+
+@pytest.mark.gpu
+def test_bucket_bias_many_rows(gpu_only):
+    """More rows than a launch has workgroups in its second dimension."""
+    tq = (1 << 20) + 3
+    bk = SF.RelativeBuckets(8, 20)
+    table = torch.randn(8, 1, device="cuda").requires_grad_()
+    bias = SF.bucket_bias(table, bk, tq, 3, q_start=-10)
+    g, = torch.autograd.grad(bias, table, torch.ones_like(bias))
+    want = torch.zeros(8)
+    for o in range(-60, 40):
+        rows = sum(1 for j in range(3) if 0 <= j - o + 10 < tq)
+        want[bucket_of(o, 8, 20, True)] += rows
+    far = 3 * tq - int(want.sum())
+    want[bucket_of(-1000, 8, 20, True)] += far
+    assert torch.equal(g[:, 0].cpu(), want)                               # (whole numbers below 2^24)
+
+
+def _block(x, gamma, beta, table, bk, H):
+    n = SF.layer_norm_nct(x, gamma, beta)
+    return SF.bucket_attention(n, n, n, table, bk, H, causal=True)
+
+
+@pytest.mark.gpu
+@_dt
+def test_block_on_another_stream(gpu_only, dt):
+    """Forward and backward on a side stream that made the inputs: the same bits as on the default stream."""
+    gen = torch.Generator().manual_seed(42)
+    raw = [torch.randn(3, 64, 500, generator=gen).to(DT[dt]), torch.rand(64, generator=gen), torch.randn(64, generator=gen), torch.randn(16, 2, generator=gen),
+           torch.randn(3, 64, 500, generator=gen).to(DT[dt])]
+    bk = SF.RelativeBuckets(16, 40, False)
+
+    def run():
+        *ls, do = [x.cuda() for x in raw]
+        ls = [x.requires_grad_() for x in ls]
+        out = _block(*ls, bk, 2)
+        return [out, *torch.autograd.grad(out, ls, do)]
+    want = run()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = run()
+    side.synchronize()
+    for g, w in zip(got, want):
+        assert torch.equal(g, w)
+
+
+def _replays(graphs, inputs, outputs, fresh, eager):
+    """Replays the graphs in turn over new inputs, eager work and a synchronization between them, against the eager result."""
+    for _ in range(4):
+        for src, dst in zip(fresh(), inputs):
+            dst.copy_(src)
+        want = eager()
+        torch.cuda.synchronize()
+        for g, out in zip(graphs, outputs):
+            g.replay()
+            torch.cuda.synchronize()
+            for a, w in zip(out, want):
+                assert torch.equal(a, w)
+            eager()
+
+
+@pytest.mark.gpu
+@_dt
+def test_cached_token_in_graphs(gpu_only, dt):
+    """The serving form captured twice (the splits' workspaces are each graph's own), with moving lengths."""
+    gen = torch.Generator(device="cuda").manual_seed(43)
+    B, H, Hkv, dk, tk = 3, 8, 2, 40, 2000
+    bk = SF.RelativeBuckets(32, 128, False)
+    shapes = ((B, H * dk, 1), (B, Hkv * dk, tk), (B, Hkv * dk, tk))
+    table = torch.randn(32, H, device="cuda", generator=gen)
+
+    def fresh():
+        return [torch.randn(s, device="cuda", generator=gen).to(DT[dt]) for s in shapes] + [torch.randint(0, tk, (B,), device="cuda", generator=gen).int()]
+    inputs = fresh()
+
+    def eager():
+        with torch.no_grad():
+            return [SF.bucket_attention(*inputs[:3], table, bk, H, causal=True, q_start=inputs[3])]
+    eager()
+    graphs, outputs = [], []
+    for _ in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outputs.append(eager())
+        graphs.append(g)
+    _replays(graphs, inputs, outputs, fresh, eager)
+
+
+@pytest.mark.gpu
+@_dt
+def test_block_training_step_in_a_graph(gpu_only, dt):
+    """Norm and attention with all gradients captured; leaves of their own in the graph."""
+    gen = torch.Generator(device="cuda").manual_seed(44)
+    bk = SF.RelativeBuckets(16, 40, False)
+
+    def fresh():
+        return [torch.randn(2, 96, 300, device="cuda", generator=gen).to(DT[dt]), torch.rand(96, device="cuda", generator=gen),
+                torch.randn(96, device="cuda", generator=gen), torch.randn(16, 2, device="cuda", generator=gen),
+                torch.randn(2, 96, 300, device="cuda", generator=gen).to(DT[dt])]
+    inputs = fresh()
+
+    def step():
+        ls = [x.detach().requires_grad_() for x in inputs[:4]]
+        out = _block(*ls, bk, 2)
+        return [out.detach(), *torch.autograd.grad(out, ls, inputs[4])]
+    step()
+    graphs, outputs = [], []
+    for _ in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outputs.append(step())
+        graphs.append(g)
+    _replays(graphs, inputs, outputs, fresh, step)
