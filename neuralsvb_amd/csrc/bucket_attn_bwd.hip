@@ -66,14 +66,22 @@ __device__ __forceinline__ void svbt_diag_add(float* skew, float* diag, const f3
     diag[kb ? l31 - 32 : l31] += kb ? there : here;                     // (64 different offsets)
 }
 
+// One sub-tile's scores -> dS in place; rows are keys, this lane's query has lse and delta.  NEAR: the bias varies; bias0: at row 0.
+template <bool NEAR>
+__device__ __forceinline__ void svbt_weights_q(f32x16& s, const f32x16& dp, float c, const float* bias0, float flat, float lse, float delta) {
+#pragma unroll
+    for (int r = 0; r < 16; ++r) s[r] = svbt_ds(__builtin_amdgcn_exp2f(fmaf(s[r], c, NEAR ? bias0[svbt_reg(r)] : flat) - lse), dp[r], delta);
+}
+
 // ---- dq, dtable, delta: 4 waves x 32 queries, keys staged ----------------------------------------------------------------------------
 template <typename T, int DKP, int KT, bool DOUBLE, bool TINY>
 __global__ __launch_bounds__(256, SvbtParts<T>::NS == 1 || DKP <= 64 ? 2 : 1) void svb_bucket_attn_dq_kernel(SvbBucketAttn a, SvbBattnBwd g, int qtiles) {
     typedef SvbtTile<T, DKP, KT, 256, TINY> Tile;
     constexpr int NS = Tile::NS, NK = DKP / 16, NDB = DKP / 32, NSUB = KT / 32;
     constexpr int BUF = NS * (2 * Tile::ROWS_BYTES + Tile::COLS_BYTES);
+    constexpr bool PACED = NS == 3 || DKP <= 64;                        // (wide bf16 heads: no registers to read ahead into, 194 us instead of 164)
     HIP_DYNAMIC_SHARED(char, smem)
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l31 = lane & 31, kb = lane >> 5;
+    const int lane = threadIdx.x & 63, wave = svb_uniform(threadIdx.x >> 6), l31 = lane & 31, kb = lane >> 5;
     int bh, qt;
     svbt_item(blockIdx.x, a.B * a.H, qtiles, a.causal, bh, qt);
     if (a.causal) qt = qtiles - 1 - qt;
@@ -190,31 +198,25 @@ __global__ __launch_bounds__(256, SvbtParts<T>::NS == 1 || DKP <= 64 ? 2 : 1) vo
                     Tile::row_frag(vrows, u, x, l31, kb, f);
                     svbt_mma<NS, false>(x & 1 ? dp_neg : dp, f, of[x]);
                 }
+                if (PACED) svbt_pace<NS, 2 * NK * NS>();
 #pragma unroll
                 for (int r = 0; r < 16; ++r) dp[r] -= dp_neg[r];
                 const unsigned su = (unsigned)(now >> (32 * u)) >> (4 * kb);
                 const int o0 = svbt_fresh(j0 + 32 * u + 4 * kb - p);     // offset of register row 0
-                if (behind || before) {
+                const bool far = behind || before;
+                if (far) svbt_weights_q<false>(s, dp, c, nullptr, flat, lse, delta);
+                else svbt_weights_q<true>(s, dp, c, s_bias + (o0 + R + SVBT_PAD), flat, lse, delta);
+                if (edge) {
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) s[r] = (su >> svbt_reg(r) & 1u) && !(a.causal && o0 + svbt_reg(r) > 0) ? s[r] : 0.f;
+                }
+                if (far) {
                     float sum = 0.f;
 #pragma unroll
-                    for (int r = 0; r < 16; ++r) {
-                        float w = __builtin_amdgcn_exp2f(fmaf(s[r], c, flat) - lse);
-                        if (edge) w = (su >> svbt_reg(r) & 1u) && !(a.causal && o0 + svbt_reg(r) > 0) ? w : 0.f;
-                        s[r] = svbt_ds(w, dp[r], delta);
-                        sum += s[r];
-                    }
+                    for (int r = 0; r < 16; ++r) sum += s[r];
                     if (behind) sum_past += sum;
                     else sum_ahead += sum;
-                } else {
-                    const float* bias0 = s_bias + (o0 + R + SVBT_PAD);
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) {
-                        float w = __builtin_amdgcn_exp2f(fmaf(s[r], c, bias0[svbt_reg(r)]) - lse);
-                        if (edge) w = (su >> svbt_reg(r) & 1u) && !(a.causal && o0 + svbt_reg(r) > 0) ? w : 0.f;
-                        s[r] = svbt_ds(w, dp[r], delta);
-                    }
-                    if (g.part) svbt_diag_add(my_skew, my_diag + (j0 + 32 * u - p0), s, l31, kb);
-                }
+                } else if (g.part) svbt_diag_add(my_skew, my_diag + (j0 + 32 * u - p0), s, l31, kb);
 #pragma unroll
                 for (int x = 0; x < 2; ++x) {
                     float w[8];
@@ -229,6 +231,7 @@ __global__ __launch_bounds__(256, SvbtParts<T>::NS == 1 || DKP <= 64 ? 2 : 1) vo
                         svbt_mma<NS, false>(acc[d], f, sf);
                     }
                 }
+                if (PACED) svbt_pace<NS, 2 * NDB * NS>();
             }
         }
         if (t + 1 < tiles) {
@@ -271,6 +274,22 @@ __global__ __launch_bounds__(256, SvbtParts<T>::NS == 1 || DKP <= 64 ? 2 : 1) vo
         }
 }
 
+// One sub-tile's scores -> P and dP -> dS, in place; rows are queries.  NEAR: the bias varies; bias0: at row 0.  ls, dl: log-sum and delta
+// of the sub-tile's rows from 4 kb on.
+template <bool NEAR>
+__device__ __forceinline__ void svbt_weights_kv(f32x16& s, f32x16& dp, float c, const float* bias0, float flat, const float* ls, const float* dl) {
+#pragma unroll
+    for (int r4 = 0; r4 < 4; ++r4) {
+        const float4 l = *reinterpret_cast<const float4*>(ls + 8 * r4), d = *reinterpret_cast<const float4*>(dl + 8 * r4);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const int r = 4 * r4 + e;
+            s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], c, NEAR ? bias0[-svbt_reg(r)] : flat) - l[e]);
+            dp[r] = svbt_ds(s[r], dp[r], d[e]);
+        }
+    }
+}
+
 // ---- dk, dv: 4 waves x 32 keys, queries of the heads that share them staged -----------------------------------------------------------
 // The (head, query tile) steps of a key tile can be split over workgroups: each then leaves its sums in memory, to be added in order.
 template <typename T, int DKP, int KT, bool DOUBLE, bool TINY>
@@ -279,7 +298,7 @@ __global__ __launch_bounds__(256, DKP <= (SvbtParts<T>::NS == 1 ? 64 : 32) ? 2 :
     constexpr int NS = Tile::NS, NK = DKP / 16, NDB = DKP / 32, NSUB = KT / 32;
     constexpr int TILE = NS * 2 * (Tile::ROWS_BYTES + Tile::COLS_BYTES), BUF = TILE + 2 * KT * 4;
     HIP_DYNAMIC_SHARED(char, smem)
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l31 = lane & 31, kb = lane >> 5;
+    const int lane = threadIdx.x & 63, wave = svb_uniform(threadIdx.x >> 6), l31 = lane & 31, kb = lane >> 5;
     int bk, ks;
     svbt_item(blockIdx.x, a.B * a.Hkv, ktiles * g.splits, a.causal, bk, ks);
     const int kt = svb_uniform(ks / g.splits), split = ks - kt * g.splits;
@@ -368,21 +387,17 @@ __global__ __launch_bounds__(256, DKP <= (SvbtParts<T>::NS == 1 ? 64 : 32) ? 2 :
                     Tile::row_frag(drows, u, x, l31, kb, f);
                     svbt_mma<NS, true>(dp, f, vf[x]);
                 }
+                svbt_pace<NS, 2 * NK * NS>();
                 const int o0 = svbt_fresh(j - (pt + 32 * u + 4 * kb));   // offset of register row 0
-                const float* bias0 = s_bias + (behind || before ? 0 : o0 + R + SVBT_PAD);
+                const float *ls = stats + 32 * u + 4 * kb, *dl = ls + KT;
+                if (behind || before) svbt_weights_kv<false>(s, dp, c, nullptr, flat, ls, dl);
+                else svbt_weights_kv<true>(s, dp, c, s_bias + (o0 + R + SVBT_PAD), flat, ls, dl);
+                if (edge) {
 #pragma unroll
-                for (int r4 = 0; r4 < 4; ++r4) {
-                    const float4 ls = *reinterpret_cast<const float4*>(stats + 32 * u + 8 * r4 + 4 * kb);
-                    const float4 dl = *reinterpret_cast<const float4*>(stats + KT + 32 * u + 8 * r4 + 4 * kb);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const int r = 4 * r4 + e, o = o0 - svbt_reg(r);
-                        float bias = flat;
-                        if (!(behind || before)) bias = bias0[-svbt_reg(r)];
-                        float w = __builtin_amdgcn_exp2f(fmaf(s[r], c, bias) - ls[e]);
-                        if (edge) w = kept && !(a.causal && o > 0) ? w : 0.f;
-                        s[r] = w;
-                        dp[r] = svbt_ds(w, dp[r], dl[e]);
+                    for (int r = 0; r < 16; ++r) {
+                        const bool sees = kept && !(a.causal && o0 - svbt_reg(r) > 0);
+                        s[r] = sees ? s[r] : 0.f;
+                        dp[r] = sees ? dp[r] : 0.f;
                     }
                 }
 #pragma unroll
@@ -402,6 +417,7 @@ __global__ __launch_bounds__(256, DKP <= (SvbtParts<T>::NS == 1 ? 64 : 32) ? 2 :
                         svbt_mma<NS, false>(dk[d], f, sf);
                     }
                 }
+                svbt_pace<NS, 4 * NDB * NS>();
             }
         }
         if (n + 1 < n1) {

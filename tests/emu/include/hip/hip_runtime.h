@@ -78,6 +78,7 @@ static inline void __builtin_amdgcn_s_barrier_emu() { emu_syncthreads(); }
 #define __builtin_amdgcn_s_barrier() emu_syncthreads()
 #define __builtin_amdgcn_s_setprio(x) ((void)0)
 #define __builtin_amdgcn_sched_barrier(x) ((void)0)
+#define __builtin_amdgcn_sched_group_barrier(mask, size, group) ((void)0)
 void emu_wave_sync();                                             // all lanes of the calling wave arrive before any continues
 #define __builtin_amdgcn_wave_barrier() emu_wave_sync()
 #define __builtin_amdgcn_fence(order, scope) ((void)0)             // (the emulator's lanes run one at a time: program order is memory order)
