@@ -220,7 +220,9 @@ template <> struct SvbtBlock<float> {
 // the loads have no branches and stay in flight together.  A channel >= dk reads channel dk - 1: own operands are 0 there, and result
 // rows of such channels are not written.
 // TINY: rows of less than 4 elements, read one by one (a form of its own: with both in one loop the loads are waited for where they join).
-template <typename T, int DKP, int KT, int NT, bool TINY>
+// FRESH: addresses are computed anew for each tile, not kept in registers over the loop -- for the kernels that run out of registers (a spilled
+// address comes back through memory, behind the tile's first loads) or get room for another workgroup.
+template <typename T, int DKP, int KT, int NT, bool TINY, bool FRESH>
 struct SvbtTile {
     static constexpr int NS = SvbtParts<T>::NS, JB = KT / 4, BLOCKS = JB * (DKP / 4), NB = (BLOCKS + NT - 1) / NT;
     static constexpr int ROWP = 2 * DKP + 16, COLP = 2 * KT + 16;                       // pitches, bytes
@@ -241,7 +243,7 @@ struct SvbtTile {
         for (int i = 0; i < NB; ++i) {
             const int id = tid + i * NT, j = j0 + pos(id);
             if (BLOCKS % NT != 0 && id >= BLOCKS) continue;
-            const int d = min(chan(id), dk - 1), more = dk - 1 - d;
+            const int d = FRESH ? svbt_fresh(min(chan(id), dk - 1)) : min(chan(id), dk - 1), more = dk - 1 - d;
             long long off = (long long)d * sc + max(0, min(j, L - 4));
             svb_opaque(off);                                            // (one offset per block through the loop, not one per row)
             const T* p = base + off;

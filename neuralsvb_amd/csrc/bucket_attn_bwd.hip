@@ -76,7 +76,8 @@ __device__ __forceinline__ void svbt_weights_q(f32x16& s, const f32x16& dp, floa
 // ---- dq, dtable, delta: 4 waves x 32 queries, keys staged ----------------------------------------------------------------------------
 template <typename T, int DKP, int KT, bool DOUBLE, bool TINY>
 __global__ __launch_bounds__(256, SvbtParts<T>::NS == 1 || DKP <= 64 ? 2 : 1) void svb_bucket_attn_dq_kernel(SvbBucketAttn a, SvbBattnBwd g, int qtiles) {
-    typedef SvbtTile<T, DKP, KT, 256, TINY> Tile;
+    // (FRESH: B2 H16/4 dk128 T2048 causal bf16 171 -> 158 us, B32 H4 dk64 T562 fp32 169 -> 156; elsewhere it costs 1 to 3 %)
+    typedef SvbtTile<T, DKP, KT, 256, TINY, DKP == 128 || (SvbtParts<T>::NS == 3 && DKP == 64)> Tile;
     constexpr int NS = Tile::NS, NK = DKP / 16, NDB = DKP / 32, NSUB = KT / 32;
     constexpr int BUF = NS * (2 * Tile::ROWS_BYTES + Tile::COLS_BYTES);
     constexpr bool PACED = NS == 3 || DKP <= 64;                        // (wide bf16 heads: no registers to read ahead into, 194 us instead of 164)
@@ -294,7 +295,8 @@ __device__ __forceinline__ void svbt_weights_kv(f32x16& s, f32x16& dp, float c, 
 // The (head, query tile) steps of a key tile can be split over workgroups: each then leaves its sums in memory, to be added in order.
 template <typename T, int DKP, int KT, bool DOUBLE, bool TINY>
 __global__ __launch_bounds__(256, DKP <= (SvbtParts<T>::NS == 1 ? 64 : 32) ? 2 : 1) void svb_bucket_attn_dkv_kernel(SvbBucketAttn a, SvbBattnBwd g, int ktiles) {
-    typedef SvbtTile<T, DKP, KT, 256, TINY> Tile;
+    // (FRESH: B16 H4 dk32 T700 bf16 62 -> 48 us, B8 H4 dk128 T562 fp32 206 -> 202; elsewhere it costs 0 to 3 %)
+    typedef SvbtTile<T, DKP, KT, 256, TINY, SvbtParts<T>::NS == 1 ? DKP == 32 : DKP == 128> Tile;
     constexpr int NS = Tile::NS, NK = DKP / 16, NDB = DKP / 32, NSUB = KT / 32;
     constexpr int TILE = NS * 2 * (Tile::ROWS_BYTES + Tile::COLS_BYTES), BUF = TILE + 2 * KT * 4;
     HIP_DYNAMIC_SHARED(char, smem)
@@ -474,7 +476,7 @@ static int bwd_lds(K* kern, int lds) {
 
 template <typename T, int DKP, int KT, bool DOUBLE, bool TINY = false>
 static int dq_launch(const SvbBucketAttn* a, const SvbBattnBwd& g, hipStream_t st) {
-    typedef SvbtTile<T, DKP, KT, 256, TINY> Tile;
+    typedef SvbtTile<T, DKP, KT, 256, TINY, false> Tile;
     const int span = svbt_span(a->buckets), qtiles = (a->Tq + 127) / 128;
     const int lds = (DOUBLE ? 2 : 1) * Tile::NS * (2 * Tile::ROWS_BYTES + Tile::COLS_BYTES) + (g.part ? 5 * span + 4 * 32 * SVBT_SKEW_P + 8 : span) * 4;
     auto* kern = svb_bucket_attn_dq_kernel<T, DKP, KT, DOUBLE, TINY>;
@@ -486,7 +488,7 @@ static int dq_launch(const SvbBucketAttn* a, const SvbBattnBwd& g, hipStream_t s
 
 template <typename T, int DKP, int KT, bool DOUBLE, bool TINY = false>
 static int dkv_launch(const SvbBucketAttn* a, const SvbBattnBwd& g, hipStream_t st) {
-    typedef SvbtTile<T, DKP, KT, 256, TINY> Tile;
+    typedef SvbtTile<T, DKP, KT, 256, TINY, false> Tile;
     const int span = svbt_span(a->buckets), ktiles = (a->Tk + 127) / 128;
     const int lds = (DOUBLE ? 2 : 1) * (2 * Tile::NS * (Tile::ROWS_BYTES + Tile::COLS_BYTES) + 2 * KT * 4) + span * 4;
     auto* kern = svb_bucket_attn_dkv_kernel<T, DKP, KT, DOUBLE, TINY>;
