@@ -153,6 +153,7 @@ __global__ __launch_bounds__(256, SvbtParts<T>::NS == 3 && DKP == 128 ? 1 : 2) v
                     svbt_mma<NS, false>(s[u], f, qf[x]);
                 }
             }
+            svbt_pace<NS, NSUB * NK * NS>();
             const bool edge = now != MINE || (a.causal && j0 + 32 * NSUB - 1 > p0);
             const bool behind = j0 + 32 * NSUB - 1 - p0 <= -R, before = j0 - p1 >= R;
             const float flat = behind ? past : ahead;
