@@ -191,6 +191,7 @@ __global__ __launch_bounds__(256, SvbtParts<T>::NS == 3 && DKP == 128 ? 1 : 2) v
                         }
                     }
                 }
+            if (PP == NS) svbt_pace<NS, NSUB * 2 * NDB * NS>();
         }
         if (t + 1 < tiles) {
             if (!DOUBLE) __syncthreads();                               // (this tile's fragments are read)
