@@ -874,6 +874,15 @@ def layer_norm(x, gamma, beta, eps=1e-5):
     return _LayerNormFn.apply(x, gamma, beta, float(eps))
 
 
+def _first_order(fn):
+    """once_differentiable (a second derivative is an error), at its cost of 10 us of host time only where the backward is itself recorded."""
+    guarded = once_differentiable(fn)
+
+    def backward(ctx, *grads):
+        return guarded(ctx, *grads) if torch.is_grad_enabled() else fn(ctx, *grads)
+    return backward
+
+
 class _LayerNormNCTFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, gamma, beta, eps):
@@ -884,7 +893,7 @@ class _LayerNormNCTFn(torch.autograd.Function):
         return y
 
     @staticmethod
-    @once_differentiable
+    @_first_order
     def backward(ctx, dy):
         x, gamma, stats = ctx.saved_tensors
         return K.ln_nct_bwd(x, gamma, _c(dy), stats, *ctx.needs_input_grad[:3], ctx.affine_dtype) + (None,)
@@ -946,7 +955,7 @@ class _BucketBiasFn(torch.autograd.Function):
         return K.bucket_bias_fwd(_c(table), buckets, tq, tk, q_start)
 
     @staticmethod
-    @once_differentiable
+    @_first_order
     def backward(ctx, dbias):
         buckets, q_start = ctx.cfg
         return K.bucket_bias_bwd(_c(dbias), buckets, q_start), None, None, None, None
@@ -973,7 +982,7 @@ class _BucketAttnFn(torch.autograd.Function):
         return out
 
     @staticmethod
-    @once_differentiable
+    @_first_order
     def backward(ctx, dout):
         q, k, v, table, keep, starts, out, lse, o32 = ctx.saved_tensors
         nq, nk, nv, nt = ctx.needs_input_grad[:4]
