@@ -626,7 +626,12 @@ __device__ __forceinline__ void svbq_pack_row(const float* v, const float* gnorm
     for (int e = threadIdx.x; e < rowlen; e += 256) {
         const int c1 = e / k, j = e - c1 * k;
         unsigned hi, lo;
-        svbq_split(vr[e] * scale, hi, lo);
+        float w;
+        {
+#pragma clang fp contract(off)
+            w = vr[e] * scale;                                           // (rounded, as a weight in memory is: lo is what hi leaves of it)
+        }
+        svbq_split(w, hi, lo);
         if (qa_hi) {
             const size_t ia = (((size_t)j * kcha + (c1 >> 4)) * d0 + row) * 16 + (c1 & 15);
             qa_hi[ia] = (unsigned short)hi; qa_lo[ia] = (unsigned short)lo;
