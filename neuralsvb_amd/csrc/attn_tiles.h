@@ -42,7 +42,7 @@ __device__ __forceinline__ unsigned svbt_pack2(float a, float b) {
 __device__ __forceinline__ float svbt_lo(unsigned u) { return __uint_as_float(u << 16); }
 __device__ __forceinline__ float svbt_hi(unsigned u) { return __uint_as_float(u & 0xffff0000u); }
 
-// two floats -> NS packed bf16 pairs that add up to them (to 2^-9, 2^-18, 2^-25 of each)
+// two floats -> NS packed bf16 pairs that add up to them (to 2^-8, 2^-16, 2^-24 of each)
 template <int NS>
 __device__ __forceinline__ void svbt_parts2(float a, float b, unsigned (&p)[NS]) {
     p[0] = svbt_pack2(a, b);

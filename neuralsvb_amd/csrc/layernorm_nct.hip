@@ -404,7 +404,7 @@ static void svbl_launch(bool fwd, const SvbLnArgs& a, const SvbLnPlan& p, unsign
 static bool svbl_fits(int B, int C, int T, int dtype, SvbLnPlan* p, int* tiles) {
     *p = svbl_plan(C, T, dtype);
     *tiles = (T + p->positions - 1) / p->positions;
-    return (long)B * *tiles < (1 << 22);                                 // (a launch has less than 2^32 threads)
+    return (long)B * *tiles < (1 << 23);                                 // (a launch has less than 2^32 threads)
 }
 static bool svbl_dtypes(int dtype, int affine_dtype) {
     return (dtype == SVB_DT_F32 && affine_dtype == SVB_DT_F32) || (dtype == SVB_DT_BF16 && (affine_dtype == SVB_DT_F32 || affine_dtype == SVB_DT_BF16));

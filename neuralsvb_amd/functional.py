@@ -1006,6 +1006,10 @@ def bucket_attention(q, k, v, table, buckets, n_head, keep=None, causal=False, s
     Tk - Tq); with causal=True and Tq = 1 a tensor of cached lengths - 1 serves one new token per request from caches of one capacity.
     A query that sees no key gives zeros and no gradient.  -> [B, H dk, Tq].
 
+    Table entries of -inf, or so low that log2(e) times them is (the type's lowest value), hide the pairs of their bucket.  q and dout are
+    finite in rows that see a key.  The leaves of a backward pass that is captured into a graph belong to that graph alone: an eager graph
+    of the same leaves that still lives ties their gradients to its stream, which ends the capture (and the process with it).
+
     float32 tensors are multiplied in three bf16 parts whatever `conv_precision` says (as the rel-pos attention of the fp32 mode)."""
     n_head = int(n_head)
     if n_head < 1:
