@@ -610,7 +610,7 @@ extern "C" int svb_bucket_attn_fwd(const SvbBucketAttn* call, float* ws, void* s
          : a->dk <= 96 ? fwd_launch<T, 96, KT, D96, PP, KG>(a, st) : fwd_launch<T, 128, KT, true, PP, KG>(a, st)
     if (a->dtype == SVB_DT_F32) SVB_FWD_GO(float, 32, 32, 3, false, 1);
     // At most one workgroup of 128 queries per CU and several tiles of keys: workgroups of 64 queries, twice as many, the keys of a tile over
-    // two waves, tiles of 128 keys up to dk 64.  B2 H8 dk64 T2000 causal (256 workgroups): 52 -> 41 us, training 72 -> 48; B4 H8 dk96 T1000
+    // two waves, tiles of 128 keys up to dk 64.  B2 H8 dk64 T2000 causal (256 workgroups): 52 -> 41 us, training 72 -> 48 (35 and 44 with the steps since); B4 H8 dk96 T1000
     // causal: 38 -> 34; B24 H4 dk48 T211, where a join and a bigger tile save nothing: 14.5 -> 16.5.  Between one and two workgroups per CU
     // (B7 H8 dk64 T1100 causal) the forward takes 39 us this way instead of 36.  fp32 tensors have six products per tile to wait behind.
     const bool thin = a->Tk > 256 && (long)a->B * a->H * ((a->Tq + 127) / 128) <= 256;

@@ -243,7 +243,8 @@ def compare(dev, dt, tensors, dout, buckets, n_head, keep=None, causal=False, sc
     # fp32: three bf16 parts keep 2^-25 of each operand; scores of size 8 carry 8 half steps into the weights' exponents, the sums
     # (up to 128 channels and some hundred keys) a few more.
     tol = 3 * UBF if dt == "bf16" else 128 * U32
-    # dtable is fp32 for either type; with bf16 tensors delta comes from P in two parts (2^-16), and a bucket's sum cancels
+    # dtable is fp32 for either type, and a bucket's sum cancels; with bf16 tensors delta comes from the output before its rounding, with P
+    # in parts of 2^-8 each (two of them leave 2^-16: the bound)
     tol_table = {"bf16": 8 * 2.0 ** -16, "f32": 128 * U32}[dt] + (UBF if tensors[3].dtype == torch.bfloat16 else 0)
     want_leaves = leaves64(*tensors)
     want = attention64(*want_leaves, buckets, n_head, keep, causal, scale, q_start)
