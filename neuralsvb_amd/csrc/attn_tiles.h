@@ -26,6 +26,7 @@ typedef unsigned svbt_u2u __attribute__((ext_vector_type(2), aligned(2)));
 
 #define SVBT_LOG2E 1.4426950408889634f
 #define SVBT_INF __builtin_inff()
+#define SVBT_BAD_WORDS 4               /* bits of the keys that a workgroup's 128 queries see in part */
 
 // T: float or unsigned short (bf16)
 template <typename T> struct SvbtParts;
@@ -109,6 +110,9 @@ __device__ __forceinline__ int svbt_fresh(int x) {
     return (int)u;
 }
 
+// not finite, or (fp32) beyond what three bf16 parts can hold: the first part would round to infinity
+__device__ __forceinline__ bool svbt_bad(float x) { return (__float_as_uint(x) & 0x7fffffffu) > 0x7f7f7fffu; }
+
 __device__ __forceinline__ float svbt_load(const float* p) { return *p; }
 __device__ __forceinline__ float svbt_load(const unsigned short* p) { return svb_bf16_f32(*p); }
 __device__ __forceinline__ void svbt_store(float* p, float v) { *p = v; }
@@ -171,6 +175,26 @@ template <> struct SvbtBlock<unsigned short> {
 #pragma unroll
         for (int c = 0; c < 4; ++c) { r[c][0] &= m0; r[c][1] &= m1; }
     }
+    // elements that are not finite become zero, at the positions of `which`; -> the positions where there were some
+    __device__ __forceinline__ unsigned clear_bad(unsigned which) {
+        unsigned any = 0u, found = 0u;
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) any |= (r[c][h] & 0x7f807f80u) + 0x00800080u;                  // (an exponent of ones carries)
+        if ((any & 0x80008000u) == 0u) return 0u;
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const unsigned m = e & 1 ? 0x7f800000u : 0x7f80u;
+                if ((which >> e & 1u) && (r[c][e >> 1] & m) == m) {
+                    r[c][e >> 1] &= e & 1 ? 0xffffu : 0xffff0000u;
+                    found |= 1u << e;
+                }
+            }
+        return found;
+    }
     __device__ __forceinline__ void parts(unsigned (&o)[1][4][2]) const {
 #pragma unroll
         for (int c = 0; c < 4; ++c) { o[0][c][0] = r[c][0]; o[0][c][1] = r[c][1]; }
@@ -201,6 +225,23 @@ template <> struct SvbtBlock<float> {
         for (int c = 0; c < 4; ++c)
 #pragma unroll
             for (int e = 0; e < 4; ++e) r[c][e] = seen >> e & 1 ? r[c][e] : 0.f;
+    }
+    __device__ __forceinline__ unsigned clear_bad(unsigned which) {
+        unsigned most = 0u, found = 0u;
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) most = max(most, __float_as_uint(r[c][e]) & 0x7fffffffu);
+        if (!svbt_bad(__uint_as_float(most))) return 0u;
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if ((which >> e & 1u) && svbt_bad(r[c][e])) {
+                    r[c][e] = 0.f;
+                    found |= 1u << e;
+                }
+        return found;
     }
     __device__ __forceinline__ void parts(unsigned (&o)[3][4][2]) const {
 #pragma unroll
@@ -269,6 +310,22 @@ struct SvbtTile {
             }
         }
     }
+    // Causal tiles on the diagonal hold keys that only some of the workgroup's queries see.  Their weight is 0 for the others, but 0 times
+    // an infinity or NaN is NaN: such elements of positions >= from become zero, and their positions' bits, counted from `from`, are set in
+    // bad[] (LDS).  svbt_add_bad then gives them to the queries that see them.
+    __device__ __forceinline__ void clear_bad(int j0, int from, unsigned* bad) {
+#pragma unroll
+        for (int i = 0; i < NB; ++i) {
+            const int id = tid + i * NT, j = j0 + pos(id);
+            if (BLOCKS % NT != 0 && id >= BLOCKS) continue;
+            unsigned found = b[i].clear_bad(from <= j ? 15u : from < j + 4 ? 15u << (from - j) & 15u : 0u);
+            while (found) {
+                const int n = j + __builtin_ctz(found) - from;
+                found &= found - 1;
+                atomicOr(bad + (n >> 5), 1u << (n & 31));
+            }
+        }
+    }
     template <bool ROWS, bool COLS>
     __device__ __forceinline__ void store(char* rows, char* cols) const {
 #pragma unroll
@@ -315,6 +372,25 @@ struct SvbtTile {
         }
     }
 };
+
+// What clear_bad took out of a tile's columns, added to the sums o[] of the query at position p where it sees them.  base, sc: the rows that
+// were staged; from: the key of bit 0 of bad[].  (twice: beyond the largest bf16 that is infinite too)  Rare, and then a memory latency a key.
+template <typename T, int NDB>
+__device__ __forceinline__ void svbt_add_bad(f32x16 (&o)[NDB], const unsigned* bad, int words, const T* base, long long sc, int dk, int from, int p, int kb) {
+#pragma unroll 1
+    for (int w = 0; w < words; ++w)
+#pragma unroll 1
+        for (unsigned bits = bad[w]; bits; bits &= bits - 1) {
+            const int j = from + 32 * w + __builtin_ctz(bits);
+#pragma unroll
+            for (int d = 0; d < NDB; ++d)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    const float x = svbt_load(base + (min(32 * d + svbt_row(r, kb), dk - 1) * sc + j));
+                    o[d][r] += j <= p && svbt_bad(x) ? x + x : 0.f;
+                }
+        }
+}
 
 // ---- positions and masks -----------------------------------------------------------------------------------------------------
 // position of query 0 of batch entry b; far beyond any key it makes no difference how far

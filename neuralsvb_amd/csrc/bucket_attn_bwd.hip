@@ -138,10 +138,12 @@ __global__ __launch_bounds__(256, SvbtParts<T>::NS == 1 || DKP <= 64 ? 2 : 1) vo
     const float lse = has ? a.lse[row] : SVBT_INF;
 
     const int span = (2 * (R + SVBT_PAD) + 1 + 3) & ~3;
-    float* s_bias = (float*)(smem + (DOUBLE ? 2 : 1) * BUF);
+    unsigned* s_bad = (unsigned*)(smem + (DOUBLE ? 2 : 1) * BUF);        // [SVBT_BAD_WORDS]
+    float* s_bias = (float*)(s_bad + SVBT_BAD_WORDS);
     float* s_skew = s_bias + span;                                      // [4][32][SVBT_SKEW_P]
     float* s_diag = s_skew + 4 * 32 * SVBT_SKEW_P;                       // [4][span], by offset + R + PAD; then [2][4] far sums
     svbt_fill_bias(s_bias, a, h, R, 256);
+    if (threadIdx.x < SVBT_BAD_WORDS) s_bad[threadIdx.x] = 0u;
     if (g.part)
         for (int e = threadIdx.x; e < 4 * span; e += 256) s_diag[e] = 0.f;
     float *my_skew = s_skew + wave * 32 * SVBT_SKEW_P, *my_diag = s_diag + wave * span + R + SVBT_PAD;
@@ -150,6 +152,7 @@ __global__ __launch_bounds__(256, SvbtParts<T>::NS == 1 || DKP <= 64 ? 2 : 1) vo
     if (a.causal) end = max(0, min(end, start + min(i0 + 128, a.Tq)));
     const int p0 = start + i0 + wave * 32, p1 = p0 + 31, p = start + i;
     const int tiles = (end + KT - 1) / KT;
+    const int part = a.causal ? start + i0 + 1 : 0x7fffffff;            // from here on a key is hidden from some of the queries here
     const float c = a.scale * SVBT_LOG2E;
 
     f32x16 acc[NDB];
@@ -165,9 +168,16 @@ __global__ __launch_bounds__(256, SvbtParts<T>::NS == 1 || DKP <= 64 ? 2 : 1) vo
         tk.settle(t * KT, a.Tk, m);
         tv.settle(t * KT, a.Tk, m);
         char* buf = smem + (DOUBLE ? (t & 1) * BUF : 0);
-        tk.template store<true, true>(buf, buf + 2 * NS * Tile::ROWS_BYTES);
         tv.template store<true, false>(buf + NS * Tile::ROWS_BYTES, nullptr);
+        // (rows as they are: a score that is not finite stays with its pair)
+        const bool some = t * KT + KT > part;                           // (uniform)
+        if (NS == 1 || some) {
+            tk.template store<true, false>(buf, nullptr);
+            if (some) tk.clear_bad(t * KT, part, s_bad);
+            tk.template store<false, true>(nullptr, buf + 2 * NS * Tile::ROWS_BYTES);
+        } else tk.template store<true, true>(buf, buf + 2 * NS * Tile::ROWS_BYTES);   // (cuts each value once)
     };
+    if (KT > part) __syncthreads();                                     // (uniform; s_bad is zero, for later tiles behind their barriers)
     if (tiles > 0) {
         seen = bits(0);
         put(0);
@@ -267,7 +277,10 @@ __global__ __launch_bounds__(256, SvbtParts<T>::NS == 1 || DKP <= 64 ? 2 : 1) vo
             if (lane == 0) part[e] = t;
         }
     }
-    if (!has || !g.dq) return;
+    if (!g.dq) return;
+    const uint4 bad = *reinterpret_cast<const uint4*>(s_bad);
+    if ((bad.x | bad.y | bad.z | bad.w) != 0u) svbt_add_bad<T, NDB>(acc, s_bad, SVBT_BAD_WORDS, k, a.k_sc, a.dk, part, p, kb);
+    if (!has) return;
     T* dq = (T*)g.dq + head + i;
 #pragma unroll
     for (int d = 0; d < NDB; ++d)
@@ -481,7 +494,7 @@ template <typename T, int DKP, int KT, bool DOUBLE, bool TINY = false>
 static int dq_launch(const SvbBucketAttn* a, const SvbBattnBwd& g, hipStream_t st) {
     typedef SvbtTile<T, DKP, KT, 256, TINY, false> Tile;
     const int span = svbt_span(a->buckets), qtiles = (a->Tq + 127) / 128;
-    const int lds = (DOUBLE ? 2 : 1) * Tile::NS * (2 * Tile::ROWS_BYTES + Tile::COLS_BYTES) + (g.part ? 5 * span + 4 * 32 * SVBT_SKEW_P + 8 : span) * 4;
+    const int lds = (DOUBLE ? 2 : 1) * Tile::NS * (2 * Tile::ROWS_BYTES + Tile::COLS_BYTES) + (SVBT_BAD_WORDS + (g.part ? 5 * span + 4 * 32 * SVBT_SKEW_P + 8 : span)) * 4;
     auto* kern = svb_bucket_attn_dq_kernel<T, DKP, KT, DOUBLE, TINY>;
     if (bwd_lds(kern, lds)) return SVB_ERR_LAUNCH;
     hipLaunchKernelGGL(kern, dim3((unsigned)(a->B * a->H * qtiles)), dim3(256), lds, st, *a, g, qtiles);

@@ -106,14 +106,17 @@ __global__ __launch_bounds__(256, SvbtParts<T>::NS == 3 && DKP == 128 ? 1 : 2) v
     own.load(q, a.q_sc, has ? i : 0, kb, a.dk);
     const int start = svbt_start(a, b);
     const int R = svb_bucket_reach(a.buckets);
-    float* s_bias = (float*)(smem + (DOUBLE ? 2 : 1) * BUF);
+    unsigned* s_bad = (unsigned*)(smem + (DOUBLE ? 2 : 1) * BUF);        // [SVBT_BAD_WORDS]
+    float* s_bias = (float*)(s_bad + SVBT_BAD_WORDS);
     svbt_fill_bias(s_bias, a, h, R, 256);
+    if (threadIdx.x < SVBT_BAD_WORDS) s_bad[threadIdx.x] = 0u;
 
     // keys that anyone here sees end at `end`; this wave's queries are at positions p0 .. p1
     int end = keep ? svbt_keep_end(keep, a.Tk, lane) : a.Tk;
     if (a.causal) end = max(0, min(end, start + min(i0 + 32 * QW, a.Tq)));
     const int p0 = start + i0 + qw * 32, p1 = p0 + 31, p = start + i;
     const int tiles = (end + KT - 1) / KT;
+    const int part = a.causal ? start + i0 + 1 : 0x7fffffff;            // from here on a key is hidden from some of the queries here
     svbt_bf16x8 qf[NK][NS];
     own.frags(kb, a.dk, has, qf);
 
@@ -132,10 +135,12 @@ __global__ __launch_bounds__(256, SvbtParts<T>::NS == 3 && DKP == 128 ? 1 : 2) v
         const unsigned long long m = seen[0] == ALL ? ~0ull : seen[0];
         tk.settle(t * KT, a.Tk, m, seen[NB64 - 1] | ~ALL);
         tv.settle(t * KT, a.Tk, m, seen[NB64 - 1] | ~ALL);
+        if (t * KT + KT > part) tv.clear_bad(t * KT, part, s_bad);       // (uniform)
         char* buf = smem + (DOUBLE ? (t & 1) * BUF : 0);
         tk.template store<true, false>(buf, nullptr);
         tv.template store<false, true>(nullptr, buf + NS * Tile::ROWS_BYTES);
     };
+    if (KT > part) __syncthreads();                                     // (uniform; s_bad is zero, for later tiles behind their barriers)
     if (tiles > 0) put(0);
     __syncthreads();
     const float past = s_bias[0], ahead = s_bias[2 * (R + SVBT_PAD)];
@@ -230,6 +235,8 @@ __global__ __launch_bounds__(256, SvbtParts<T>::NS == 3 && DKP == 128 ? 1 : 2) v
     }
     const float l = st.l + __shfl_xor(st.l, 32, 64);
     const float inv = l > 0.f ? 1.f / l : 0.f;                          // (no key: zeros)
+    const uint4 bad = *reinterpret_cast<const uint4*>(s_bad);
+    if ((bad.x | bad.y | bad.z | bad.w) != 0u) svbt_add_bad<T, NDB>(st.o, s_bad, SVBT_BAD_WORDS, v, a.v_sc, a.dk, part, p, kb);
     if (!has) return;
     const size_t head = ((size_t)b * a.H + h) * a.dk;
     T* out = (T*)a.out + head * a.Tq + i;
@@ -326,6 +333,15 @@ template <typename T> struct SvbFewValues;
 template <> struct SvbFewValues<unsigned short> {
     unsigned r[4];
     __device__ __forceinline__ void load(const unsigned short* p) { __builtin_memcpy(r, p, 16); }
+    __device__ __forceinline__ unsigned bad() const {                   // the bits of those that are not finite
+        unsigned found = 0u;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const unsigned m = e & 1 ? 0x7f800000u : 0x7f80u;
+            found |= (r[e >> 1] & m) == m ? 1u << e : 0u;
+        }
+        return found;
+    }
     template <bool FULL>
     __device__ __forceinline__ void frag(unsigned seen, svbt_bf16x8 (&f)[1]) const {
         unsigned u[4];
@@ -338,6 +354,12 @@ template <> struct SvbFewValues<unsigned short> {
 template <> struct SvbFewValues<float> {
     float r[8];
     __device__ __forceinline__ void load(const float* p) { __builtin_memcpy(r, p, 32); }
+    __device__ __forceinline__ unsigned bad() const {
+        unsigned found = 0u;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) found |= svbt_bad(r[e]) ? 1u << e : 0u;
+        return found;
+    }
     template <bool FULL>
     __device__ __forceinline__ void frag(unsigned seen, svbt_bf16x8 (&f)[3]) const {
         float v[8];
@@ -405,6 +427,8 @@ __global__ __launch_bounds__(256, DKP * SvbtParts<T>::NS > 192 || DKP == 128 ? 1
     const float* tab = s_tab + hl * nb;
     const float past = tab[s_idx[0]], ahead = tab[s_idx[2 * R]];
 
+    unsigned bad = 0u;                                                  // of keys start + 1 ..: those that svbt_add_bad adds below
+
     auto tile = [&](int t, auto full_c) {
         constexpr bool FULL = decltype(full_c)::value;                   // 64 keys, all of them seen by every row
         const int j0 = FULL ? 64 * t : min(64 * t, a.Tk - 64);
@@ -439,6 +463,10 @@ __global__ __launch_bounds__(256, DKP * SvbtParts<T>::NS > 192 || DKP == 128 ? 1
                 if (!FULL) s[u][r] = ((r < 8 ? w0 : w1) >> (key & 31) & 1u) && !(a.causal && o > 0) ? s[u][r] : -SVBT_INF;
             }
         svbt_softmax<2, NDB>(s, st);
+        // keys that only some of the rows see: as SvbtTile::clear_bad
+        unsigned long long some = 0ull;
+        if (!FULL && a.causal && a.Tq > 1 && j0 + 63 > start) some = start + 1 <= j0 ? seen : seen & ~0ull << (start + 1 - j0);      // (uniform)
+        unsigned found[2] = {0u, 0u};
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
             float w[8];
@@ -448,10 +476,20 @@ __global__ __launch_bounds__(256, DKP * SvbtParts<T>::NS > 192 || DKP == 128 ? 1
             svbt_frag8<NS>(w, pf);
 #pragma unroll
             for (int d = 0; d < NDB; ++d) {
+                unsigned sees = (unsigned)(seen >> (16 * g + 8 * kb)) & 0xffu;
+                if (!FULL && some != 0ull) {
+                    const unsigned n = vt[g][d].bad() & (unsigned)(some >> (16 * g + 8 * kb));
+                    found[g >> 1] |= (n & 0xffu) << (16 * (g & 1) + 8 * kb);
+                    sees &= ~n;
+                }
                 svbt_bf16x8 f[NS];
-                vt[g][d].template frag<FULL>((unsigned)(seen >> (16 * g + 8 * kb)), f);
+                vt[g][d].template frag<FULL>(sees, f);
                 svbt_mma<NS, false>(st.o[d], f, pf);
             }
+        }
+        if (!FULL && some != 0ull) {
+            const unsigned long long m = (unsigned long long)found[1] << 32 | found[0];
+            bad |= (unsigned)(start + 1 <= j0 ? m << (j0 - start - 1) : m >> (start + 1 - j0));       // (keys up to start + 31)
         }
         if (NS == 1 && t + 1 < t1) load_v(t + 1);
     };
@@ -462,6 +500,11 @@ __global__ __launch_bounds__(256, DKP * SvbtParts<T>::NS > 192 || DKP == 128 ? 1
         for (int t = t0; t < whole; ++t) tile(t, std::true_type{});
     for (int t = whole; t < t1; ++t) tile(t, std::false_type{});
     st.l += __shfl_xor(st.l, 32, 64);
+    if (a.causal && a.Tq > 1) {                                         // (uniform)
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) bad |= __shfl_xor(bad, o, 64);
+        svbt_add_bad<T, NDB>(st.o, &bad, 1, v, a.v_sc, a.dk, start + 1, p, kb);
+    }
 
     // join of the four waves
     __syncthreads();                                                    // (the tables are read)
@@ -542,7 +585,7 @@ int svb_bucket_attn_check(const SvbBucketAttn* a) {
 template <typename T, int DKP, int KT, bool DOUBLE, int PP, int KG, bool TINY = false>
 static int fwd_launch(const SvbBucketAttn* a, hipStream_t st) {
     typedef SvbtTile<T, DKP, KT, 256, TINY, DKP == 128> Tile;
-    const int lds = (DOUBLE ? 2 : 1) * Tile::NS * (Tile::ROWS_BYTES + Tile::COLS_BYTES) + svbt_span(a->buckets) * 4;
+    const int lds = (DOUBLE ? 2 : 1) * Tile::NS * (Tile::ROWS_BYTES + Tile::COLS_BYTES) + (SVBT_BAD_WORDS + svbt_span(a->buckets)) * 4;
     auto* kern = svb_bucket_attn_fwd_kernel<T, DKP, KT, DOUBLE, PP, KG, TINY>;
     if (lds > 65536 && hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024) != hipSuccess) return SVB_ERR_LAUNCH;
     constexpr int ROWS = 128 / KG;

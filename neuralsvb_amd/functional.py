@@ -1002,7 +1002,7 @@ def bucket_attention(q, k, v, table, buckets, n_head, keep=None, causal=False, s
     q [B, H dk, Tq], k, v [B, Hkv dk, Tk] (float32 or bfloat16; any batch and channel strides, e.g. slices of one projection),
     H = n_head a multiple of Hkv: query head h reads key / value head h // (H / Hkv).  dk <= 128.  table [n_buckets, H], float32 or
     bfloat16.  keep [B, Tk] float32: 0 hides a key, and whatever k and v hold there has no influence.  causal: a query sees the keys
-    up to its own position.  scale: 1 / sqrt(dk).  q_start: position of query 0 among the keys, an int or an int32 tensor [B] (default
+    up to its own position, and whatever k and v hold at later ones has no influence on it.  scale: 1 / sqrt(dk).  q_start: position of query 0 among the keys, an int or an int32 tensor [B] (default
     Tk - Tq); with causal=True and Tq = 1 a tensor of cached lengths - 1 serves one new token per request from caches of one capacity.
     A query that sees no key gives zeros and no gradient.  -> [B, H dk, Tq].
 

@@ -249,6 +249,7 @@ static inline int __builtin_amdgcn_readfirstlane_emu(int v) { return emu_shfl_fr
 static inline float atomicAdd(float* p, float v) { float o = *p; *p = o + v; return o; }
 static inline int atomicAdd(int* p, int v) { int o = *p; *p = o + v; return o; }
 static inline unsigned atomicAdd(unsigned* p, unsigned v) { unsigned o = *p; *p = o + v; return o; }
+static inline unsigned atomicOr(unsigned* p, unsigned v) { unsigned o = *p; *p = o | v; return o; }
 
 static inline float __fdividef(float a, float b) { return a / b; }
 static inline double __dadd_rn(double a, double b) { volatile double r = a + b; return r; }   /* (volatile: no contraction) */

@@ -1,0 +1,100 @@
+"""LayerNorm over channels, the bias by buckets and the attention with it, where their promises are hardest to keep: values that are not
+finite, rows with nearly all their weight on one key, gradients that are not offered, strides and sizes at the limits."""
+import math
+
+import pytest
+import torch
+
+from neuralsvb_amd import functional as SF
+from tests.test_attention_block import DT, U32, UBF, bucket_index, case, leaves64, near
+
+_dt = pytest.mark.parametrize("dt", ["f32", "bf16"])
+
+
+def attention_by_rows(q, k, v, table, buckets, n_head, keep=None, causal=False, q_start=None):
+    """The definition in 64 bits, each query over the keys that it sees and no others: what is hidden from it is not even read."""
+    B, D, tq = q.shape
+    tk, dk = k.shape[2], D // n_head
+    g = n_head // (k.shape[1] // dk)
+    q, k, v, table = q.double(), k.double(), v.double(), table.double()
+    out = []
+    for b in range(B):
+        start = tk - tq if q_start is None else int(q_start[b])
+        idx = bucket_index(buckets, tq, tk, start)
+        see = torch.ones(tq, tk, dtype=torch.bool) if keep is None else (keep[b] != 0)[None].expand(tq, tk)
+        if causal:
+            see = see & (torch.arange(tk)[None] <= start + torch.arange(tq)[:, None])
+        for h in range(n_head):
+            ks, vs = k[b, h // g * dk:(h // g + 1) * dk], v[b, h // g * dk:(h // g + 1) * dk]
+            rows = []
+            for i in range(tq):
+                at = torch.nonzero(see[i])[:, 0]
+                s = q[b, h * dk:(h + 1) * dk, i] @ ks[:, at] * dk ** -0.5 + table[idx[i, at], h]
+                rows.append(vs[:, at] @ torch.softmax(s, 0) if len(at) else torch.zeros(dk, dtype=torch.float64))
+            out.append(torch.stack(rows, 1))
+    return torch.cat(out).reshape(B, D, tq)
+
+
+def like(got, want, tol, what):
+    """NaN or infinite exactly where the definition is, and near it (2-norm) elsewhere."""
+    got, want = got.detach().double().cpu(), want.detach()
+    assert torch.equal(torch.isfinite(got), torch.isfinite(want)), what
+    near(torch.nan_to_num(got, 0.0, 0.0, 0.0), torch.nan_to_num(want, 0.0, 0.0, 0.0), tol, what)
+
+
+# ---- keys that only some queries see ---------------------------------------------------------------------------------------
+# (Tq, Tk, start): tokens over a cache (few rows), whole tiles of queries, keys of a tile over two waves (bf16), rows of less than 4 elements,
+# queries ahead of the keys, a diagonal that crosses several tiles of keys
+DIAGONALS = [(4, 70, 60), (4, 200, 196), (40, 90, 50), (70, 300, 230), (3, 3, 0), (50, 40, -10), (150, 280, 101)]
+
+
+@_dt
+@pytest.mark.parametrize("shape", DIAGONALS)
+def test_hidden_keys_may_hold_anything(dev, dt, shape):
+    """NaN and infinities in keys and values reach the queries that see them, and no other (causal: a later key is hidden)."""
+    tq, tk, start = shape
+    bk = SF.RelativeBuckets(16, 24, False)
+    q, k, v, table, do = case(tq + tk, dt, 2, 2, 1, 24, tq, tk)
+    starts = torch.tensor([start, start - 1], dtype=torch.int32)
+    first = max(start, 0)                                                # (the last rows see them all, the first rows none of them)
+    for n, (c, value) in enumerate(((3, math.nan), (23, math.inf), (0, -math.inf))):
+        j = min(tk - 1, first + 1 + n * tq // 3)
+        v[:, c, j] = value
+    v[1, 5, tk - 1] = math.nan
+    tol = 3 * UBF if dt == "bf16" else 128 * U32
+    keep = torch.ones(2, tk)
+    keep[:, 2::5] = 0
+    for mask in (None, keep):
+        want = attention_by_rows(q, k, v, table, bk, 2, mask, True, starts)
+        assert mask is not None or not torch.isfinite(want).all()
+        m = None if mask is None else mask.to(dev)
+        with torch.no_grad():
+            like(SF.bucket_attention(*(t.to(dev) for t in (q, k, v, table)), bk, 2, keep=m, causal=True, q_start=starts.to(dev)), want, tol, "values")
+        leaves = [t.clone().to(dev).requires_grad_() for t in (q, k, v, table)]
+        like(SF.bucket_attention(*leaves, bk, 2, keep=m, causal=True, q_start=starts.to(dev)), want, tol, "values, recorded")
+    k[:, 4, min(tk - 1, first + 1 + tq // 2)] = math.nan                  # (and a key)
+    want = attention_by_rows(q, k, v, table, bk, 2, None, True, starts)
+    with torch.no_grad():
+        like(SF.bucket_attention(*(t.to(dev) for t in (q, k, v, table)), bk, 2, causal=True, q_start=starts.to(dev)), want, tol, "keys")
+
+
+@_dt
+@pytest.mark.parametrize("shape", [(40, 90, 50), (5, 70, 60), (3, 3, 0), (150, 150, 0)])
+def test_hidden_keys_and_the_query_gradient(dev, dt, shape):
+    """dq of a query that sees none of the keys that are not finite is that of the definition."""
+    tq, tk, start = shape
+    bk = SF.RelativeBuckets(16, 24, False)
+    q, k, v, table, do = case(tq + tk, dt, 1, 2, 1, 24, tq, tk)
+    starts = torch.tensor([start], dtype=torch.int32)
+    bad = start + tq // 2
+    for what in ("k", "v"):
+        kv = {"k": k.clone(), "v": v.clone()}
+        kv[what][0, 7, bad] = math.nan
+        kv[what][0, 8, min(tk - 1, bad + 1)] = math.inf
+        clean = leaves64(q, *(torch.nan_to_num(kv[m], 0.0, 0.0, 0.0) for m in "kv"), table)
+        want, = torch.autograd.grad(attention_by_rows(*clean, bk, 2, None, True, starts), clean[0], do.double())
+        leaves = [t.clone().to(dev).requires_grad_() for t in (q, kv["k"], kv["v"], table)]
+        dq, = torch.autograd.grad(SF.bucket_attention(*leaves, bk, 2, causal=True, q_start=starts.to(dev)), leaves[0], do.to(dev))
+        n = bad - start                                                  # queries before the bad key
+        near(dq[:, :, :n], want[:, :, :n], 3 * UBF if dt == "bf16" else 128 * U32, what)
+        assert not torch.isfinite(dq[:, :, n:]).all(1).any(), what       # (and of the others it is not finite)
