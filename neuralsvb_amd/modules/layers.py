@@ -120,8 +120,8 @@ class LinearNCT(nn.Module):
 
 
 class LayerNormNCT(nn.Module):
-    """nn.LayerNorm(C) parameters, applied over the channel dim of [B, C, T] (functional.layer_norm_nct: differentiable; the frozen PPG
-    encoder runs it without gradients)."""
+    """nn.LayerNorm(C) parameters, applied over the channel dim of [B, C, T] (functional.layer_norm_nct: differentiable by itself; the
+    PPG encoder that holds these has parts without a gradient, which refuse to be trained)."""
 
     def __init__(self, channels, eps=1e-5):
         super().__init__()

@@ -51,6 +51,12 @@ POS_IN_KERNEL = True     # frozen encoder, d_k = 64: position scores computed in
 FUSE_QKV = True          # frozen encoder: one D -> 4D projection instead of three + an add (see RelPositionMultiHeadedAttention.forward)
 
 
+def _forward_only(what, *tensors):
+    """Kernels without a gradient follow: refuse a call that wants one, which would come out without their paths."""
+    if any(t.requires_grad for t in tensors):
+        raise RuntimeError(f"{what} is forward-only (frozen encoder): its input or parameters require a gradient")
+
+
 class RelPositionMultiHeadedAttention(nn.Module):
     def __init__(self, n_head, n_feat):
         super().__init__()
@@ -101,9 +107,10 @@ class RelPositionMultiHeadedAttention(nn.Module):
         residual: added to the result in the output projection's epilogue (the block's `x + self_attn(...)`)."""
         B, D, T = x.shape
         h, dk = self.h, self.d_k
-        frozen = not (torch.is_grad_enabled() and (x.requires_grad or self.pos_bias_u.requires_grad
-                                                   or self.linear_q.weight.requires_grad))
-        if frozen and FUSE_QKV and POS_IN_KERNEL and dk == 64:
+        if torch.is_grad_enabled():
+            _forward_only("rel-pos attention", x, self.pos_bias_u, self.pos_bias_v, *self.linear_q.parameters(),
+                          *self.linear_k.parameters(), *self.linear_v.parameters(), *self.linear_pos.parameters())
+        if FUSE_QKV and POS_IN_KERNEL and dk == 64:
             # ... and the position scores inside the attention kernel: no [B,h,T,T] tensor, no GEMM (round 4)
             w4, b4, w3, b3 = self._fused_qkv()
             with SF.precision_scope(self.linear_q.precision):
@@ -112,7 +119,7 @@ class RelPositionMultiHeadedAttention(nn.Module):
             o = K.relpos_attention_pos(y[:, :D], y[:, D:2 * D], y[:, 2 * D:], self.pos_bias_u.contiguous(),
                                        self.pos_bias_v.contiguous(), pt_hi, pt_lo, mask.float().contiguous(), 1.0 / math.sqrt(dk), h)
             return self.linear_out(o, residual=residual)
-        if frozen and FUSE_QKV:
+        if FUSE_QKV:
             # frozen encoder: q, k, v and q + pos_bias_v as ONE 1x1 conv D -> 4D (the three projections read the same x; the
             # fourth block is linear_q again with pos_bias_v folded into its bias), the position projection of the (constant)
             # position embedding cached per length
@@ -130,7 +137,7 @@ class RelPositionMultiHeadedAttention(nn.Module):
             q_v = (q4 + self.pos_bias_v[None, :, :, None]).transpose(-1, -2)
         bd = torch.matmul(q_v, p)                                   # [B,h,T,T] position scores, unshifted
         scale = 1.0 / math.sqrt(dk)
-        if dk == 64 and frozen:
+        if dk == 64:
             # frozen encoder (the hot path): content scores, rel_shift (:125-148), scale, key mask, softmax and the value
             # product in ONE kernel -- neither `ac` nor `attn` ([B,h,T,T] each) is ever written
             o = K.relpos_attention(q, k, v, self.pos_bias_u.contiguous(), bd, mask.float().contiguous(), scale, h)
@@ -191,6 +198,8 @@ class ConvolutionModule(nn.Module):
             x = x * torch.sigmoid(x)
         else:                                            # GLU + depthwise k31 + folded BatchNorm + Swish: one HIP kernel
             dw, bn = self.depthwise_conv, self.norm
+            if torch.is_grad_enabled():
+                _forward_only("conv module in eval mode", y, *dw.parameters(), *bn.parameters())
             x = K.glu_dwconv_bn_swish(y.contiguous(), dw.weight, dw.bias, bn.weight, bn.bias, bn.running_mean, bn.running_var,
                                       bn.eps)
         return self.pointwise_conv2(x, residual=residual)

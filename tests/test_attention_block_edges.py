@@ -98,3 +98,44 @@ def test_hidden_keys_and_the_query_gradient(dev, dt, shape):
         n = bad - start                                                  # queries before the bad key
         near(dq[:, :, :n], want[:, :, :n], 3 * UBF if dt == "bf16" else 128 * U32, what)
         assert not torch.isfinite(dq[:, :, n:]).all(1).any(), what       # (and of the others it is not finite)
+
+
+# ---- the frozen encoder beside the trainable operators ---------------------------------------------------------------------
+@pytest.mark.parametrize("mode", ["train", "eval"])
+@pytest.mark.parametrize("heads", [4, 1])                                # (one head of 64: the fused attention kernel)
+def test_frozen_encoder_refuses_gradients(dev, mode, heads):
+    """Its attention, and in eval mode its conv module, have no gradient: a call that wants one is an error, not a gradient without them."""
+    from neuralsvb_amd.modules.vc_asr import ConformerLayers, ConvolutionModule, RelPositionMultiHeadedAttention
+    size = 64 if heads == 1 else 32
+    enc = getattr(ConformerLayers(size, 1, 7, heads).to(dev), mode)()
+    x = torch.randn(2, size, 20, generator=torch.Generator().manual_seed(51)).to(dev)
+    with pytest.raises(RuntimeError, match="forward-only"):
+        enc(x)
+    for p in enc.parameters():
+        p.requires_grad_(False)
+    frozen = enc(x)                                                      # (gradients enabled, none wanted)
+    assert not frozen.requires_grad
+    with pytest.raises(RuntimeError, match="forward-only"):
+        enc(x.clone().requires_grad_())
+    attn = enc.encoder_layers[0].self_attn
+    for p in (attn.linear_q.bias, attn.linear_k.weight, attn.linear_pos.weight, attn.pos_bias_v):
+        p.requires_grad_()
+        with pytest.raises(RuntimeError, match="forward-only"):
+            enc(x)
+        with torch.no_grad():
+            assert torch.equal(enc(x), frozen) or mode == "train"         # (train: BatchNorm statistics move)
+        p.requires_grad_(False)
+    conv = enc.encoder_layers[0].conv_module
+    if mode == "eval":
+        for p in (conv.pointwise_conv1.weight, conv.depthwise_conv.bias, conv.norm.weight):
+            p.requires_grad_()
+            with pytest.raises(RuntimeError, match="forward-only"):
+                conv(x)
+            p.requires_grad_(False)
+    # behind the last of them gradients flow
+    last = enc.encoder_layers[0].norm_final
+    last.bias.requires_grad_()
+    do = torch.randn(2, size, 20, generator=torch.Generator().manual_seed(52)).to(dev)
+    out = enc.encoder_layers[0](x, enc._pos_emb(20, dev), torch.ones(2, 20, dtype=torch.bool, device=dev))
+    g, = torch.autograd.grad(out, last.bias, do)
+    near(g, do.double().cpu().sum((0, 2)), 8 * U32 * (math.sqrt(40) + 4), "bias of the last norm")
