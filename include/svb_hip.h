@@ -595,14 +595,15 @@ int svb_bucket_bias_bwd(const void* dbias, void* dtable, const SvbRelBuckets* bu
  * Shared heads: H query heads use Hkv key / value heads, query head h reads head h / (H / Hkv).
  * q [B][H dk][Tq], k, v [B][Hkv dk][Tk]: unit time stride, any batch stride, channel stride 0 ... 2^25 (elements).  dk <= 128.
  * out, dout, dq [B][H dk][Tq], dk, dv [B][Hkv dk][Tk] contiguous.  table, dtable [n_buckets][H] (table_dtype).
- * Training: lse [B][H][Tq] and out_f32 (bf16 tensors only: out before its rounding, [B][H dk][Tq]) are written by the forward and
- * read by the backward; both NULL for inference.                                                                                  */
+ * Training: stats [2][B][H][Tq] (each query's maximum in log2 units, +infinity where it sees no key, and the reciprocal of its sum)
+ * and out_f32 (bf16 tensors only: out before its rounding, [B][H dk][Tq]) are written by the forward and read by the backward; both
+ * NULL for inference.                                                                                                             */
 typedef struct SvbBucketAttn {
     const void *q, *k, *v, *table;
     const float* keep;          /* [B][Tk] or NULL */
     const int* q_start_b;       /* [B] or NULL */
     void* out;
-    float *lse, *out_f32;
+    float *stats, *out_f32;
     long long q_sb, q_sc, k_sb, k_sc, v_sb, v_sc;
     int B, H, Hkv, dk, Tq, Tk, q_start, causal, dtype, table_dtype;
     float scale;
@@ -613,7 +614,7 @@ typedef struct SvbBucketAttnGrad {
     void *d_q, *d_k, *d_v, *d_table; /* each may be NULL (d_k and d_v both or neither) */
     float* ws;                  /* svb_bucket_attn_bwd_workspace_floats */
 } SvbBucketAttnGrad;
-/* ws may be NULL where svb_bucket_attn_fwd_workspace_floats says 0.  Few query rows and no lse: the keys are split over workgroups
+/* ws may be NULL where svb_bucket_attn_fwd_workspace_floats says 0.  Few query rows and no stats: the keys are split over workgroups
  * and joined (ws holds the parts); otherwise one launch of query tiles.                                                            */
 size_t svb_bucket_attn_fwd_workspace_floats(const SvbBucketAttn* a);
 int svb_bucket_attn_fwd(const SvbBucketAttn* a, float* ws, void* stream);

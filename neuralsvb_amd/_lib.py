@@ -87,7 +87,7 @@ class SvbRelBuckets(C.Structure):
 
 
 class SvbBucketAttn(C.Structure):
-    _fields_ = ([(n, C.c_void_p) for n in ("q", "k", "v", "table", "keep", "q_start_b", "out", "lse", "out_f32")] +
+    _fields_ = ([(n, C.c_void_p) for n in ("q", "k", "v", "table", "keep", "q_start_b", "out", "stats", "out_f32")] +
                 [(n, C.c_longlong) for n in ("q_sb", "q_sc", "k_sb", "k_sc", "v_sb", "v_sc")] +
                 [(n, C.c_int) for n in ("B", "H", "Hkv", "dk", "Tq", "Tk", "q_start", "causal", "dtype", "table_dtype")] +
                 [("scale", C.c_float), ("buckets", SvbRelBuckets)])

@@ -68,7 +68,7 @@ __device__ __forceinline__ void svbt_frag8(const float* v, svbt_bf16x8 (&f)[NS])
     for (int n = 0; n < NS; ++n) __builtin_memcpy(&f[n], u[n], 16);
 }
 // acc += A B.  `FLIP` issues the two mixed orders of three-part operands the other way round, so that A B and (B^T A^T)^T are equal
-// bit for bit: the backward recomputes the scores in both orientations and compares them with one log-sum.
+// bit for bit: the backward recomputes the scores in both orientations and compares them with the forward's maximum.
 template <int NS, bool FLIP>
 __device__ __forceinline__ void svbt_mma(f32x16& acc, const svbt_bf16x8 (&a)[NS], const svbt_bf16x8 (&b)[NS]) {
     if constexpr (NS == 3) {

@@ -1,6 +1,6 @@
 // bucket_attn_bwd.hip -- gradients of the attention with a learned relative-position bias by buckets.
 //
-//   t_ij = log2(e) (scale q_i . k_j + bias),  P_ij = 2^(t_ij - lse_i)  (recomputed),  dP_ij = dout_i . v_j,  delta_i = dout_i . out_i
+//   t_ij = log2(e) (scale q_i . k_j + bias),  P_ij = 2^(t_ij - m_i) / l_i  (recomputed),  dP_ij = dout_i . v_j,  delta_i = dout_i . out_i
 //   dS_ij = P_ij (dP_ij - delta_i):   dv_j = sum_i P_ij dout_i,  dk_j = scale sum_i dS_ij q_i,  dq_i = scale sum_j dS_ij k_j,
 //   dtable[k][h] = sum of dS_ij over the pairs of bucket k
 //
@@ -15,7 +15,8 @@
 // Bound, as the forward, by what a wave does between its products, and in the second kernel by one wave per SIMD above dk 64 (its two sums
 // take 128 registers of each lane at dk 128): B2 H16/4 dk128 T2048 causal bf16 170 us (dq: three products, 303 TFLOP/s) and 170 us (dk, dv:
 // four, 404 TFLOP/s); B32 H4 dk64 T562 fp32 150 and 230 us (620 and 540 TFLOP/s of bf16 products).
-// A row whose weight is all on one key (P == 1) has dS = 0: dP - delta is then rounding noise alone.
+// P comes from the forward's maximum and sum as the forward had it: of a row with nearly all its weight on one key, dS of that key is what
+// the others' small weights leave.  Where 32 bits hold nothing of them (l == 1: P == 1) its dS is 0, dP - delta being rounding noise alone.
 //
 // dtable: dS of pairs further than the last bucket border is summed in registers.  Nearer pairs are summed along the diagonals of each
 // 32 x 32 sub-tile: the tile goes to LDS skewed, row (key - query) mod 32, which puts the diagonals d and d - 32 side by side into one row of
@@ -37,7 +38,7 @@ struct SvbBattnBwd {
 
 __device__ __forceinline__ float svbt_ds(float p, float dp, float delta) {
     const float ds = p * (dp - delta);
-    return p == 0.f || p == 1.f ? 0.f : ds;
+    return p == 0.f || p == 1.f ? 0.f : ds;                             // (p == 1: its row's sum is exactly 1)
 }
 
 // Adds a sub-tile's diagonal sums to diag[key - query], one wave.  s: register r is key svbt_row(r, kb) of query l31; skew: [32][36] floats
@@ -69,11 +70,11 @@ __device__ __forceinline__ void svbt_diag_add(float* skew, float* diag, const f3
     diag[kb ? l31 - 32 : l31] += kb ? there : here;                     // (64 different offsets)
 }
 
-// One sub-tile's scores -> dS in place; rows are keys, this lane's query has lse and delta.  NEAR: the bias varies; bias0: at row 0.
+// One sub-tile's scores -> dS in place; rows are keys, this lane's query has maximum m, 1 / sum inv and delta.  NEAR: the bias varies; bias0: at row 0.
 template <bool NEAR>
-__device__ __forceinline__ void svbt_weights_q(f32x16& s, const f32x16& dp, float c, const float* bias0, float flat, float lse, float delta) {
+__device__ __forceinline__ void svbt_weights_q(f32x16& s, const f32x16& dp, float c, const float* bias0, float flat, float m, float inv, float delta) {
 #pragma unroll
-    for (int r = 0; r < 16; ++r) s[r] = svbt_ds(__builtin_amdgcn_exp2f(fmaf(s[r], c, NEAR ? bias0[svbt_reg(r)] : flat) - lse), dp[r], delta);
+    for (int r = 0; r < 16; ++r) s[r] = svbt_ds(__builtin_amdgcn_exp2f(fmaf(s[r], c, NEAR ? bias0[svbt_reg(r)] : flat) - m) * inv, dp[r], delta);
 }
 
 // ---- dq, dtable, delta: 4 waves x 32 queries, keys staged ----------------------------------------------------------------------------
@@ -135,7 +136,7 @@ __global__ __launch_bounds__(256, SvbtParts<T>::NS == 1 || DKP <= 64 ? 2 : 1) vo
     delta += __shfl_xor(delta, 32, 64);
     if (has && kb == 0) g.delta[row] = delta;
     if (!g.dq && !g.part) return;                                       // (only delta is wanted; uniform)
-    const float lse = has ? a.lse[row] : SVBT_INF;
+    const float m = has ? a.stats[row] : SVBT_INF, inv = has ? a.stats[(size_t)a.B * a.H * a.Tq + row] : 0.f;
 
     const int span = (2 * (R + SVBT_PAD) + 1 + 3) & ~3;
     unsigned* s_bad = (unsigned*)(smem + (DOUBLE ? 2 : 1) * BUF);        // [SVBT_BAD_WORDS]
@@ -218,8 +219,8 @@ __global__ __launch_bounds__(256, SvbtParts<T>::NS == 1 || DKP <= 64 ? 2 : 1) vo
                 const unsigned su = (unsigned)(now >> (32 * u)) >> (4 * kb);
                 const int o0 = svbt_fresh(j0 + 32 * u + 4 * kb - p);     // offset of register row 0
                 const bool far = behind || before;
-                if (far) svbt_weights_q<false>(s, dp, c, nullptr, flat, lse, delta);
-                else svbt_weights_q<true>(s, dp, c, s_bias + (o0 + R + SVBT_PAD), flat, lse, delta);
+                if (far) svbt_weights_q<false>(s, dp, c, nullptr, flat, m, inv, delta);
+                else svbt_weights_q<true>(s, dp, c, s_bias + (o0 + R + SVBT_PAD), flat, m, inv, delta);
                 if (edge) {
 #pragma unroll
                     for (int r = 0; r < 16; ++r) s[r] = (su >> svbt_reg(r) & 1u) && !(a.causal && o0 + svbt_reg(r) > 0) ? s[r] : 0.f;
@@ -291,17 +292,18 @@ __global__ __launch_bounds__(256, SvbtParts<T>::NS == 1 || DKP <= 64 ? 2 : 1) vo
         }
 }
 
-// One sub-tile's scores -> P and dP -> dS, in place; rows are queries.  NEAR: the bias varies; bias0: at row 0.  ls, dl: log-sum and delta
-// of the sub-tile's rows from 4 kb on.
-template <bool NEAR>
-__device__ __forceinline__ void svbt_weights_kv(f32x16& s, f32x16& dp, float c, const float* bias0, float flat, const float* ls, const float* dl) {
+// One sub-tile's scores -> P and dP -> dS, in place; rows are queries.  NEAR: the bias varies; bias0: at row 0.  st: the sub-tile's
+// rows' maxima from 4 kb on, KT further their 1 / sum, 2 KT further their delta.
+template <bool NEAR, int KT>
+__device__ __forceinline__ void svbt_weights_kv(f32x16& s, f32x16& dp, float c, const float* bias0, float flat, const float* st) {
 #pragma unroll
     for (int r4 = 0; r4 < 4; ++r4) {
-        const float4 l = *reinterpret_cast<const float4*>(ls + 8 * r4), d = *reinterpret_cast<const float4*>(dl + 8 * r4);
+        const float4 m = *reinterpret_cast<const float4*>(st + 8 * r4), inv = *reinterpret_cast<const float4*>(st + KT + 8 * r4),
+                     d = *reinterpret_cast<const float4*>(st + 2 * KT + 8 * r4);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             const int r = 4 * r4 + e;
-            s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], c, NEAR ? bias0[-svbt_reg(r)] : flat) - l[e]);
+            s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], c, NEAR ? bias0[-svbt_reg(r)] : flat) - m[e]) * inv[e];
             dp[r] = svbt_ds(s[r], dp[r], d[e]);
         }
     }
@@ -314,7 +316,7 @@ __global__ __launch_bounds__(256, DKP <= (SvbtParts<T>::NS == 1 ? 64 : 32) ? 2 :
     // (FRESH: B16 H4 dk32 T700 bf16 62 -> 48 us, B8 H4 dk128 T562 fp32 206 -> 202; elsewhere it costs 0 to 3 %)
     typedef SvbtTile<T, DKP, KT, 256, TINY, SvbtParts<T>::NS == 1 ? DKP == 32 : DKP == 128> Tile;
     constexpr int NS = Tile::NS, NK = DKP / 16, NDB = DKP / 32, NSUB = KT / 32;
-    constexpr int TILE = NS * 2 * (Tile::ROWS_BYTES + Tile::COLS_BYTES), BUF = TILE + 2 * KT * 4;
+    constexpr int TILE = NS * 2 * (Tile::ROWS_BYTES + Tile::COLS_BYTES), BUF = TILE + 3 * KT * 4;
     HIP_DYNAMIC_SHARED(char, smem)
     const int lane = threadIdx.x & 63, wave = svb_uniform(threadIdx.x >> 6), l31 = lane & 31, kb = lane >> 5;
     int bk, ks;
@@ -342,31 +344,32 @@ __global__ __launch_bounds__(256, DKP <= (SvbtParts<T>::NS == 1 ? 64 : 32) ? 2 :
     const int tiles = max(0, (a.Tq + KT - 1) / KT - first);
     const float c = a.scale * SVBT_LOG2E;
     Tile tq(false), td(true);
-    float stat = 0.f, row_lse = 0.f;                                    // this thread's lse (threads < KT) or delta (KT .. 2 KT - 1); lane's lse
+    float stat = 0.f, row_max = 0.f;                                    // thread n KT + i: maximum, 1 / sum or delta of row i; the lane's row's maximum
     const int n0 = svb_uniform((int)((long long)G * tiles * split / g.splits)), n1 = svb_uniform((int)((long long)G * tiles * (split + 1) / g.splits));
     auto fetch = [&](int n) {
         const int hh = hk * G + svb_uniform(n / tiles), i0 = (first + n % tiles) * KT;
         const size_t hd = (size_t)b * a.H + hh;
         tq.load((const T*)a.q + b * a.q_sb + (long long)hh * a.dk * a.q_sc, a.q_sc, i0, a.Tq, a.dk);
         td.load((const T*)g.dout + hd * a.dk * a.Tq, a.Tq, i0, a.Tq, a.dk);
-        if (threadIdx.x < 2 * KT) {
+        if (threadIdx.x < 3 * KT) {
             const int i = i0 + (threadIdx.x & (KT - 1));
             const float none = threadIdx.x < KT ? SVBT_INF : 0.f;       // (a query that does not exist has P = 0)
-            stat = i < a.Tq ? (threadIdx.x < KT ? a.lse : g.delta)[hd * a.Tq + i] : none;
+            const float* of = threadIdx.x < KT ? a.stats : threadIdx.x < 2 * KT ? a.stats + (size_t)a.B * a.H * a.Tq : g.delta;
+            stat = i < a.Tq ? of[hd * a.Tq + i] : none;
         }
-        row_lse = a.lse[hd * a.Tq + min(i0 + lane, a.Tq - 1)];
+        row_max = a.stats[hd * a.Tq + min(i0 + lane, a.Tq - 1)];
     };
     auto put = [&](int n) {
         const int i0 = (first + n % tiles) * KT;
         // a query that sees no key has no part in dk and dv, whatever q and dout hold there
         constexpr unsigned long long OTHERS = KT == 64 ? 0ull : ~0xffffffffull;
-        const unsigned long long seen = OTHERS | __ballot(row_lse != SVBT_INF);
+        const unsigned long long seen = OTHERS | __ballot(row_max != SVBT_INF);
         tq.settle(i0, a.Tq, seen);
         td.settle(i0, a.Tq, seen);
         char* buf = smem + (DOUBLE ? (n & 1) * BUF : 0);
         tq.template store<true, true>(buf, buf + 2 * NS * Tile::ROWS_BYTES);
         td.template store<true, true>(buf + NS * Tile::ROWS_BYTES, buf + NS * (2 * Tile::ROWS_BYTES + Tile::COLS_BYTES));
-        if (threadIdx.x < 2 * KT) ((float*)(buf + TILE))[threadIdx.x] = stat;
+        if (threadIdx.x < 3 * KT) ((float*)(buf + TILE))[threadIdx.x] = stat;
     };
     float past = 0.f, ahead = 0.f;
     if (n0 < n1) fetch(n0);
@@ -407,9 +410,9 @@ __global__ __launch_bounds__(256, DKP <= (SvbtParts<T>::NS == 1 ? 64 : 32) ? 2 :
                 }
                 svbt_pace<NS, 2 * NK * NS>();
                 const int o0 = svbt_fresh(j - (pt + 32 * u + 4 * kb));   // offset of register row 0
-                const float *ls = stats + 32 * u + 4 * kb, *dl = ls + KT;
-                if (behind || before) svbt_weights_kv<false>(s, dp, c, nullptr, flat, ls, dl);
-                else svbt_weights_kv<true>(s, dp, c, s_bias + (o0 + R + SVBT_PAD), flat, ls, dl);
+                const float* st = stats + 32 * u + 4 * kb;
+                if (behind || before) svbt_weights_kv<false, KT>(s, dp, c, nullptr, flat, st);
+                else svbt_weights_kv<true, KT>(s, dp, c, s_bias + (o0 + R + SVBT_PAD), flat, st);
                 if (edge) {
 #pragma unroll
                     for (int r = 0; r < 16; ++r) {
@@ -506,7 +509,7 @@ template <typename T, int DKP, int KT, bool DOUBLE, bool TINY = false>
 static int dkv_launch(const SvbBucketAttn* a, const SvbBattnBwd& g, hipStream_t st) {
     typedef SvbtTile<T, DKP, KT, 256, TINY, false> Tile;
     const int span = svbt_span(a->buckets), ktiles = (a->Tk + 127) / 128;
-    const int lds = (DOUBLE ? 2 : 1) * (2 * Tile::NS * (Tile::ROWS_BYTES + Tile::COLS_BYTES) + 2 * KT * 4) + span * 4;
+    const int lds = (DOUBLE ? 2 : 1) * (2 * Tile::NS * (Tile::ROWS_BYTES + Tile::COLS_BYTES) + 3 * KT * 4) + span * 4;
     auto* kern = svb_bucket_attn_dkv_kernel<T, DKP, KT, DOUBLE, TINY>;
     if (bwd_lds(kern, lds)) return SVB_ERR_LAUNCH;
     hipLaunchKernelGGL(kern, dim3((unsigned)(a->B * a->Hkv * ktiles * g.splits)), dim3(256), lds, st, *a, g, ktiles);
@@ -537,7 +540,7 @@ extern "C" int svb_bucket_attn_bwd(const SvbBucketAttn* call, const SvbBucketAtt
     SvbBucketAttn filled = *call;
     svb_bucket_fill(&filled.buckets);
     const SvbBucketAttn* a = &filled;
-    if (!g || !g->dout || !g->ws || !a->lse || (a->dtype == SVB_DT_BF16 && !a->out_f32) || (!g->d_k != !g->d_v)) return SVB_ERR_ARG;
+    if (!g || !g->dout || !g->ws || !a->stats || (a->dtype == SVB_DT_BF16 && !a->out_f32) || (!g->d_k != !g->d_v)) return SVB_ERR_ARG;
     hipStream_t st = (hipStream_t)stream;
     SvbBattnBwd w = {g->dout, g->d_q, g->d_k, g->d_v, g->ws, g->d_table ? g->ws + delta_floats(a) : nullptr, nullptr, kv_splits(a)};
     if (w.splits > 1) w.kv_part = g->ws + delta_floats(a) + table_floats(a);

@@ -252,7 +252,12 @@ __global__ __launch_bounds__(256, SvbtParts<T>::NS == 3 && DKP == 128 ? 1 : 2) v
                 if (out_f32) out_f32[(size_t)ch * a.Tq] = o;
             }
         }
-    if (a.lse && kb == 0) a.lse[((size_t)b * a.H + h) * a.Tq + i] = l > 0.f ? st.m + __log2f(l) : SVBT_INF;
+    // (apart: added up, the logarithm of a sum near 1 is lost behind a large maximum, and with it the weight of the other keys)
+    if (a.stats && kb == 0) {
+        float* stats = a.stats + ((size_t)b * a.H + h) * a.Tq + i;
+        stats[0] = l > 0.f ? st.m : SVBT_INF;
+        stats[(size_t)a.B * a.H * a.Tq] = inv;
+    }
 }
 
 // ---- few query rows: the cache's keys split over waves and workgroups ------------------------------------------------------------------
@@ -598,7 +603,7 @@ static int fwd_launch(const SvbBucketAttn* a, hipStream_t st) {
 // Few rows: what a wave holds in its 32 columns, a tile of keys at least, and nothing kept for a backward.  Splits: enough workgroups for two per CU, at least
 // 256 keys (a tile for each wave) in each; 0: not this form.
 static int few_splits(const SvbBucketAttn* a) {
-    if (a->lse || (long)(a->H / a->Hkv) * a->Tq > 32 || a->Tk < 64 || a->B > 65535 || a->Hkv > 65535) return 0;
+    if (a->stats || (long)(a->H / a->Hkv) * a->Tq > 32 || a->Tk < 64 || a->B > 65535 || a->Hkv > 65535) return 0;
     const int most = (a->Tk + 255) / 256, want = 512 / max(1, min(512, a->B * a->Hkv));
     return max(1, min(most, want));
 }
@@ -657,8 +662,8 @@ extern "C" int svb_bucket_attn_fwd(const SvbBucketAttn* call, float* ws, void* s
     // causal: 38 -> 34; B24 H4 dk48 T211, where a join and a bigger tile save nothing: 14.5 -> 16.5.  Between one and two workgroups per CU
     // (B7 H8 dk64 T1100 causal) the forward takes 39 us this way instead of 36.  fp32 tensors have six products per tile to wait behind.
     const bool thin = a->Tk > 256 && (long)a->B * a->H * ((a->Tq + 127) / 128) <= 256;
-    if (a->lse && thin) SVB_FWD_GO(unsigned short, 128, 64, 3, true, 2);
-    if (a->lse) SVB_FWD_GO(unsigned short, 64, 64, 3, true, 1);
+    if (a->stats && thin) SVB_FWD_GO(unsigned short, 128, 64, 3, true, 2);
+    if (a->stats) SVB_FWD_GO(unsigned short, 64, 64, 3, true, 1);
     if (thin) SVB_FWD_GO(unsigned short, 128, 64, 1, true, 2);
     SVB_FWD_GO(unsigned short, 64, 64, 1, true, 1);
 #undef SVB_FWD_GO

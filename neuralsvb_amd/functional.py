@@ -975,20 +975,20 @@ def bucket_bias(table, buckets, tq, tk, q_start=None):
 class _BucketAttnFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, table, keep, q_start, cfg):
-        out, lse, o32 = K.bucket_attn_fwd(q, k, v, table, *cfg[:2], keep, q_start, *cfg[2:], train=True)
+        out, stats, o32 = K.bucket_attn_fwd(q, k, v, table, *cfg[:2], keep, q_start, *cfg[2:], train=True)
         ctx.cfg = cfg
         ctx.start = None if isinstance(q_start, torch.Tensor) else q_start
-        ctx.save_for_backward(q, k, v, table, keep, None if ctx.start is not None else q_start, out if o32 is None else None, lse, o32)
+        ctx.save_for_backward(q, k, v, table, keep, None if ctx.start is not None else q_start, out if o32 is None else None, stats, o32)
         return out
 
     @staticmethod
     @_first_order
     def backward(ctx, dout):
-        q, k, v, table, keep, starts, out, lse, o32 = ctx.saved_tensors
+        q, k, v, table, keep, starts, out, stats, o32 = ctx.saved_tensors
         nq, nk, nv, nt = ctx.needs_input_grad[:4]
         cfg = ctx.cfg
         dq, dk, dv, dt = K.bucket_attn_bwd(_c(dout), q, k, v, table, *cfg[:2], keep, starts if ctx.start is None else ctx.start, *cfg[2:], out,
-                                           lse, o32, nq, nk or nv, nt)
+                                           stats, o32, nq, nk or nv, nt)
         return dq, dk if nk else None, dv if nv else None, dt, None, None, None
 
 

@@ -1192,14 +1192,14 @@ def _bucket_attn_desc(q, k, v, table, buckets, n_head, keep, q_start, causal, sc
 
 
 def bucket_attn_fwd(q, k, v, table, buckets, n_head, keep, q_start, causal, scale, train=False):
-    """-> out [B, H dk, Tq]; with train also lse [B, H, Tq] and, for bf16 tensors, out in float32 (None for float32)."""
+    """-> out [B, H dk, Tq]; with train also stats [2, B, H, Tq] (maximum, 1 / sum) and, for bf16 tensors, out in float32 (None for float32)."""
     lib, st, d = _bucket_attn_desc(q, k, v, table, buckets, n_head, keep, q_start, causal, scale)
     B, D, tq = q.shape
     out = q.new_empty((B, D, tq))
-    lse = o32 = None
+    stats = o32 = None
     if train:
-        lse = q.new_empty((B, n_head, tq), dtype=torch.float32)
-        d.lse = lse.data_ptr()
+        stats = q.new_empty((2, B, n_head, tq), dtype=torch.float32)
+        d.stats = stats.data_ptr()
         if q.dtype is not torch.float32:
             o32 = q.new_empty((B, D, tq), dtype=torch.float32)
             d.out_f32 = o32.data_ptr()
@@ -1210,17 +1210,17 @@ def bucket_attn_fwd(q, k, v, table, buckets, n_head, keep, q_start, causal, scal
         n = 0 if train else lib.svb_bucket_attn_fwd_workspace_floats(_byref(d))
         ws = q.new_empty((n,), dtype=torch.float32) if n else None
         _issue(q.get_device(), "svb_bucket_attn_fwd", lib.svb_bucket_attn_fwd, _byref(d), _ptr(ws), st)
-    return (out, lse, o32) if train else out
+    return (out, stats, o32) if train else out
 
 
-def bucket_attn_bwd(dout, q, k, v, table, buckets, n_head, keep, q_start, causal, scale, out, lse, o32, want_q=True, want_kv=True,
+def bucket_attn_bwd(dout, q, k, v, table, buckets, n_head, keep, q_start, causal, scale, out, stats, o32, want_q=True, want_kv=True,
                     want_table=True):
     """-> dq, dk, dv, dtable, contiguous, None where not wanted.  out is read for float32 tensors, o32 for bfloat16 ones (the other may
     be None)."""
     lib, st, d = _bucket_attn_desc(q, k, v, table, buckets, n_head, keep, q_start, causal, scale)
     if dout.shape != q.shape or dout.dtype is not q.dtype:
         raise ValueError("dout must have the shape and dtype of the output")
-    _prep(dout, out, lse, o32)
+    _prep(dout, out, stats, o32)
     dq = q.new_empty(q.shape) if want_q else None
     dk, dv = (k.new_empty(k.shape), k.new_empty(k.shape)) if want_kv else (None, None)
     dt = table.new_empty(table.shape) if want_table else None
@@ -1229,7 +1229,7 @@ def bucket_attn_bwd(dout, q, k, v, table, buckets, n_head, keep, q_start, causal
             if t is not None:
                 t.zero_()
         return dq, dk, dv, dt
-    d.out, d.lse, d.out_f32 = _ptr(o32 if out is None else out), lse.data_ptr(), _ptr(o32)
+    d.out, d.stats, d.out_f32 = _ptr(o32 if out is None else out), stats.data_ptr(), _ptr(o32)
     ws = q.new_empty((lib.svb_bucket_attn_bwd_workspace_floats(_byref(d)),), dtype=torch.float32)
     g = L.SvbBucketAttnGrad(dout.data_ptr(), _ptr(dq), _ptr(dk), _ptr(dv), _ptr(dt), ws.data_ptr())
     _issue(q.get_device(), "svb_bucket_attn_bwd", lib.svb_bucket_attn_bwd, _byref(d), _byref(g), st)

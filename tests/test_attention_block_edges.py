@@ -139,3 +139,58 @@ def test_frozen_encoder_refuses_gradients(dev, mode, heads):
     out = enc.encoder_layers[0](x, enc._pos_emb(20, dev), torch.ones(2, 20, dtype=torch.bool, device=dev))
     g, = torch.autograd.grad(out, last.bias, do)
     near(g, do.double().cpu().sum((0, 2)), 8 * U32 * (math.sqrt(40) + 4), "bias of the last norm")
+
+
+# ---- rows with nearly all their weight on one key --------------------------------------------------------------------------
+def peaked(dt, t, gap, offset, table_offset):
+    """Query i scores key (5 i) mod t higher than the others by about `gap`; all scores are near `offset`, table entries near `table_offset`."""
+    gen = torch.Generator().manual_seed(61)
+    dk = t + 8
+    q, k = (torch.randn(1, dk, t, generator=gen) * 0.3 for _ in range(2))
+    at = 5 * torch.arange(t) % t
+    q[0, :t], k[0, :t] = 0.0, torch.eye(t)
+    q[0, at, torch.arange(t)] = gap
+    q[0, t], k[0, t] = 16.0, offset / 16.0
+    v, do = (torch.randn(1, dk, t, generator=gen) for _ in range(2))
+    table = torch.randn(16, 1, generator=gen) * 0.3 + table_offset
+    return tuple(x.to(DT[dt]) for x in (q, k, v)) + (table, do.to(DT[dt]))
+
+
+@_dt
+@pytest.mark.parametrize("gap,offset,table_offset", [(15.0, 184.0, 0.0), (15.0, 0.0, 200.0), (11.0, 0.0, 200.0), (12.0, 184.0, -150.0)])
+def test_peaked_rows(dev, dt, gap, offset, table_offset):
+    """The gradient of a row whose other keys hold a weight of 1e-6: their weights, and the small difference dP - delta of the main one."""
+    from tests.test_attention_block import attention64
+    t, bk = 32, SF.RelativeBuckets(16, 24, True)
+    *x, do = peaked(dt, t, gap, offset, table_offset)
+    want = leaves64(*x)
+    out = attention64(*want, bk, 1, scale=1.0)
+    out.backward(do.double())
+    got = [m.clone().to(dev).requires_grad_() for m in x]
+    o = SF.bucket_attention(*got, bk, 1, scale=1.0)
+    o.backward(do.to(dev))
+    unit = 3 * UBF if dt == "bf16" else 0.0                              # (operands and results rounded, as in the other tests)
+    near(o, out.detach(), unit + 16 * U32, "out")
+    near(got[2].grad, want[2].grad, unit + 16 * U32, "dv")
+    # dS of the main key is P (dP - delta), of the size of the others' weight `rest`, from two sums with errors of some half steps of
+    # themselves (40 products each, three bf16 parts); scores of size 300 carry 300 half steps into the others' weights
+    rest = (t - 1) * math.exp(-gap)
+    tol = 16 * (U32 / rest + 300 * U32)
+    # dq_i = sum_j dS_ij k_j: the sum over j of dS is 0, so what all keys have in common (the offset) leaves the result and stays in the
+    # errors: e |k| against dS |k_j - k_l|
+    k = x[1][0].double()
+    common = max(1.0, float(k.norm(dim=0).mean() / (k - k.mean(1, keepdim=True)).norm(dim=0).mean()))
+    for name, a, b, f in (("dq", got[0], want[0], common), ("dk", got[1], want[1], 1.0)):
+        near(a.grad, b.grad, unit + f * tol, name)
+    near(got[3].grad, want[3].grad, tol + (8 * 2.0 ** -16 if dt == "bf16" else 0.0), "dtable")
+
+
+@_dt
+def test_rows_with_all_weight_on_one_key(dev, dt):
+    """Beyond what 32 bits can tell from one key alone the gradient of the scores is 0, not the rounding of dP - delta."""
+    bk = SF.RelativeBuckets(16, 24, True)
+    *x, do = peaked(dt, 32, 60.0, 0.0, 3.0)
+    got = [m.clone().to(dev).requires_grad_() for m in x]
+    dq, dk, dtable = torch.autograd.grad(SF.bucket_attention(*got, bk, 1, scale=1.0), (got[0], got[1], got[3]), do.to(dev))
+    for g in (dq, dk, dtable):
+        assert float(g.float().abs().max()) <= 1e-20                     # (the others' weights: exp(-57) at most)
