@@ -37,8 +37,7 @@ struct SvbBattnBwd {
 };
 
 __device__ __forceinline__ float svbt_ds(float p, float dp, float delta) {
-    const float ds = p * (dp - delta);
-    return p == 0.f || p == 1.f ? 0.f : ds;                             // (p == 1: its row's sum is exactly 1)
+    return (p == 1.f ? 0.f : p) * (dp - delta);                         // (p == 1: its row's sum is exactly 1; NaN and infinities stay)
 }
 
 // Adds a sub-tile's diagonal sums to diag[key - query], one wave.  s: register r is key svbt_row(r, kb) of query l31; skew: [32][36] floats
@@ -60,9 +59,8 @@ __device__ __forceinline__ void svbt_diag_add(float* skew, float* diag, const f3
         const float4 v = *reinterpret_cast<const float4*>(skew + l31 * SVBT_SKEW_P + 16 * kb + 4 * m);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            const float x = 4 * m + e <= last ? v[e] : 0.f;
-            here += x;
-            there += v[e] - x;                                          // (exactly v or 0)
+            here += 4 * m + e <= last ? v[e] : 0.f;                     // (a choice each: a difference would carry a NaN over)
+            there += 4 * m + e <= last ? 0.f : v[e];
         }
     }
     here += __shfl_xor(here, 32, 64);
@@ -110,6 +108,8 @@ __global__ __launch_bounds__(256, SvbtParts<T>::NS == 1 || DKP <= 64 ? 2 : 1) vo
     const size_t head = ((size_t)b * a.H + h) * a.dk * a.Tq;
     const int ic = has ? i : 0;
     const size_t row = ((size_t)b * a.H + h) * a.Tq + ic;
+    // a query that sees no key has no part in anything, whatever q and dout hold there
+    const float m = has ? a.stats[row] : SVBT_INF, inv = has ? a.stats[(size_t)a.B * a.H * a.Tq + row] : 0.f;
     svbt_bf16x8 qf[NK][NS], of[NK][NS];
     float delta = 0.f;
     {
@@ -119,11 +119,12 @@ __global__ __launch_bounds__(256, SvbtParts<T>::NS == 1 || DKP <= 64 ? 2 : 1) vo
         own_o.load((NS == 3 ? (const float*)a.out : a.out_f32) + head, a.Tq, ic, kb, a.dk);
         own_q.load(q, a.q_sc, ic, kb, a.dk);
         if (g.dq || g.part) fetch(0);                                   // (uniform)
+        const bool sees = m != SVBT_INF;
 #pragma unroll
         for (int s = 0; s < NK; ++s) {
             float v8[8], o8[8];
-            own_do.get(s, kb, a.dk, has, v8);
-            own_o.get(s, kb, a.dk, has, o8);
+            own_do.get(s, kb, a.dk, sees, v8);
+            own_o.get(s, kb, a.dk, sees, o8);
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
                 delta = fmaf(v8[e], o8[e], delta);
@@ -131,12 +132,11 @@ __global__ __launch_bounds__(256, SvbtParts<T>::NS == 1 || DKP <= 64 ? 2 : 1) vo
             }
             svbt_frag8<NS>(v8, of[s]);
         }
-        own_q.frags(kb, a.dk, has, qf);
+        own_q.frags(kb, a.dk, sees, qf);
     }
     delta += __shfl_xor(delta, 32, 64);
     if (has && kb == 0) g.delta[row] = delta;
     if (!g.dq && !g.part) return;                                       // (only delta is wanted; uniform)
-    const float m = has ? a.stats[row] : SVBT_INF, inv = has ? a.stats[(size_t)a.B * a.H * a.Tq + row] : 0.f;
 
     const int span = (2 * (R + SVBT_PAD) + 1 + 3) & ~3;
     unsigned* s_bad = (unsigned*)(smem + (DOUBLE ? 2 : 1) * BUF);        // [SVBT_BAD_WORDS]
@@ -193,7 +193,7 @@ __global__ __launch_bounds__(256, SvbtParts<T>::NS == 1 || DKP <= 64 ? 2 : 1) vo
         const char* vrows = krows + NS * Tile::ROWS_BYTES;
         const char* kcols = vrows + NS * Tile::ROWS_BYTES;
         if (now != 0ull && !(a.causal && j0 > p1)) {
-            const bool edge = now != ALL || (a.causal && j0 + KT - 1 > p0);
+            const bool edge = now != ALL || (a.causal && j0 + KT - 1 > p0) || i0 + wave * 32 + 32 > a.Tq;
             const bool behind = j0 + KT - 1 - p0 <= -R, before = j0 - p1 >= R;
             const float flat = behind ? past : ahead;
 #pragma unroll 1
@@ -216,7 +216,7 @@ __global__ __launch_bounds__(256, SvbtParts<T>::NS == 1 || DKP <= 64 ? 2 : 1) vo
                 if (PACED) svbt_pace<NS, 2 * NK * NS>();
 #pragma unroll
                 for (int r = 0; r < 16; ++r) dp[r] -= dp_neg[r];
-                const unsigned su = (unsigned)(now >> (32 * u)) >> (4 * kb);
+                const unsigned su = has ? (unsigned)(now >> (32 * u)) >> (4 * kb) : 0u;
                 const int o0 = svbt_fresh(j0 + 32 * u + 4 * kb - p);     // offset of register row 0
                 const bool far = behind || before;
                 if (far) svbt_weights_q<false>(s, dp, c, nullptr, flat, m, inv, delta);
@@ -456,12 +456,13 @@ __global__ __launch_bounds__(256, DKP <= (SvbtParts<T>::NS == 1 ? 64 : 32) ? 2 :
         for (int r = 0; r < 16; ++r) {
             const int ch = 32 * d + svbt_row(r, kb);
             if (ch >= a.dk) continue;
+            const float sk = kept ? dk[d][r] : 0.f, sv = kept ? dv[d][r] : 0.f;        // (0 times a NaN of q or dout is one)
             if (g.splits > 1) {
-                pk[(size_t)ch * a.Tk] = dk[d][r];
-                pk[g.splits * all + (size_t)ch * a.Tk] = dv[d][r];
+                pk[(size_t)ch * a.Tk] = sk;
+                pk[g.splits * all + (size_t)ch * a.Tk] = sv;
             } else {
-                svbt_store((T*)g.dk + head + (size_t)ch * a.Tk, dk[d][r] * a.scale);
-                svbt_store((T*)g.dv + head + (size_t)ch * a.Tk, dv[d][r]);
+                svbt_store((T*)g.dk + head + (size_t)ch * a.Tk, sk * a.scale);
+                svbt_store((T*)g.dv + head + (size_t)ch * a.Tk, sv);
             }
         }
 }

@@ -234,7 +234,7 @@ __global__ __launch_bounds__(256, SvbtParts<T>::NS == 3 && DKP == 128 ? 1 : 2) v
             for (int r = 0; r < 16; ++r) st.o[d][r] = st.o[d][r] * f0 + s_st[(16 * d + r) * 64] * f1;
     }
     const float l = st.l + __shfl_xor(st.l, 32, 64);
-    const float inv = l > 0.f ? 1.f / l : 0.f;                          // (no key: zeros)
+    const float inv = l == 0.f ? 0.f : 1.f / l;                         // (no key: zeros; NaN stays)
     const uint4 bad = *reinterpret_cast<const uint4*>(s_bad);
     if ((bad.x | bad.y | bad.z | bad.w) != 0u) svbt_add_bad<T, NDB>(st.o, s_bad, SVBT_BAD_WORDS, v, a.v_sc, a.dk, part, p, kb);
     if (!has) return;
@@ -255,7 +255,7 @@ __global__ __launch_bounds__(256, SvbtParts<T>::NS == 3 && DKP == 128 ? 1 : 2) v
     // (apart: added up, the logarithm of a sum near 1 is lost behind a large maximum, and with it the weight of the other keys)
     if (a.stats && kb == 0) {
         float* stats = a.stats + ((size_t)b * a.H + h) * a.Tq + i;
-        stats[0] = l > 0.f ? st.m : SVBT_INF;
+        stats[0] = l > 0.f ? st.m : l == 0.f ? SVBT_INF : l;            // (NaN: the row has keys, and NaN gradients)
         stats[(size_t)a.B * a.H * a.Tq] = inv;
     }
 }
@@ -536,7 +536,7 @@ __global__ __launch_bounds__(256, DKP * SvbtParts<T>::NS > 192 || DKP == 128 ? 1
         }
         const int g = r / a.Tq, i2 = r - g * a.Tq;
         if (!parts.o) {
-            const float inv = l > 0.f ? 1.f / l : 0.f;
+            const float inv = l == 0.f ? 0.f : 1.f / l;
             svbt_store((T*)a.out + (((size_t)b * a.H + hk * G + g) * a.dk + ch) * a.Tq + i2, o * inv);
         } else {
             parts.o[(item * rows + r) * a.dk + ch] = o;
@@ -565,7 +565,7 @@ __global__ __launch_bounds__(256) void svb_bucket_attn_join_kernel(SvbBucketAttn
         for (int u = 0; u < 2; ++u)
             if (lane + 64 * u < a.dk) o[u] = fmaf(po[(size_t)s * rows * a.dk + lane + 64 * u], f, o[u]);
     }
-    const float inv = l > 0.f ? 1.f / l : 0.f;
+    const float inv = l == 0.f ? 0.f : 1.f / l;
     const int g = r / a.Tq, i = r - g * a.Tq;
 #pragma unroll
     for (int u = 0; u < 2; ++u)

@@ -194,3 +194,35 @@ def test_rows_with_all_weight_on_one_key(dev, dt):
     dq, dk, dtable = torch.autograd.grad(SF.bucket_attention(*got, bk, 1, scale=1.0), (got[0], got[1], got[3]), do.to(dev))
     for g in (dq, dk, dtable):
         assert float(g.float().abs().max()) <= 1e-20                     # (the others' weights: exp(-57) at most)
+
+
+# ---- what is not finite stays visible in the gradients -----------------------------------------------------------------------
+@_dt
+@pytest.mark.parametrize("what,causal", [("k", False), ("v", False), ("q", False), ("k", True), ("v", True)])      # (q: finite, if causal)
+@pytest.mark.parametrize("shape", [(41, 41), (70, 100), (3, 40), (100, 3)])
+def test_nan_reaches_the_gradients(dev, dt, what, causal, shape):
+    """A NaN in a key or value that some queries see, or in a query, makes those gradients NaN that the definition makes NaN, and no others."""
+    tq, tk = shape
+    bk = SF.RelativeBuckets(16, 24, not causal)
+    q, k, v, table, do = case(tq + tk, dt, 2, 2, 2, 24, tq, tk)
+    {"k": k, "v": v, "q": q}[what][0, 24 + 5, (tk if what != "q" else tq) // 2] = math.nan          # (one entry, second head)
+    keep = torch.ones(2, tk)
+    keep[:, 0] = 0
+    starts = torch.tensor([tk - tq] * 2, dtype=torch.int32)
+    want = leaves64(q, k, v, table)
+    out = attention_by_rows(*want, bk, 2, keep, causal, starts)
+    wg = torch.autograd.grad(out, want, do.double())
+    leaves = [t.clone().to(dev).requires_grad_() for t in (q, k, v, table)]
+    o = SF.bucket_attention(*leaves, bk, 2, keep=keep.to(dev), causal=causal)
+    gg = torch.autograd.grad(o, leaves, do.to(dev))
+    tol = 3 * UBF if dt == "bf16" else 128 * U32
+    like(o, out, tol, "out")
+    for name, g, w in zip(("dq", "dk", "dv", "dtable"), gg, wg):
+        assert not torch.isfinite(w).all() or (what, name) == ("v", "dv")
+        # (dtable: sums that cancel, as elsewhere against the size of their terms)
+        if name == "dtable":
+            assert torch.equal(torch.isfinite(g.cpu()), torch.isfinite(w)), name
+            g, w = (torch.nan_to_num(t.detach().double().cpu(), 0.0, 0.0, 0.0) for t in (g, w))
+            near(g, w, {"bf16": 8 * 2.0 ** -16, "f32": 128 * U32}[dt], name, float(do.double().norm()))
+        else:
+            like(g, w, tol, name)
