@@ -13,6 +13,7 @@ import functools
 import weakref
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _lib as L_
@@ -883,6 +884,12 @@ def _first_order(fn):
     return backward
 
 
+def _no_tangents(what, *ts):
+    """Calls that bypass their autograd Function would drop a forward-mode derivative, which the Function refuses."""
+    if forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in ts):
+        raise NotImplementedError(f"{what} has no forward-mode derivative")
+
+
 class _LayerNormNCTFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, gamma, beta, eps):
@@ -904,6 +911,7 @@ def layer_norm_nct(x, gamma, beta, eps=1e-5):
     dtype, each may be None.  Statistics and sums are float32; the affine gradients have a fixed order of summation."""
     if x.dim() != 3:
         raise ValueError(f"layer_norm_nct: x must be [B, C, T], got {tuple(x.shape)}")
+    _no_tangents("layer_norm_nct", x, gamma, beta)
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, gamma, beta)):
         return _LayerNormNCTFn.apply(x, gamma, beta, float(eps))
     if x.dtype == torch.float32 and x.numel():
@@ -1014,6 +1022,7 @@ def bucket_attention(q, k, v, table, buckets, n_head, keep=None, causal=False, s
     n_head = int(n_head)
     if n_head < 1:
         raise ValueError(f"bucket_attention: n_head = {n_head}")
+    _no_tangents("bucket_attention", q, k, v, table)
     q, k, v, table, keep = _time_rows(q), _time_rows(k), _time_rows(v), _c(table), _c(keep)
     if scale is None:
         scale = (q.shape[1] // n_head) ** -0.5 if q.dim() == 3 and q.shape[1] >= n_head else 1.0

@@ -226,3 +226,28 @@ def test_nan_reaches_the_gradients(dev, dt, what, causal, shape):
             near(g, w, {"bf16": 8 * 2.0 ** -16, "f32": 128 * U32}[dt], name, float(do.double().norm()))
         else:
             like(g, w, tol, name)
+
+
+# ---- forward-mode derivatives --------------------------------------------------------------------------------------------
+def test_forward_mode_is_refused(dev):
+    """No operator here has a forward-mode derivative: dual numbers are an error, not a result without its tangent."""
+    from torch.autograd import forward_ad
+    bk = SF.RelativeBuckets(8, 20)
+    x, table = torch.randn(1, 16, 9, device=dev), torch.randn(8, 2, device=dev)
+    one = torch.ones(16, device=dev)
+    plain = SF.layer_norm_nct(x, one, None)
+    with forward_ad.dual_level():
+        dual = lambda t: forward_ad.make_dual(t, torch.ones_like(t))  # noqa: E731
+        calls = [lambda: SF.layer_norm_nct(dual(x), one, None), lambda: SF.layer_norm_nct(x, dual(one), None), lambda: SF.layer_norm_nct(x, None, dual(one)),
+                 lambda: SF.layer_norm_nct(dual(x.bfloat16()), None, None), lambda: SF.bucket_bias(dual(table), bk, 3, 4)]
+        for i in range(4):
+            args = [x, x, x, table]
+            args[i] = dual(args[i])
+            calls.append(lambda args=args: SF.bucket_attention(*args, bk, 2))
+        for call in calls:
+            with pytest.raises(NotImplementedError):
+                call()
+            with torch.no_grad(), pytest.raises(NotImplementedError):
+                call()
+        assert torch.equal(SF.layer_norm_nct(x, one, None), plain)        # (no tangent in it)
+    assert torch.equal(SF.layer_norm_nct(x, one, None), plain)
