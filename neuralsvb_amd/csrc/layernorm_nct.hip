@@ -270,33 +270,35 @@ __global__ __launch_bounds__(NT) void svb_ln_nct_bwd_kernel(SvbLnArgs a) {
     }
 }
 
-// More channels than the register form holds: 32 positions x 8 channel groups, values read again for each use (they come from L2).
-template <typename T>
-__global__ __launch_bounds__(256) void svb_ln_nct_fwd_wide_kernel(SvbLnArgs a) {
-    __shared__ float red[2][8][32];
+// More channels (or longer rows) than the register form takes: 32 positions x G channel groups, values read again for each use (they come
+// from L2).  The forward is a chain of C / G loads in each of its three passes: 32 groups where there are channels for them
+// (4 x 1500 x 700 fp32 207 us with 8 groups).
+template <typename T, int G>
+__global__ __launch_bounds__(32 * G) void svb_ln_nct_fwd_wide_kernel(SvbLnArgs a) {
+    __shared__ float red[2][G][32];
     const int tl = threadIdx.x & 31, cg = threadIdx.x >> 5;
     const int b = blockIdx.x / a.tiles, t = (blockIdx.x - b * a.tiles) * 32 + tl;
     const int n = a.T - t;
     const size_t base = (size_t)b * a.C * a.T + (n > 0 ? t : 0);
     const T* x = (const T*)a.x + base;
     float s = 0.f;
-    for (int c = cg; c < a.C; c += 8) s += svbl_ld(x + (size_t)c * a.T, n);
+    for (int c = cg; c < a.C; c += G) s += svbl_ld(x + (size_t)c * a.T, n);
     red[0][cg][tl] = s;
     __syncthreads();
     s = 0.f;
 #pragma unroll
-    for (int q = 0; q < 8; ++q) s += red[0][q][tl];
+    for (int q = 0; q < G; ++q) s += red[0][q][tl];
     const float mu = s / (float)a.C;
     s = 0.f;
-    for (int c = cg; c < a.C; c += 8) { const float d = svbl_ld(x + (size_t)c * a.T, n) - mu; s = fmaf(d, d, s); }
+    for (int c = cg; c < a.C; c += G) { const float d = svbl_ld(x + (size_t)c * a.T, n) - mu; s = fmaf(d, d, s); }
     red[1][cg][tl] = s;
     __syncthreads();
     s = 0.f;
 #pragma unroll
-    for (int q = 0; q < 8; ++q) s += red[1][q][tl];
+    for (int q = 0; q < G; ++q) s += red[1][q][tl];
     const float rs = 1.f / sqrtf(s / (float)a.C + a.eps);
     if (a.mean && cg == 0 && n > 0) { a.mean[(size_t)b * a.T + t] = mu; a.rstd[(size_t)b * a.T + t] = rs; }
-    for (int c = cg; c < a.C; c += 8) {
+    for (int c = cg; c < a.C; c += G) {
         const float g = a.gamma ? svb_ld_table(a.gamma, c, a.affine_bf16) : 1.f;
         const float bt = a.beta ? svb_ld_table(a.beta, c, a.affine_bf16) : 0.f;
         const float o[1] = {fmaf((svbl_ld(x + (size_t)c * a.T, n) - mu) * rs, g, bt)};
@@ -392,7 +394,8 @@ static void svbl_launch(bool fwd, const SvbLnArgs& a, const SvbLnPlan& p, unsign
         else hipLaunchKernelGGL((svb_ln_nct_bwd_kernel<T, V, L, N, P>), dim3(grid), dim3(N), 0, st, a);              \
     } while (0)
     if (p.rows == 0) {
-        if (fwd) hipLaunchKernelGGL((svb_ln_nct_fwd_wide_kernel<T>), dim3(grid), dim3(256), 0, st, a);
+        if (fwd && a.C > 256) hipLaunchKernelGGL((svb_ln_nct_fwd_wide_kernel<T, 32>), dim3(grid), dim3(1024), 0, st, a);
+        else if (fwd) hipLaunchKernelGGL((svb_ln_nct_fwd_wide_kernel<T, 8>), dim3(grid), dim3(256), 0, st, a);
         else hipLaunchKernelGGL((svb_ln_nct_bwd_wide_kernel<T>), dim3(grid), dim3(256), 0, st, a);
     } else if (p.positions == 4) SVBL_GO(1, 4, 256, 16);
     else if (p.rows == 256) SVBL_GO(VEC, 8, 256, 8);
@@ -401,10 +404,12 @@ static void svbl_launch(bool fwd, const SvbLnArgs& a, const SvbLnPlan& p, unsign
 #undef SVBL_GO
 }
 
+static int svbl_threads(const SvbLnPlan& p, int C) { return p.rows == 0 ? (C > 256 ? 1024 : 256) : p.rows > 256 && p.positions != 4 ? 512 : 256; }
 static bool svbl_fits(int B, int C, int T, int dtype, SvbLnPlan* p, int* tiles) {
     *p = svbl_plan(C, T, dtype);
     *tiles = (T + p->positions - 1) / p->positions;
-    return (long)B * *tiles < (1 << 23);                                 // (a launch has less than 2^32 threads)
+    // (a launch has less than 2^32 threads; the tiles of all entries are counted in 31 bits)
+    return *tiles <= 0xffffffffL / svbl_threads(*p, C) && (long)B * *tiles <= 0x7fffffffL - SVB_LN_MAX_WG;
 }
 static bool svbl_dtypes(int dtype, int affine_dtype) {
     return (dtype == SVB_DT_F32 && affine_dtype == SVB_DT_F32) || (dtype == SVB_DT_BF16 && (affine_dtype == SVB_DT_F32 || affine_dtype == SVB_DT_BF16));
@@ -416,11 +421,20 @@ extern "C" int svb_ln_nct_fwd(const void* x, const void* gamma, const void* beta
     SvbLnArgs a = {};
     SvbLnPlan p;
     if (!svbl_dtypes(dtype, affine_dtype) || !svbl_fits(B, C, T, dtype, &p, &a.tiles)) return SVB_ERR_UNSUPPORTED;
-    a.x = x; a.gamma = gamma; a.beta = beta; a.y = y; a.mean = mean; a.rstd = rstd;
-    a.B = B; a.C = C; a.T = T; a.eps = eps; a.affine_bf16 = affine_dtype == SVB_DT_BF16;
-    if (dtype == SVB_DT_BF16) svbl_launch<unsigned short, 8>(true, a, p, (unsigned)(B * a.tiles), (hipStream_t)stream);
-    else svbl_launch<float, 4>(true, a, p, (unsigned)(B * a.tiles), (hipStream_t)stream);
-    SVB_CHECK_LAUNCH();
+    a.gamma = gamma; a.beta = beta;
+    a.C = C; a.T = T; a.eps = eps; a.affine_bf16 = affine_dtype == SVB_DT_BF16;
+    const size_t entry = (size_t)C * T * (dtype == SVB_DT_BF16 ? 2 : 4);
+    const int most = (int)(0xffffffffL / svbl_threads(p, C) / a.tiles);      // batch entries of a launch
+    for (int b = 0; b < B; b += a.B) {
+        a.B = B - b < most ? B - b : most;
+        a.x = (const char*)x + b * entry;
+        a.y = (char*)y + b * entry;
+        a.mean = mean ? mean + (size_t)b * T : nullptr;
+        a.rstd = mean ? rstd + (size_t)b * T : nullptr;
+        if (dtype == SVB_DT_BF16) svbl_launch<unsigned short, 8>(true, a, p, (unsigned)(a.B * a.tiles), (hipStream_t)stream);
+        else svbl_launch<float, 4>(true, a, p, (unsigned)(a.B * a.tiles), (hipStream_t)stream);
+        SVB_CHECK_LAUNCH();
+    }
     return SVB_OK;
 }
 

@@ -350,6 +350,9 @@ __global__ __launch_bounds__(256) void svb_layernorm_bwd_kernel(const float* x, 
 // LayerNorm over the channel dim of an NCT tensor.  Block = 32 time columns x 8 channel groups (a wave covers two
 // 128-byte row segments per load); each thread keeps its C/8 values in registers (all loads in flight at once, x is
 // read ONCE), the groups combine their shifted moments through LDS.  1 read + 1 write of x.
+// Moments about channel 0 cancel where that channel lies far from the others: sum / C is then 1 + md^2 / var times the variance that is
+// left, and so are its half steps.  Beyond 32 (channel 0 more than 5.6 deviations off the mean) the column takes moments about its mean, from
+// a second pass over the same registers; columns within keep what they had.
 // (Round 6: 3.0 TB/s at C = 256, T = 1124.  A 64-column x 4-group block -- 256-byte runs per load instruction, 64 values per
 // thread -- measured 2.47 TB/s, profiles/r06_streaming_kernels_2.log: not the run length; kept as is.)
 #define SVB_LN_MAXV 48          /* register-resident values per thread: C <= 384 (larger C re-reads x) */
@@ -357,6 +360,7 @@ __global__ __launch_bounds__(256) void svb_layernorm_nct_fwd_kernel(const float*
                                                                     float* y, int B, int C, int T, float eps) {
     __shared__ float s_sum[8][32];
     __shared__ float s_sq[8][32];
+    __shared__ int s_far;
     const int tl = threadIdx.x & 31, cg = threadIdx.x >> 5;
     const int tiles = (T + 31) / 32;
     const int b = blockIdx.x / tiles, t = (blockIdx.x % tiles) * 32 + tl;
@@ -388,13 +392,45 @@ __global__ __launch_bounds__(256) void svb_layernorm_nct_fwd_kernel(const float*
     }
     s_sum[cg][tl] = s;
     s_sq[cg][tl] = ss;
+    if (threadIdx.x == 0) s_far = 0;
     __syncthreads();
     s = 0.f; ss = 0.f;
 #pragma unroll
     for (int q = 0; q < 8; ++q) { s += s_sum[q][tl]; ss += s_sq[q][tl]; }
     const float md = s / (float)C;
-    const float var = fmaxf(ss / (float)C - md * md, 0.f);
-    const float mu = x0 + md;
+    float var = fmaxf(ss / (float)C - md * md, 0.f);
+    float mu = x0 + md;
+    const bool far = ss > 32.f * (float)C * var;              // (the same in all groups of a column)
+    if (far) s_far = 1;
+    __syncthreads();
+    if (s_far) {                                              // (uniform)
+        s = 0.f; ss = 0.f;
+        if (inreg) {
+#pragma unroll
+            for (int i = 0; i < SVB_LN_MAXV; ++i) {
+                const float d = cg + 8 * i < C ? v[i] - mu : 0.f;
+                s += d;
+                ss = fmaf(d, d, ss);
+            }
+        } else {
+            for (int c = cg; c < C; c += 8) {
+                const float d = xc[(size_t)c * T] - mu;
+                s += d;
+                ss = fmaf(d, d, ss);
+            }
+        }
+        s_sum[cg][tl] = s;
+        s_sq[cg][tl] = ss;
+        __syncthreads();
+        s = 0.f; ss = 0.f;
+#pragma unroll
+        for (int q = 0; q < 8; ++q) { s += s_sum[q][tl]; ss += s_sq[q][tl]; }
+        if (far) {
+            const float off = s / (float)C;                   // (what the first mean was off by)
+            mu += off;
+            var = fmaxf(ss / (float)C - off * off, 0.f);
+        }
+    }
     const float rs = 1.f / sqrtf(var + eps);
     if (!ok) return;
     if (inreg) {

@@ -912,14 +912,10 @@ def layer_norm_nct(x, gamma, beta, eps=1e-5):
     if x.dim() != 3:
         raise ValueError(f"layer_norm_nct: x must be [B, C, T], got {tuple(x.shape)}")
     _no_tangents("layer_norm_nct", x, gamma, beta)
+    gamma, beta = (p if p is None or p.dim() == 1 else p.reshape(-1) for p in (gamma, beta))
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, gamma, beta)):
         return _LayerNormNCTFn.apply(x, gamma, beta, float(eps))
-    if x.dtype == torch.float32 and x.numel():
-        for p in (gamma, beta):
-            if p is not None and p.numel() != x.shape[1]:
-                raise ValueError(f"gamma, beta: [{x.shape[1]}], got {tuple(p.shape)}")
-        return K.layernorm_nct_fwd(x.contiguous(), _c(gamma), _c(beta), eps)
-    return K.ln_nct_fwd(_c(x), _c(gamma), _c(beta), eps)
+    return K.ln_nct_fwd(_c(x), _c(gamma), _c(beta), float(eps))
 
 
 @functools.lru_cache(maxsize=64)

@@ -10,6 +10,7 @@ import torch
 from torch import nn
 
 from .. import functional as SF
+from .. import kernels as K
 
 
 class Conv1d(nn.Module):
@@ -130,7 +131,11 @@ class LayerNormNCT(nn.Module):
         self.eps = eps
 
     def forward(self, x):
-        return SF.layer_norm_nct(x, self.weight, self.bias, self.eps)
+        wanted = torch.is_grad_enabled() and (x.requires_grad or self.weight.requires_grad or self.bias.requires_grad)
+        if wanted or x.dtype != torch.float32 or not x.numel():
+            return SF.layer_norm_nct(x, self.weight, self.bias, self.eps)
+        SF._no_tangents("LayerNormNCT", x, self.weight, self.bias)
+        return K.layernorm_nct_fwd(x.contiguous(), self.weight, self.bias, self.eps)       # (bit for bit what the frozen encoder has had)
 
 
 def attach_opaque(root, dotted, shape, buffer=False, dtype=torch.float32):

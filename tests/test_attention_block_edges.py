@@ -251,3 +251,91 @@ def test_forward_mode_is_refused(dev):
                 call()
         assert torch.equal(SF.layer_norm_nct(x, one, None), plain)        # (no tangent in it)
     assert torch.equal(SF.layer_norm_nct(x, one, None), plain)
+
+
+# ---- LayerNorm: statistics, many tiles, many positions ------------------------------------------------------------------------
+@pytest.mark.parametrize("shape", [(1, 64, 40), (2, 256, 37), (1, 400, 9), (1, 1030, 35), (3, 300, 2)])
+@pytest.mark.parametrize("size", [5.0, 30.0, 1000.0])
+def test_layer_norm_nct_one_large_channel(dev, shape, size):
+    """One channel far from the others: the variance is that of centred values, with and without gradients, the same bits in both; and in
+    the module that the frozen encoder holds, which takes moments about channel 0 where that costs less than a factor 32 of half steps."""
+    from neuralsvb_amd.modules.layers import LayerNormNCT
+    B, C, T = shape
+    gen = torch.Generator().manual_seed(71)
+    x = torch.randn(shape, generator=gen)
+    x[:, 0] += size
+    gamma, beta = torch.rand(C, generator=gen) + 0.5, torch.randn(C, generator=gen)
+    want = torch.nn.functional.layer_norm(x.double().transpose(1, 2), (C,), gamma.double(), beta.double(), 1e-5).transpose(1, 2)
+    args = [t.to(dev) for t in (x, gamma, beta)]
+    recorded = SF.layer_norm_nct(args[0].clone().requires_grad_(), *args[1:])
+    # Of the other channels: (x - mu) rs gamma + beta, mu and the sum of squares each off by the half steps of a sum whose terms have one
+    # sign or are dominated by one (8 adds in a lane, 6 + 3 steps between them), of the values they are sums of: mu ~ size / C (at most the
+    # size of the other values times it), rs relative; then three roundings of the result
+    rest = want[:, 1:]
+    n = 32 * U32 * (1 + size / C)
+    for y in (SF.layer_norm_nct(*args), recorded):
+        near(y[:, 1:], rest, n, "other channels")
+        near(y, want, n, "all")
+        assert torch.equal(y, recorded)
+    module = LayerNormNCT(C).to(dev)
+    module.weight.data, module.bias.data = args[1], args[2]
+    with torch.no_grad():
+        y = module(args[0])
+    wide = n + (32 * 4 * U32 if size < 6 else 0.0)                       # (8 half steps of the variance, half of them in rs)
+    near(y[:, 1:], rest, wide, "module, other channels")
+    near(y, want, wide, "module")
+    trained = module(args[0])
+    assert trained.requires_grad and torch.equal(trained, recorded)
+
+
+def _many_tiles(dev, dt, B, C, T):
+    shape = (B, C, T)
+    gen = torch.Generator().manual_seed(C)
+    x = (torch.randn(shape, generator=gen) * 2 + 0.5).to(DT[dt])
+    dy = torch.randn(shape, generator=gen).to(DT[dt])
+    gamma, beta = torch.rand(C, generator=gen) + 0.5, torch.randn(C, generator=gen)
+    lx, lg, lb = leaves64(x, gamma, beta)
+    want = torch.nn.functional.layer_norm(lx.transpose(1, 2), (C,), lg, lb, 1e-5).transpose(1, 2)
+    want.backward(dy.double())
+    got = [t.clone().to(dev).requires_grad_() for t in (x, gamma, beta)]
+    y = SF.layer_norm_nct(*got)
+    y.backward(dy.to(dev))
+    n, unit = 8 * U32 * (math.sqrt(C) + 4), UBF if dt == "bf16" else 0.0           # (as in the tests of one tile)
+    near(y, want.detach(), unit + n, "y")
+    near(got[0].grad, lx.grad, unit + 4 * n, "dx")
+    near(got[1].grad, lg.grad, 8 * U32 * (math.sqrt(C) + math.sqrt(B * T) + 4), "dgamma")
+    near(got[2].grad, lb.grad, 8 * U32 * (math.sqrt(B * T) + 4), "dbeta")
+
+
+# more tiles than the backward has workgroups: sums carried from tile to tile
+@pytest.mark.parametrize("dt,shape", [("f32", (1, 40, 32 * 300 + 5)), ("bf16", (3, 20, 64 * 100 + 9)), ("bf16", (140, 9, 7))])
+def test_layer_norm_nct_many_tiles(dev, dt, shape):
+    _many_tiles(dev, dt, *shape)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt,shape", [("f32", (2, 1030, 32 * 140 + 3)), ("bf16", (2, 1030, 32 * 140 + 3)), ("f32", (1, 600, 16 * 900 + 3)), ("bf16", (1, 1024, 32 * 700 + 1)),
+                                      ("f32", (1, 40, 32 * 1300 + 5)), ("bf16", (3, 300, 64 * 400 + 9)), ("f32", (1000, 70, 5)), ("f32", (1, 3, (1 << 20) + 5)), ("bf16", (1, 3, (1 << 20) + 5))])
+def test_layer_norm_nct_many_tiles_of_every_form(gpu_only, dt, shape):
+    _many_tiles("cuda", dt, *shape)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", ["f32", "bf16"])
+def test_layer_norm_nct_many_entries(gpu_only, dt):
+    """More batch entries than a launch has workgroups."""
+    B, C = (1 << 24) + 77, 4
+    x = torch.randn(B, C, 1, device="cuda", generator=torch.Generator(device="cuda").manual_seed(72)).to(DT[dt])
+    gamma, beta = torch.tensor([1.0, 2.0, -1.0, 0.5], device="cuda"), torch.tensor([0.0, 1.0, 2.0, -3.0], device="cuda")
+    wide = x[:, :, 0].double()                                           # (the library's own form leaves rows beyond 2^24 zero)
+    wide = wide - wide.mean(1, keepdim=True)
+    want = wide / torch.sqrt(wide.square().mean(1, keepdim=True) + 1e-5) * gamma.double() + beta.double()
+    tol = (UBF if dt == "bf16" else 0.0) + 8 * U32 * 6
+    leaves = [x.clone().requires_grad_(), gamma.clone().requires_grad_(), beta.clone().requires_grad_()]
+    y = SF.layer_norm_nct(*leaves)
+    for out in (y, SF.layer_norm_nct(x, gamma, beta)):
+        assert float((out[:, :, 0].detach().double() - want).norm() / want.norm()) <= tol
+        tail = slice(B - 100, B)
+        near(out[tail, :, 0], want[tail].cpu(), tol, "the last entries")
+    y.backward(torch.ones_like(y))
+    near(leaves[2].grad, torch.full((C,), float(B), dtype=torch.float64), 8 * U32 * (math.sqrt(B) + 4), "dbeta")
