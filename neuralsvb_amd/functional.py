@@ -997,7 +997,10 @@ class _BucketAttnFn(torch.autograd.Function):
 
 
 def _time_rows(t):
-    return t if t.dim() != 3 or t.stride(2) == 1 or t.shape[2] <= 1 else t.contiguous()
+    """t as the attention kernels take it: unit time stride, channels at most 2^25 elements apart."""
+    if t.dim() != 3 or ((t.stride(2) == 1 or t.shape[2] <= 1) and (t.stride(1) <= 1 << 25 or t.shape[1] <= 1)):
+        return t
+    return t.contiguous()
 
 
 def bucket_attention(q, k, v, table, buckets, n_head, keep=None, causal=False, scale=None, q_start=None):

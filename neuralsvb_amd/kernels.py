@@ -1166,6 +1166,10 @@ def _bucket_attn_desc(q, k, v, table, buckets, n_head, keep, q_start, causal, sc
     d.q_sb, d.q_sc, q_st = q.stride()
     d.k_sb, d.k_sc, k_st = k.stride()
     d.v_sb, d.v_sc, v_st = v.stride()
+    if D == 1:
+        d.q_sc = 0                                       # (the stride of one element means nothing)
+    if Dk == 1:
+        d.k_sc = d.v_sc = 0
     if (tq > 1 and q_st != 1) or (tk > 1 and (k_st != 1 or v_st != 1)):
         raise ValueError("bucket_attention: q, k, v need unit time stride")
     if keep is not None:

@@ -339,3 +339,30 @@ def test_layer_norm_nct_many_entries(gpu_only, dt):
         near(out[tail, :, 0], want[tail].cpu(), tol, "the last entries")
     y.backward(torch.ones_like(y))
     near(leaves[2].grad, torch.full((C,), float(B), dtype=torch.float64), 8 * U32 * (math.sqrt(B) + 4), "dbeta")
+
+
+# ---- strides and sizes at the limits -------------------------------------------------------------------------------------------
+def test_attention_far_apart_channels(dev):
+    """Channels further apart than the kernels' pitch reaches, and the stride of a dimension of one element, which means nothing."""
+    bk = SF.RelativeBuckets(8, 20)
+    gen = torch.Generator().manual_seed(81)
+    q, k, v = (torch.randn(1, 2, t, generator=gen).to(dev) for t in (5, 9, 9))
+    table = torch.randn(8, 1, generator=gen).to(dev)
+    want = SF.bucket_attention(q, k, v, table, bk, 1)
+    pitch = (1 << 25) + 8
+    room = torch.zeros(pitch + 9, device=dev)
+    far = room.as_strided((1, 2, 9), (1, pitch, 1))
+    far.copy_(k)
+    assert torch.equal(SF.bucket_attention(q, far, v, table, bk, 1), want)
+    leaf = far.detach().requires_grad_()
+    g, = torch.autograd.grad(SF.bucket_attention(q, leaf, v, table, bk, 1).sum(), leaf)
+    leaf = k.clone().requires_grad_()
+    assert torch.equal(g, torch.autograd.grad(SF.bucket_attention(q, leaf, v, table, bk, 1).sum(), leaf)[0])
+    q, k, v = q[:, :1], k[:, :1], v[:, :1]                                # (one channel)
+    want = SF.bucket_attention(q.contiguous(), k.contiguous(), v.contiguous(), table, bk, 1)
+    for strides in ((1 << 40, 1 << 40, 1), (7, 1, 1)):
+        odd = [t.clone().as_strided(t.shape, strides) for t in (q, k, v)]
+        assert torch.equal(SF.bucket_attention(*odd, table, bk, 1), want)
+        odd = [t.requires_grad_() for t in odd]
+        for a, b in zip(torch.autograd.grad(SF.bucket_attention(*odd, table, bk, 1).sum(), odd), odd):
+            assert a.shape == b.shape
