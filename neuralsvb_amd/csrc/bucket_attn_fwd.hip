@@ -609,7 +609,7 @@ static int few_splits(const SvbBucketAttn* a) {
 }
 
 extern "C" size_t svb_bucket_attn_fwd_workspace_floats(const SvbBucketAttn* a) {
-    if (!a || a->B <= 0 || a->H <= 0 || a->Hkv <= 0 || a->Tq <= 0 || a->Tk <= 0 || a->dk <= 0) return 0;
+    if (svb_bucket_attn_check(a) != SVB_OK) return 0;                    // (sizes whose products below fit their types)
     const int n = few_splits(a);
     return n > 1 ? (size_t)a->B * a->H * a->Tq * n * (a->dk + 2) : 0;
 }

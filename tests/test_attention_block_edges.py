@@ -366,3 +366,18 @@ def test_attention_far_apart_channels(dev):
         odd = [t.requires_grad_() for t in odd]
         for a, b in zip(torch.autograd.grad(SF.bucket_attention(*odd, table, bk, 1).sum(), odd), odd):
             assert a.shape == b.shape
+
+
+def test_attention_workspace_of_a_refused_call(_emu_lib):
+    """Sizes that the forward refuses need no workspace, whatever their product is."""
+    from neuralsvb_amd import _lib as L
+    lib = _emu_lib
+    a = L.SvbBucketAttn()
+    a.q = a.k = a.v = a.table = a.out = 16                                # (never read)
+    a.buckets = SF.RelativeBuckets(8, 20).c
+    a.dk, a.Tq, a.Tk, a.scale = 1, 1, 1000, 1.0
+    a.B, a.H, a.Hkv = 2, 2, 2
+    assert lib.svb_bucket_attn_fwd_workspace_floats(L.C.byref(a)) > 0
+    a.B = a.H = a.Hkv = 65535
+    assert lib.svb_bucket_attn_fwd_workspace_floats(L.C.byref(a)) == 0
+    assert lib.svb_bucket_attn_bwd_workspace_floats(L.C.byref(a)) == 0
