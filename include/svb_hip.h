@@ -17,7 +17,7 @@
 extern "C" {
 #endif
 
-#define SVB_ABI_VERSION 10
+#define SVB_ABI_VERSION 11
 int svb_abi_version(void);
 
 /* ---- fused conv epilogue / prologue description ------------------------------------------------------
@@ -591,11 +591,11 @@ int svb_bucket_bias_bwd(const void* dbias, void* dtable, const SvbRelBuckets* bu
 /* ---- attention with that bias inside ----
  * out[b][h dk + d][i] = sum_j softmax_j(scale q_i . k_j + table[bucket(j - p_i)][h]) v_j[d],   p_i = start + i,
  * start = q_start_b[b] where that is given, else q_start.  Keys j with keep[b][j] == 0, and with `causal` those with j > p_i, are
- * hidden: what K and V hold there has no influence.  A query that sees no key gets zeros and passes no gradient.
+ * hidden: what K and V hold there has no influence on that query.  A query that sees no key gets zeros and passes no gradient.
  * Shared heads: H query heads use Hkv key / value heads, query head h reads head h / (H / Hkv).
  * q [B][H dk][Tq], k, v [B][Hkv dk][Tk]: unit time stride, any batch stride, channel stride 0 ... 2^25 (elements).  dk <= 128.
  * out, dout, dq [B][H dk][Tq], dk, dv [B][Hkv dk][Tk] contiguous.  table, dtable [n_buckets][H] (table_dtype).
- * Training: stats [2][B][H][Tq] (each query's maximum in log2 units, +infinity where it sees no key, and the reciprocal of its sum)
+ * Training (ABI v11): stats [2][B][H][Tq] (each query's maximum in log2 units, +infinity where it sees no key, and the reciprocal of its sum)
  * and out_f32 (bf16 tensors only: out before its rounding, [B][H dk][Tq]) are written by the forward and read by the backward; both
  * NULL for inference.                                                                                                             */
 typedef struct SvbBucketAttn {
