@@ -426,7 +426,8 @@ __device__ __forceinline__ int svbt_keep_end(const float* keep, int n, int lane)
 }
 // (group, tile) of workgroup `id` of groups x tiles.  A group's workgroups read the same keys or queries, so they belong on one XCD
 // (workgroups go round the 8 in turn).  LONG_FIRST: tile 0 of every group is the longest, the last is short; a group's tiles one after the
-// other would leave the long ones of the last groups to the end (B2 H16 dk128 T2048 causal, dk and dv: 364 us that way, 250 this way).
+// other would leave the long ones of the last groups to the end (B2 H16 dk128 T2048 causal, dk and dv as they were then: 364 us that way, 250
+// this way; 169 with the steps since).
 __device__ __forceinline__ void svbt_item(int id, int groups, int tiles, bool long_first, int& group, int& tile) {
     if (long_first) {
         if ((groups & 7) == 0) {                                         // the groups of this XCD, tile by tile

@@ -13,8 +13,8 @@
 // forward keeps the output in fp32 for bf16 tensors.  P and dS are rounded to bf16 as operands for bf16 tensors (relative 2^-8 each at most,
 // averaged over the sum), and cut into three parts for fp32 tensors; dtable sums dS in fp32 before any rounding.
 // Bound, as the forward, by what a wave does between its products, and in the second kernel by one wave per SIMD above dk 64 (its two sums
-// take 128 registers of each lane at dk 128): B2 H16/4 dk128 T2048 causal bf16 170 us (dq: three products, 303 TFLOP/s) and 170 us (dk, dv:
-// four, 404 TFLOP/s); B32 H4 dk64 T562 fp32 150 and 230 us (620 and 540 TFLOP/s of bf16 products).
+// take 128 registers of each lane at dk 128): B2 H16/4 dk128 T2048 causal bf16 154 to 160 us (dq: three products, 330 TFLOP/s) and 169 us (dk,
+// dv: four, 407 TFLOP/s); B32 H4 dk64 T562 fp32 164 and 241 us (569 and 516 TFLOP/s of bf16 products).
 // P comes from the forward's maximum and sum as the forward had it: of a row with nearly all its weight on one key, dS of that key is what
 // the others' small weights leave.  Where 32 bits hold nothing of them (l == 1: P == 1) its dS is 0, dP - delta being rounding noise alone.
 //
@@ -78,7 +78,8 @@ __device__ __forceinline__ void svbt_weights_q(f32x16& s, const f32x16& dp, floa
 // ---- dq, dtable, delta: 4 waves x 32 queries, keys staged ----------------------------------------------------------------------------
 template <typename T, int DKP, int KT, bool DOUBLE, bool TINY>
 __global__ __launch_bounds__(256, SvbtParts<T>::NS == 1 || DKP <= 64 ? 2 : 1) void svb_bucket_attn_dq_kernel(SvbBucketAttn a, SvbBattnBwd g, int qtiles) {
-    // (FRESH: B2 H16/4 dk128 T2048 causal bf16 171 -> 158 us, B32 H4 dk64 T562 fp32 169 -> 156; elsewhere it costs 1 to 3 %)
+    // (FRESH, both ways in one build: B2 H16/4 dk128 T2048 causal bf16 171 -> 158 us, B32 H4 dk64 T562 fp32 169 -> 156; elsewhere it costs
+    // 1 to 3 %)
     typedef SvbtTile<T, DKP, KT, 256, TINY, DKP == 128 || (SvbtParts<T>::NS == 3 && DKP == 64)> Tile;
     constexpr int NS = Tile::NS, NK = DKP / 16, NDB = DKP / 32, NSUB = KT / 32;
     constexpr int BUF = NS * (2 * Tile::ROWS_BYTES + Tile::COLS_BYTES);

@@ -12,9 +12,9 @@
 // The bias of a pair is that of its diagonal: a head's table is expanded to one value per offset in LDS.  A tile of keys that lies
 // further than the last bucket border from all queries of a wave has one bias for all its pairs and reads none.
 //
-// Bound by what a wave does between its products (B2 H16/4 dk128 T2048 causal bf16: 83 us, 413 TFLOP/s; in training 110 us, with P V in
-// three parts 626 TFLOP/s issued; B2 H8 dk64 T2000 causal: 35 us, 234 TFLOP/s, 256 workgroups' longest chain of 16 tiles; B32 H4 dk64 T562
-// fp32: 100 us, 620 TFLOP/s of bf16 products): a 32 x 32 sub-tile is 512 ticks of the matrix core at dk 128 and about as many of
+// Bound by what a wave does between its products (kernel times; B2 H16/4 dk128 T2048 causal bf16: 89 us, 386 TFLOP/s; in training 118 us,
+// with P V in three parts 582 TFLOP/s issued; B2 H8 dk64 T2000 causal: 38 us, 213 TFLOP/s, 512 workgroups at once, the longest with a chain of
+// 16 tiles of 128 keys; B32 H4 dk64 T562 fp32: 104 us, 597 TFLOP/s of bf16 products): a 32 x 32 sub-tile is 512 ticks of the matrix core at dk 128 and about as many of
 // exponentials, sums and roundings, one after the other, and two workgroups share a CU.
 #include "attn_tiles.h"
 #include <type_traits>
@@ -71,7 +71,7 @@ __device__ __forceinline__ void svbt_softmax(f32x16 (&s)[NSUB], SvbtState<NDB>& 
 // PP: parts of P.  KG: the waves are 4 / KG groups of 32 queries, each tile's keys are split over KG waves, which join at the end.
 template <typename T, int DKP, int KT, bool DOUBLE, int PP, int KG, bool TINY>
 __global__ __launch_bounds__(256, SvbtParts<T>::NS == 3 && DKP == 128 ? 1 : 2) void svb_bucket_attn_fwd_kernel(SvbBucketAttn a, int qtiles) {
-    // (FRESH, B2 H16/4 dk128 T2048 causal bf16: 104 -> 84 us, training 134 -> 112; to dk 64 it costs 3 %)
+    // (FRESH, both ways in one build: B2 H16/4 dk128 T2048 causal bf16 104 -> 84 us, training 134 -> 112; to dk 64 it costs 3 %)
     typedef SvbtTile<T, DKP, KT, 256, TINY, DKP == 128> Tile;
     constexpr int NS = Tile::NS, NK = DKP / 16, NDB = DKP / 32, NSUB = KT / 32 / KG, QW = 4 / KG;
     constexpr int BUF = NS * (Tile::ROWS_BYTES + Tile::COLS_BYTES);
@@ -269,7 +269,7 @@ __global__ __launch_bounds__(256, SvbtParts<T>::NS == 3 && DKP == 128 ? 1 : 2) v
 //      interleaved, are the eight consecutive keys 16 g + 8 kb + 0..7
 //   V: 16 bytes of consecutive keys of a channel per lane, in just that order.
 // Waves join in LDS, workgroups in a second launch from [split][row] parts (m, l, sum of P v) in memory, in order.
-// 16 requests, H16/4 dk64, caches of 8192 filled to three quarters on average (101 MB): 26 to 29 us, 3.7 TB/s, and 6 us for the join.
+// 16 requests, H16/4 dk64, caches of 8192 filled to three quarters on average (101 MB): 26 to 29 us, 3.5 TB/s, and 6 us for the join.
 struct SvbFewParts {
     float *o, *ml;                 // [item][split][rows][dk], [item][split][rows][2]; NULL: one split, out is written
     int splits;
@@ -658,8 +658,8 @@ extern "C" int svb_bucket_attn_fwd(const SvbBucketAttn* call, float* ws, void* s
          : a->dk <= 96 ? fwd_launch<T, 96, KT, D96, PP, KG>(a, st) : fwd_launch<T, 128, KT, true, PP, KG>(a, st)
     if (a->dtype == SVB_DT_F32) SVB_FWD_GO(float, 32, 32, 3, false, 1);
     // At most one workgroup of 128 queries per CU and several tiles of keys: workgroups of 64 queries, twice as many, the keys of a tile over
-    // two waves, tiles of 128 keys up to dk 64.  B2 H8 dk64 T2000 causal (256 workgroups): 52 -> 41 us, training 72 -> 48 (35 and 44 with the steps since); B4 H8 dk96 T1000
-    // causal: 38 -> 34; B24 H4 dk48 T211, where a join and a bigger tile save nothing: 14.5 -> 16.5.  Between one and two workgroups per CU
+    // two waves, tiles of 128 keys up to dk 64.  Both ways in one build: B2 H8 dk64 T2000 causal (256 workgroups become 512) 52 -> 41 us,
+    // training 72 -> 48 (38 and 47 with the steps since); B4 H8 dk96 T1000 causal: 38 -> 34; B24 H4 dk48 T211, where a join and a bigger tile save nothing: 14.5 -> 16.5.  Between one and two workgroups per CU
     // (B7 H8 dk64 T1100 causal) the forward takes 39 us this way instead of 36.  fp32 tensors have six products per tile to wait behind.
     const bool thin = a->Tk > 256 && (long)a->B * a->H * ((a->Tq + 127) / 128) <= 256;
     if (a->stats && thin) SVB_FWD_GO(unsigned short, 128, 64, 3, true, 2);

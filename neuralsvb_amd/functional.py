@@ -912,7 +912,10 @@ def layer_norm_nct(x, gamma, beta, eps=1e-5):
     if x.dim() != 3:
         raise ValueError(f"layer_norm_nct: x must be [B, C, T], got {tuple(x.shape)}")
     _no_tangents("layer_norm_nct", x, gamma, beta)
-    gamma, beta = (p if p is None or p.dim() == 1 else p.reshape(-1) for p in (gamma, beta))
+    if gamma is not None and gamma.dim() != 1:
+        gamma = gamma.reshape(-1)
+    if beta is not None and beta.dim() != 1:
+        beta = beta.reshape(-1)
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, gamma, beta)):
         return _LayerNormNCTFn.apply(x, gamma, beta, float(eps))
     return K.ln_nct_fwd(_c(x), _c(gamma), _c(beta), float(eps))
@@ -1008,16 +1011,21 @@ def bucket_attention(q, k, v, table, buckets, n_head, keep=None, causal=False, s
 
     q [B, H dk, Tq], k, v [B, Hkv dk, Tk] (float32 or bfloat16; any batch and channel strides, e.g. slices of one projection),
     H = n_head a multiple of Hkv: query head h reads key / value head h // (H / Hkv).  dk <= 128.  table [n_buckets, H], float32 or
-    bfloat16.  keep [B, Tk] float32: 0 hides a key, and whatever k and v hold there has no influence.  causal: a query sees the keys
-    up to its own position, and whatever k and v hold at later ones has no influence on it.  scale: 1 / sqrt(dk).  q_start: position of query 0 among the keys, an int or an int32 tensor [B] (default
-    Tk - Tq); with causal=True and Tq = 1 a tensor of cached lengths - 1 serves one new token per request from caches of one capacity.
-    A query that sees no key gives zeros and no gradient.  -> [B, H dk, Tq].
+    bfloat16.  keep [B, Tk] float32: 0 hides a key.  causal: a query sees the keys up to its own position.  Whatever k and v hold where
+    they are hidden from a query has no influence on it.  scale: 1 / sqrt(dk).  q_start: position of query 0 among the keys, an int or an
+    int32 tensor [B] (default Tk - Tq); with causal=True and Tq = 1 a tensor of cached lengths - 1 serves one new token per request from
+    caches of one capacity.  A query that sees no key gives zeros and no gradient.  -> [B, H dk, Tq].
 
-    Table entries of -inf, or so low that log2(e) times them is (the type's lowest value), hide the pairs of their bucket.  q and dout are
-    finite in rows that see a key.  The leaves of a backward pass that is captured into a graph belong to that graph alone: an eager graph
-    of the same leaves that still lives ties their gradients to its stream, which ends the capture (and the process with it).
+    Table entries of -inf, or so low that log2(e) times them is (the type's lowest value), give the pairs of their bucket no weight; k and v
+    are finite there.  q and dout are finite in rows that see a key.  A NaN in k or v reaches the queries that see it and their gradients;
+    so does an infinity, which float32 tensors may turn into NaN (as values beyond the largest bfloat16, 3.39e38).  The leaves of a backward
+    pass that is captured into a graph belong to that graph alone: an eager graph of the same leaves that still lives ties their gradients
+    to its stream, which ends the capture (and the process with it).
 
-    float32 tensors are multiplied in three bf16 parts whatever `conv_precision` says (as the rel-pos attention of the fp32 mode)."""
+    Arithmetic: scores, softmax, sums and the table's gradient are float32.  float32 tensors are multiplied in three bf16 parts (2^-24)
+    whatever `conv_precision` says (as the rel-pos attention of the fp32 mode).  bfloat16 tensors: the weights are rounded to bfloat16
+    (2^-8 each) before they multiply v, in the backward pass P and dS as well; recorded calls keep the output in float32 beside the
+    rounded one, for the table's gradient."""
     n_head = int(n_head)
     if n_head < 1:
         raise ValueError(f"bucket_attention: n_head = {n_head}")
