@@ -3,7 +3,7 @@
 //   bias[h][i][j] = table[bucket(j - i - start)][h],      dtable[k][h] = sum of dbias[h][i][j] over bucket(j - i - start) == k
 //
 // Both are HBM-bound: the forward writes, the backward reads H Tq Tk elements once (8 x 2048 x 2051 fp32, 134 MB: 24 us, 5.6 TB/s, and
-// 45 us, 3.0 TB/s; 4 x 562 x 562: 8 and 9 us, the time of a launch).  The bias of a pair depends on its diagonal
+// 45 us, 3.0 TB/s, and 8 us for the sums; 4 x 562 x 562: 7, 9 and 3 us, the time of a launch).  The bias of a pair depends on its diagonal
 // alone.  Forward: a workgroup expands its head's table to one value per offset (constant beyond the last bucket border) in LDS and
 // writes rows from it.  Backward: a thread owns offsets, not columns -- it walks down the rows along its diagonals, lanes side by
 // side, so that the loads are contiguous and the sums stay in its registers without a scatter; then the diagonals of a bucket are

@@ -6,8 +6,8 @@
 // positions of their neighbours, bit for bit -- same loads, same order of sums, same stores --, and count `skip` of them out of the
 // affine sums.  No access needs a tail.
 //
-// HBM-bound: forward reads and writes x once, backward reads x and dy and writes dx (32 x 1024 x 2048 bf16: forward 64 us, 4.2 TB/s;
-// backward 150 us, 2.7 TB/s; 32 x 512 x 700 fp32: 17 us and 38 us).  A workgroup owns whole columns, so it has to
+// HBM-bound: forward reads and writes x once, backward reads x and dy and writes dx (32 x 1024 x 2048 bf16: forward 66 us, 4.1 TB/s;
+// backward 145 us, 2.8 TB/s, and 5 us for the sums; 32 x 512 x 700 fp32: 23 us, and 31 + 4 us).  A workgroup owns whole columns, so it has to
 // hold C values of each: LPR lanes side by side along time take VEC values (16 bytes) each, NT / LPR rows of them cover that many
 // channels at once, and P such passes stay in registers -- all loads of a tile are in flight together and nothing is read twice.
 // Sums over channels: in-lane over the passes, lanes of a wave by shuffles, waves through LDS; variance from centred values.
@@ -18,7 +18,7 @@
 #include <svb_opaque.h>
 
 /* workgroups of the backward that walk tiles: one per CU.  With two of them dx waits for a second round of loads on each CU and the affine
-   sums have twice the rows: 32 x 512 x 700 fp32 46 us instead of 38, 32 x 1024 x 2048 bf16 159 instead of 150 */
+   sums have twice the rows: both launches of 32 x 512 x 700 fp32 46 us instead of 38, of 32 x 1024 x 2048 bf16 159 instead of 150 */
 #define SVB_LN_MAX_WG 256
 
 typedef float svbl_f4 __attribute__((ext_vector_type(4), aligned(4)));
@@ -272,7 +272,7 @@ __global__ __launch_bounds__(NT) void svb_ln_nct_bwd_kernel(SvbLnArgs a) {
 
 // More channels (or longer rows) than the register form takes: 32 positions x G channel groups, values read again for each use (they come
 // from L2).  The forward is a chain of C / G loads in each of its three passes: 32 groups where there are channels for them
-// (4 x 1500 x 700 fp32 207 us with 8 groups).
+// (4 x 1500 x 700 fp32 66 us, 207 with 8 groups).
 template <typename T, int G>
 __global__ __launch_bounds__(32 * G) void svb_ln_nct_fwd_wide_kernel(SvbLnArgs a) {
     __shared__ float red[2][G][32];
